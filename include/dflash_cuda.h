@@ -225,6 +225,79 @@ int32_t dflash_kv_append(const void* k_new, const void* v_new, void* k_cache, vo
 int32_t dflash_kv_commit(int32_t* kv_len, const int32_t* commit, int32_t B, int32_t T, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * The KV cache outside the verify cycle: plain decoding, prompts, and cutting a cache to a budget.
+ * The reference leaves these to its model library (the attention over its growing arrays) and to the
+ * draft model's sink-and-window context cache (64 leading tokens and the last 1024 stay visible,
+ * Sources/DFlash/DFlashDraftModel.swift:107-147); here they read the cache dflash_kv_append writes.
+ *
+ * Shared conventions.
+ *   k, v       dense [B,Hkv,N,D], or with page_table a pool [num_pages,Hkv,page_tokens,D] as for
+ *              dflash_verify_sdpa, here with page_tokens any multiple of 16.  With a page table N is an upper bound
+ *              of the lengths (<= max_pages * page_tokens).  A page id outside the pool reads as zeros and
+ *              is reported through dflash_device_status.
+ *   kv_len     int32[B] or NULL (N each): cached tokens of sequence b, the queries' own tokens among them.
+ *   q_len      int32[B] or NULL (T each): query rows of sequence b that are in use.  Rows behind them are neither
+ *              read nor written (out, lse).
+ *              Entries outside [0,N] and [0,T] are clamped to that range and reported (DFLASH_ERR_DEVICE_DATA).
+ *   visibility query row r of sequence b stands at position p = kv_len[b] - q_len[b] + r and sees token n iff
+ *              n <= p and (window == 0 or n > p - window or n < sinks).  window counts the query's own
+ *              token.  A row that sees nothing has out = 0 and lse = -infinity.
+ *   values     K and V rows [0, kv_len[b]) are finite; rows behind them are never used, whatever they hold.
+ *   lse        fp32, natural logarithm of the sum of exp(scale * q.k) over the visible tokens.
+ *   mass       fp32 [B,Hkv,mass_stride], mass_stride >= N: the weight every cached token has received, summed over
+ *              the query heads of its KV head.  Always added to, in an order that does not change from run to run.
+ *   Supported: dtype bf16 / f16, D in {64, 128, 256}, Hq % Hkv == 0.  Neither outputs nor workspace may overlap
+ *   another argument unless it is said.
+ */
+
+/* Attention of one new token per sequence (the last cached one):  q, out [B,Hq,D];  lse [B,Hq] or NULL;
+ * mass or NULL: mass[b,h,n] += sum over the query heads of h of their weight on token n.  kv_len[b] == 0 (an unused
+ * place of a batch) gives out = 0, lse = -infinity. */
+int32_t dflash_decode_sdpa(const void* q, const void* k, const void* v, const int32_t* page_table,
+                           const int32_t* kv_len, void* out, float* lse, float* mass, void* workspace,
+                           size_t workspace_bytes, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t N,
+                           int32_t page_tokens, int32_t max_pages, int32_t num_pages, int32_t mass_stride,
+                           int32_t window, int32_t sinks, float scale, int32_t dtype, void* stream);
+size_t dflash_decode_sdpa_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t N, int32_t window,
+                                          int32_t sinks, int32_t with_mass);
+
+/* Attention of a prompt or a chunk of one:  q, out [B,Hq,T,D];  lse [B,Hq,T] or NULL.  The chunk's own keys and
+ * values are in the cache already (dflash_kv_append first). */
+int32_t dflash_prompt_sdpa(const void* q, const void* k, const void* v, const int32_t* page_table,
+                           const int32_t* q_len, const int32_t* kv_len, void* out, float* lse, void* workspace,
+                           size_t workspace_bytes, int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t D, int32_t N,
+                           int32_t page_tokens, int32_t max_pages, int32_t num_pages, int32_t window, int32_t sinks,
+                           float scale, int32_t dtype, void* stream);
+size_t dflash_prompt_sdpa_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t D, int32_t N);
+
+/* mass[b,h,n] += sum over query rows r and query heads of h of exp(scale * q.k - lse) on the tokens the rows see,
+ * with the lse [B,Hq,T] of an attention over the same cache (a row whose lse is -infinity adds nothing). */
+int32_t dflash_attention_mass(const void* q, const void* k, const int32_t* page_table, const int32_t* q_len,
+                              const int32_t* kv_len, const float* lse, float* mass, void* workspace,
+                              size_t workspace_bytes, int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t D, int32_t N,
+                              int32_t page_tokens, int32_t max_pages, int32_t num_pages, int32_t mass_stride,
+                              int32_t window, int32_t sinks, float scale, int32_t dtype, void* stream);
+size_t dflash_attention_mass_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t D, int32_t N);
+
+/* Cuts every sequence longer than `budget` tokens down to `budget`, per KV head: the first `sinks` tokens, the last
+ * `recent` and, of the others, those with the largest mass stay (equal masses: the lower index; a NaN counts as
+ * larger than every number).  The rows that stay move to the front in place, in the order they are in; rows
+ * [budget, kv_len) keep what they hold.  sinks + recent <= budget.
+ *   kv_len_out int32[B]: min(kv_len, budget); may be kv_len itself.
+ *   mass_out   fp32, laid out as mass and possibly mass itself: the masses of the rows that stay, then zeros up to the
+ *              old length; nothing behind it is written.
+ *   kept       int32 [B,Hkv,budget] or NULL: the old place of each row that stays, ascending; -1 behind the last.
+ * k_cache / v_cache rows of any dtype of dflash_kv_append with D * size a multiple of 16 bytes; page_tokens any
+ * positive number.  The pages of a sequence that is cut must belong to it alone (a page shared with another
+ * sequence would change under it).  Rows on a page outside the pool are skipped and reported. */
+int32_t dflash_kv_evict(void* k_cache, void* v_cache, const int32_t* page_table, const int32_t* kv_len, const float* mass,
+                        int32_t* kv_len_out, float* mass_out, int32_t* kept, void* workspace, size_t workspace_bytes,
+                        int32_t B, int32_t Hkv, int32_t D, int32_t N, int32_t page_tokens, int32_t max_pages,
+                        int32_t num_pages, int32_t mass_stride, int32_t budget, int32_t recent, int32_t sinks,
+                        int32_t dtype, void* stream);
+size_t dflash_kv_evict_workspace_bytes(int32_t B, int32_t Hkv, int32_t N, int32_t budget);
+
+/* ---------------------------------------------------------------------------------------------
  * TurboQuant 3-bit KV codec, 128-dimension blocks (a 256-dimension head vector is two blocks).
  * Follows the codec as stated in the reference's tests/test_turbo_quant.cpp: V path :69-75, K path
  * with residual sign bits :85-98, primitives :14-22 (the production encoder lives in a dependency

@@ -32,6 +32,14 @@ SIGNATURES = {
     "dflash_rebuild_conv_state": (_i32, [_vp, _vp, _vp, _i32, _vp, _i32, _i32, _i32, C.c_int64, C.POINTER(_i32), _vp]),
     "dflash_kv_append": (_i32, [_vp] * 6 + [_i32, _vp] + [_i32] * 9 + [_vp]),
     "dflash_kv_commit": (_i32, [_vp, _vp, _i32, _i32, _vp]),
+    "dflash_decode_sdpa": (_i32, [_vp] * 9 + [_sz] + [_i32] * 11 + [_f32, _i32, _vp]),
+    "dflash_decode_sdpa_workspace_bytes": (_sz, [_i32] * 8),
+    "dflash_prompt_sdpa": (_i32, [_vp] * 9 + [_sz] + [_i32] * 11 + [_f32, _i32, _vp]),
+    "dflash_prompt_sdpa_workspace_bytes": (_sz, [_i32] * 6),
+    "dflash_attention_mass": (_i32, [_vp] * 8 + [_sz] + [_i32] * 12 + [_f32, _i32, _vp]),
+    "dflash_attention_mass_workspace_bytes": (_sz, [_i32] * 6),
+    "dflash_kv_evict": (_i32, [_vp] * 9 + [_sz] + [_i32] * 12 + [_vp]),
+    "dflash_kv_evict_workspace_bytes": (_sz, [_i32] * 4),
     "dflash_turbo_encode": (_i32, [_vp] * 5 + [C.c_int64, _i32, _i32, _vp]),
     "dflash_turbo_decode": (_i32, [_vp] * 5 + [C.c_int64, _i32, _i32, _vp]),
     "dflash_verify_step_workspace_bytes": (_sz, [_vp]),

@@ -345,12 +345,16 @@ int32_t dflash_device_status(void* stream) {
     DFLASH_CUDA_CHECK(cudaStreamSynchronize(s));
     switch (host) {
       case kStatusKvRange:
-        set_error("a KV position beyond the cache's capacity, or a page id outside the pool: kv_append skipped the row / "
-                  "verify_sdpa read the page as zeros");
+        set_error("a KV position beyond the cache's capacity, or a page id outside the pool: kv_append / kv_evict skipped the row, "
+                  "the attention kernels read the page as zeros");
         return DFLASH_ERR_DEVICE_DATA;
       case kStatusKvLen:
         set_error("verify_sdpa: a kv_len_per_seq entry outside [16, N] was clamped; that sequence's output is not the attention "
                   "over its keys (no output at all for a length <= 0)");
+        return DFLASH_ERR_DEVICE_DATA;
+      case kStatusCacheLen:
+        set_error("decode_sdpa / prompt_sdpa / attention_mass / kv_evict: a kv_len entry outside [0, N] or a q_len entry outside "
+                  "[0, T] was clamped");
         return DFLASH_ERR_DEVICE_DATA;
       case kStatusMergeRanges:
         set_error("verify_sdpa: a unit was cut into more key ranges than the merge kernel takes; its output is incomplete");

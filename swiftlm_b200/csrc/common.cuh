@@ -32,6 +32,7 @@ enum DeviceStatusCode : int {
   kStatusSelftestWait = 8,   // dflash_selftest_bounded_wait: the wait that nothing satisfies gave up (as it must)
   kStatusKvRange = 16,       // a KV position beyond the capacity, or a page id outside the pool
   kStatusKvLen = 17,         // attention: a kv_len_per_seq entry outside [16, N] (clamped)
+  kStatusCacheLen = 18,      // cache operators: a kv_len entry outside [0, N] or a q_len entry outside [0, T] (clamped)
 };
 
 #define DFLASH_CUDA_CHECK(expr)                                                          \

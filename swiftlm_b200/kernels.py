@@ -11,6 +11,7 @@ from __future__ import annotations
 
 from typing import Optional, Tuple
 
+import contextlib
 import ctypes as C
 
 import torch
@@ -266,6 +267,220 @@ def kv_commit(kv_len, commit, block: int = 16) -> None:
     """kv_len[b] += clamp(commit[b], 0, block): keeps the accepted prefix of the block just appended and
     leaves the rejected rows to be overwritten (the reference's cache.trim(offset - targetLen))."""
     _lib.check(_lib.lib().dflash_kv_commit(_ptr(kv_len), _ptr(commit), kv_len.numel(), int(block), _stream()))
+
+
+# ---- the cache outside the verify cycle: plain decoding, prompts, eviction (no counterpart among the reference's kernels) ----
+
+def _bad(what: str):
+    return _lib.DFlashError(_lib.ERR_INVALID_ARG, what)
+
+
+def _on_device_of(t: torch.Tensor):
+    """The tensor's device made current for a call (allocation, stream and launch all go to it)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _same_device(first: torch.Tensor, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise _bad(f"tensors on different devices: {first.device} and {t.device}")
+
+
+def _int_vector(x, n: int, device, name: str):
+    if x is None:
+        return None
+    if not (isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.device == device and x.is_contiguous()):
+        x = torch.as_tensor(x, device=device).to(torch.int32).contiguous()
+    if x.shape != (n,):
+        raise _bad(f"{name} must have one entry per sequence")
+    return x
+
+
+def _cache_shape(keys, page_table, n_max, B: int):
+    """(page_table as the kernels take it, N, page_tokens, max_pages, num_pages) of a dense cache [B,Hkv,capacity,D] or of a
+    page pool [num_pages,Hkv,page_tokens,D]."""
+    if page_table is None:
+        if keys.shape[0] != B:
+            raise _bad("a dense cache has one entry per sequence")
+        return None, keys.shape[2], 0, 0, 0
+    if page_table.dim() != 2 or page_table.shape[0] != B:
+        raise _bad("page_table must be [B, max_pages]")
+    if page_table.dtype != torch.int32 or not page_table.is_contiguous():
+        page_table = page_table.to(torch.int32).contiguous()
+    capacity = page_table.shape[1] * keys.shape[2]
+    return page_table, (capacity if n_max is None else min(int(n_max), capacity)), keys.shape[2], page_table.shape[1], keys.shape[0]
+
+
+def _cache_tensors(queries, keys, values):
+    _need_cuda(queries, keys, values)
+    _same_device(queries, keys, values)
+    if keys.dim() != 4 or (values is not None and values.shape != keys.shape):
+        raise _bad("keys and values must be two 4-dimensional tensors of one shape")
+    if queries.shape[-1] != keys.shape[3]:
+        raise _bad("queries and keys have different head dimensions")
+    if keys.dtype != queries.dtype or (values is not None and values.dtype != queries.dtype):
+        raise _lib.DFlashUnsupported(_lib.ERR_UNSUPPORTED, "queries, keys and values must have one dtype")
+    if queries.dtype not in (torch.bfloat16, torch.float16):
+        raise _lib.DFlashUnsupported(_lib.ERR_UNSUPPORTED, f"dtype {queries.dtype} (bf16 or f16)")
+
+
+def _mass_arg(mass, B: int, Hkv: int, N: int, name: str = "mass"):
+    if mass.dtype != torch.float32 or mass.dim() != 3 or mass.shape[:2] != (B, Hkv) or mass.shape[2] < N or not mass.is_contiguous():
+        raise _bad(f"{name} must be a contiguous fp32 tensor [B, Hkv, >= {N}]")
+    return mass
+
+
+def _out_arg(out, like: torch.Tensor, name: str = "out"):
+    if out is None:
+        return torch.empty_like(like)
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device or not out.is_contiguous():
+        raise _bad(f"{name} must be a contiguous tensor of the queries' shape, dtype and device")
+    return out
+
+
+def _scratch(nbytes: int, device) -> Optional[torch.Tensor]:
+    """Workspace of one call.  Taken from torch's allocator call by call, so that calls on several streams and calls captured
+    into different CUDA graphs never share one."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def decode_sdpa(queries, keys, values, scale: float, kv_len=None, page_table=None, window: int = 0, sinks: int = 0,
+                mass: Optional[torch.Tensor] = None, return_lse: bool = False, out=None, n_max=None):
+    """Attention of one new token per sequence over its cache, the new token being the last cached one.
+
+    queries [B,Hq,D]; keys/values a dense cache [B,Hkv,capacity,D] or, with page_table int32 [B,max_pages], page pools
+    [num_pages,Hkv,page_tokens,D] (page_tokens a multiple of 16); kv_len int32 [B]: cached tokens (0 for an unused place:
+    its output is 0).  window > 0: the last `window` tokens are visible, and the first `sinks`.  mass fp32
+    [B,Hkv,>= capacity]: the weight of every visible token, summed over the query heads of its KV head, is added to
+    it.  n_max: an upper bound of kv_len for a page pool, when less than the table's reach is in use.
+    Returns [B,Hq,D], or (that, lse fp32 [B,Hq]) with return_lse.
+    """
+    _cache_tensors(queries, keys, values)
+    if queries.dim() != 3:
+        raise _bad("queries must be [B, Hq, D]")
+    B, Hq, D = queries.shape
+    Hkv = keys.shape[1]
+    _same_device(queries, page_table, mass, out)
+    page_table, N, page_tokens, max_pages, num_pages = _cache_shape(keys, page_table, n_max, B)
+    if mass is not None:
+        _mass_arg(mass, B, Hkv, N)
+    with _on_device_of(queries):
+        q, k, v = queries.contiguous(), keys.contiguous(), values.contiguous()
+        kv_len = _int_vector(kv_len, B, q.device, "kv_len")
+        out = _out_arg(out, q)
+        lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+        L = _lib.lib()
+        ws = _scratch(L.dflash_decode_sdpa_workspace_bytes(B, Hq, Hkv, D, N, int(window), int(sinks), int(mass is not None)), q.device)
+        _lib.check(L.dflash_decode_sdpa(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(page_table), _ptr(kv_len), _ptr(out), _ptr(lse), _ptr(mass), _ptr(ws),
+            0 if ws is None else ws.numel(), B, Hq, Hkv, D, N, page_tokens, max_pages, num_pages,
+            0 if mass is None else mass.shape[2], int(window), int(sinks), float(scale), _DT[q.dtype], _stream()))
+    return (out, lse) if return_lse else out
+
+
+def prompt_sdpa(queries, keys, values, scale: float, q_len=None, kv_len=None, page_table=None, window: int = 0, sinks: int = 0,
+                return_lse: bool = False, out=None, n_max=None):
+    """Attention of a prompt, or of a chunk of one behind what the cache holds already, with the chunk's own rows in the
+    cache (append first).
+
+    queries [B,Hq,T,D]; keys/values, kv_len, page_table, window, sinks, n_max as for decode_sdpa.  q_len int32 [B]: query
+    rows in use (default T); row r of sequence b stands at position kv_len[b] - q_len[b] + r and sees the tokens up to its
+    own, within the window or among the sinks.  Rows at and behind q_len[b] are left as they are in `out`.
+    Returns [B,Hq,T,D], or (that, lse fp32 [B,Hq,T]) with return_lse (-inf on rows that see nothing or are not in use).
+    """
+    _cache_tensors(queries, keys, values)
+    if queries.dim() != 4:
+        raise _bad("queries must be [B, Hq, T, D]")
+    B, Hq, T, D = queries.shape
+    Hkv = keys.shape[1]
+    _same_device(queries, page_table, out)
+    page_table, N, page_tokens, max_pages, num_pages = _cache_shape(keys, page_table, n_max, B)
+    with _on_device_of(queries):
+        q, k, v = queries.contiguous(), keys.contiguous(), values.contiguous()
+        kv_len, q_len = _int_vector(kv_len, B, q.device, "kv_len"), _int_vector(q_len, B, q.device, "q_len")
+        out = _out_arg(out, q)
+        lse = None
+        if return_lse:
+            lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if q_len is None else \
+                torch.full((B, Hq, T), float("-inf"), dtype=torch.float32, device=q.device)
+        L = _lib.lib()
+        ws = _scratch(L.dflash_prompt_sdpa_workspace_bytes(B, Hq, Hkv, T, D, N), q.device)
+        _lib.check(L.dflash_prompt_sdpa(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(page_table), _ptr(q_len), _ptr(kv_len), _ptr(out), _ptr(lse), _ptr(ws),
+            0 if ws is None else ws.numel(), B, Hq, Hkv, T, D, N, page_tokens, max_pages, num_pages, int(window), int(sinks),
+            float(scale), _DT[q.dtype], _stream()))
+    return (out, lse) if return_lse else out
+
+
+def attention_mass(queries, keys, lse, scale: float, mass, q_len=None, kv_len=None, page_table=None, window: int = 0,
+                   sinks: int = 0, n_max=None) -> None:
+    """Adds to mass fp32 [B,Hkv,>= capacity] the weight that the queries [B,Hq,T,D] give to every cached token, summed over
+    rows and the query heads of a KV head: exp(scale * q.k - lse) with the lse [B,Hq,T] of prompt_sdpa over the same cache
+    (all of a chunk's rows, or its last ones: the rows given are the last T, or q_len, tokens of the cache)."""
+    _cache_tensors(queries, keys, None)
+    if queries.dim() != 4:
+        raise _bad("queries must be [B, Hq, T, D]")
+    B, Hq, T, D = queries.shape
+    Hkv = keys.shape[1]
+    if lse.dtype != torch.float32 or lse.shape != (B, Hq, T):
+        raise _bad("lse must be fp32 [B, Hq, T]")
+    _same_device(queries, page_table, lse, mass)
+    page_table, N, page_tokens, max_pages, num_pages = _cache_shape(keys, page_table, n_max, B)
+    _mass_arg(mass, B, Hkv, N)
+    with _on_device_of(queries):
+        q, k, lse = queries.contiguous(), keys.contiguous(), lse.contiguous()
+        kv_len, q_len = _int_vector(kv_len, B, q.device, "kv_len"), _int_vector(q_len, B, q.device, "q_len")
+        L = _lib.lib()
+        ws = _scratch(L.dflash_attention_mass_workspace_bytes(B, Hq, Hkv, T, D, N), q.device)
+        _lib.check(L.dflash_attention_mass(
+            _ptr(q), _ptr(k), _ptr(page_table), _ptr(q_len), _ptr(kv_len), _ptr(lse), _ptr(mass), _ptr(ws),
+            0 if ws is None else ws.numel(), B, Hq, Hkv, T, D, N, page_tokens, max_pages, num_pages, mass.shape[2], int(window),
+            int(sinks), float(scale), _DT[q.dtype], _stream()))
+
+
+def kv_evict(k_cache, v_cache, mass, kv_len, budget: int, recent: int, sinks: int = 0, page_table=None, kv_len_out=None,
+             mass_out=None, kept=None, n_max=None) -> torch.Tensor:
+    """Cuts every sequence longer than `budget` tokens down to it, per KV head and in place: the first `sinks` tokens, the
+    last `recent` and the heaviest of the others (mass fp32 [B,Hkv,>= capacity], ties to the lowest index) move to the
+    front of the cache in the order they are in.
+
+    k_cache/v_cache a dense cache [B,Hkv,capacity,D] or, with page_table, page pools; the pages of a sequence that is cut
+    belong to it alone.  mass_out (default: mass itself) receives the masses of the rows that stay and zeros up to the
+    old length; kept int32 [B,Hkv,budget], if given, their old places (-1 behind the last).  Returns kv_len_out
+    (default: kv_len itself, updated): min(kv_len, budget).
+    """
+    _need_cuda(k_cache, v_cache, mass, kv_len)
+    _same_device(k_cache, v_cache, mass, kv_len, page_table, kv_len_out, mass_out, kept)
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+        raise _bad("k_cache and v_cache must be two 4-dimensional tensors of one shape and dtype")
+    if k_cache.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise _lib.DFlashUnsupported(_lib.ERR_UNSUPPORTED, f"dtype {k_cache.dtype}")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise _bad("the caches are changed in place and must be contiguous")
+    B, Hkv, D = kv_len.numel(), k_cache.shape[1], k_cache.shape[3]
+    budget = int(budget)
+    page_table, N, page_tokens, max_pages, num_pages = _cache_shape(k_cache, page_table, n_max, B)
+    kv_len_out = kv_len if kv_len_out is None else kv_len_out
+    for t, name in ((kv_len, "kv_len"), (kv_len_out, "kv_len_out")):
+        if t.dtype != torch.int32 or t.shape != (B,) or not t.is_contiguous():
+            raise _bad(f"{name} must be a contiguous int32 tensor [B]")
+    mass_out = mass if mass_out is None else mass_out
+    _mass_arg(mass, B, Hkv, N)
+    _mass_arg(mass_out, B, Hkv, N, "mass_out")
+    if mass_out.shape != mass.shape:
+        raise _bad("mass_out must have the shape of mass")
+    if kept is not None and (kept.dtype != torch.int32 or kept.shape != (B, Hkv, budget) or not kept.is_contiguous()):
+        raise _bad("kept must be a contiguous int32 tensor [B, Hkv, budget]")
+    with _on_device_of(k_cache):
+        L = _lib.lib()
+        ws = _scratch(0 if kept is not None else L.dflash_kv_evict_workspace_bytes(B, Hkv, N, budget), k_cache.device)
+        _lib.check(L.dflash_kv_evict(
+            _ptr(k_cache), _ptr(v_cache), _ptr(page_table), _ptr(kv_len), _ptr(mass), _ptr(kv_len_out), _ptr(mass_out), _ptr(kept),
+            _ptr(ws), 0 if ws is None else ws.numel(), B, Hkv, D, N, page_tokens, max_pages, num_pages, mass.shape[2], budget,
+            int(recent), int(sinks), _DT[k_cache.dtype], _stream()))
+    return kv_len_out
 
 
 def gated_delta_into(q, k, v, g, beta, state, n_per_seq, y, state_out, tape=None, mask=None) -> None:
