@@ -6,16 +6,18 @@
 // against n D elements of keys and values that stay in L2: bound by the tensor pipe and, next to it, by the 128 x 128
 // exponentials of a tile (16 a clock per SM, 1024 clocks; a tile's two products take 1024 at D = 128, 2048 at 256).
 //
-// * A query tile is 128 rows: the heads of one KV head for consecutive tokens (tc_common.cuh).  D <= 128: two query
-//   tiles a CTA, each with its score columns and accumulator in tensor memory and a softmax warpgroup (one thread a
-//   row); the tiles take turns, one's products run under the other's exponentials, and a key tile is loaded once for both.
-//   D = 256: the accumulator takes half of the tensor memory, so one query tile with two score buffers; two threads
-//   share a row.
+// * A query tile is 128 rows: the heads of one KV head for consecutive tokens (tc_common.cuh); a unit of work has two.
+//   D <= 128: one CTA takes both, each with its score columns and accumulator in tensor memory and a softmax warpgroup
+//   (one thread a row); the tiles take turns, one's products run under the other's exponentials, and a key tile is
+//   loaded once for both.  D = 256: the accumulator takes half of the tensor memory, so a pair of CTAs takes a unit with
+//   products of 256 rows across the two SMs (cta_group::2), each holding its query tile, two score buffers, half of the
+//   keys of a tile and half of the value columns; two threads share a row.  One CTA alone would read 128 KiB of keys and
+//   values from L2 for each 128 x 128 tile: that ran at 4600 clocks a tile, waiting for L2 and for shared memory.
 // * Warps: 0 loads queries and keys, 1 values, 2 issues S = Q K^T, 3 issues O += P V (P replaces S in tensor memory,
 //   in the inputs' type: the product needs a 16-bit operand), 4-11 softmax.
 // * Only the key tiles that some row of the unit sees are visited; only those that some row does not see whole are masked.
 //   Value rows behind the sequence's length are zeroed in shared memory before the product, whatever the cache holds there.
-// * One persistent CTA per SM.  plan_kernel lays the key tiles of all units in a row and cuts them into equal ranges, so
+// * Persistent CTAs, one per SM.  plan_kernel lays the key tiles of all units in a row and cuts them into equal ranges, so
 //   that unequal lengths, causal triangles and few query rows over a long cache all fill the GPU; a cut closer than kMinCut
 //   tiles to a unit's edge moves to the edge.  A unit cut in pieces leaves (O, m, l) per piece in the workspace and
 //   join_kernel adds them up in order.
@@ -40,7 +42,7 @@ struct Cut { long long unit; int first, count; };
 struct PromptParams {
   CacheArgs a;
   Tiling t;
-  int NTT;                     // units (of NQ query tiles) per (sequence, KV head, head group)
+  int NTT;                     // units (of two query tiles) per (sequence, KV head, head group)
   int box;
   int grid;
   float scale_log2;
@@ -48,29 +50,33 @@ struct PromptParams {
   long long* steps;            // [B * NTT + 1] key tiles in front of every (sequence, unit)
   Boundary* bounds;            // [grid + 1]
   Cut* cuts;                   // [grid]
-  float4* part_o;              // [2 * grid][D / 4][128 NQ]
-  float2* part_ml;             // [2 * grid][128 NQ]
+  float4* part_o;              // [2 * grid][D / 4][256]
+  float2* part_ml;             // [2 * grid][256]
 };
 
 template <int D> struct Cfg {
-  static constexpr int NQ = D == 256 ? 1 : 2;               // query tiles
+  static constexpr bool PAIR = D == 256;                    // two CTAs on one unit, a query tile each
   static constexpr int NC = D / 64;                         // 64-column chunks of a row
-  static constexpr int ring = 10;                           // 16 KiB chunks of keys and values
-  static constexpr int KS = D == 64 ? 4 : 4, VS = ring - KS;
+  static constexpr int QT = PAIR ? 1 : 2;                   // query tiles of one CTA (a unit has two)
+  static constexpr int k_rows = PAIR ? 64 : 128;            // this CTA's share of a key tile: rows ...
+  static constexpr int v_chunks = PAIR ? NC / 2 : NC;       // ... and of a value tile: columns
+  static constexpr int k_chunk = k_rows * 128, k_stage = NC * k_chunk, v_stage = v_chunks * kChunk;
+  static constexpr int KS = D == 64 ? 4 : 2, VS = D == 64 ? 6 : 3;
   static constexpr int q = 0;
-  static constexpr int kv = NQ * NC * kChunk;
-  static constexpr int bars = kv + ring * kChunk;
+  static constexpr int k = QT * NC * kChunk, v = k + KS * k_stage;
+  static constexpr int bars = v + VS * v_stage;
   // barriers
   static constexpr int b_q_full = 0, b_q_empty = 1, b_s_full = 2, b_p_full = 4, b_s_free = 6, b_pv_done = 8, b_o_free = 10,
-                       b_kv_full = 12, b_kv_empty = 12 + ring, n_bars = 12 + 2 * ring;
-  static constexpr int misc = bars + 8 * n_bars;            // tensor-memory base, abort flag
+                       b_tail = 12, b_k_full = 13, b_k_empty = b_k_full + KS, b_v_full = b_k_empty + KS, b_v_empty = b_v_full + VS,
+                       n_bars = b_v_empty + VS;
+  static constexpr int misc = bars + (8 * n_bars + 15) / 16 * 16;   // tensor-memory base, abort flag
   static constexpr int xch = misc + 16;                     // [2][2][128] row maxima of the two halves (D = 256)
-  static constexpr int total = xch + 2 * 2 * 128 * 4;
+  static constexpr int total = xch + (PAIR ? 2 * 2 * 128 * 4 : 0);
   // tensor-memory columns: accumulators first, score buffers in the upper half
   __host__ __device__ static constexpr int col_o(int qi) { return qi * 128; }
   __host__ __device__ static constexpr int col_s(int i) { return 256 + i * 128; }
 };
-static_assert(Cfg<256>::total <= 232448 && Cfg<128>::total <= 232448, "shared memory");
+static_assert(Cfg<256>::total <= 232448 && Cfg<128>::total <= 232448 && Cfg<64>::total <= 232448, "shared memory");
 
 // ---- the plan ----
 __device__ __forceinline__ int unit_steps(const PromptParams& p, RowLens len, int tt, int tokens) {
@@ -181,22 +187,21 @@ struct Segment {
   int nq;                      // query tiles with rows in use
   int slot;                    // -1: the whole unit
 };
-// the segments of one CTA, in order; every role walks them for itself
-template <int NQ>
+// the segments of one worker (a CTA or a pair of CTAs), in order; every role walks them for itself
 struct Walker {
   const PromptParams& p;
   long long unit, left;
   int off;
-  bool first;
-  __device__ explicit Walker(const PromptParams& p_) : p(p_), first(true) {
-    const Boundary x = p.bounds[blockIdx.x], y = p.bounds[blockIdx.x + 1];
+  int worker;
+  __device__ Walker(const PromptParams& p_, int worker_) : p(p_), worker(worker_) {
+    const Boundary x = p.bounds[worker], y = p.bounds[worker + 1];
     unit = x.unit;
     off = x.off;
     left = y.pos - x.pos;
   }
   __device__ bool next(Segment& s) {
     if (left <= 0) return false;
-    const int tokens = NQ * p.t.Tt;
+    const int tokens = 2 * p.t.Tt;
     for (;;) {
       s.u = unit_at(p, unit, tokens);
       if (s.u.t0 < s.u.len.rows) break;
@@ -205,8 +210,8 @@ struct Walker {
     s.lo = off;
     const int size = s.u.k.count;
     s.hi = left < size - off ? off + (int)left : size;
-    s.nq = NQ == 2 && s.u.t0 + p.t.Tt < s.u.len.rows ? 2 : 1;
-    s.slot = (s.lo == 0 && s.hi == size) ? -1 : 2 * (int)blockIdx.x + (s.lo > 0 ? 0 : 1);
+    s.nq = s.u.t0 + p.t.Tt < s.u.len.rows ? 2 : 1;
+    s.slot = (s.lo == 0 && s.hi == size) ? -1 : 2 * worker + (s.lo > 0 ? 0 : 1);
     left -= s.hi - s.lo;
     off = 0;
     ++unit;
@@ -222,19 +227,36 @@ __device__ __forceinline__ bool row_of(const PromptParams& p, const Unit& u, int
   return r < p.t.Gt * p.t.Tt && g < p.t.G && t < u.len.rows;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// (x, y) * s + t in one instruction; (x, y) + (u, v) in one
+__device__ __forceinline__ float2 fma2(float x, float y, float s, float t) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, e;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\tfma.rn.f32x2 e, a, b, c;\n\tmov.b64 {%0, %1}, e;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(x), "f"(y), "f"(s), "f"(t));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, e;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 e, a, b;\n\tmov.b64 {%0, %1}, e;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
               const __grid_constant__ CUtensorMap map_v, const PromptParams p) {
   using C = Cfg<D>;
-  constexpr int NQ = C::NQ, NC = C::NC, KS = C::KS, VS = C::VS;
+  constexpr bool PAIR = C::PAIR;
+  constexpr int NC = C::NC, KS = C::KS, VS = C::VS;
   extern __shared__ __align__(1024) uint8_t sm[];
   const CacheArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if ((ptx::smem_u32(sm) & 1023u) != 0u) {   // swizzled tiles need 1024-byte alignment; never seen violated
-    if (threadIdx.x == 0) atomicExch(a.status, kStatusSmemAlign);
-    return;
-  }
+  const int rank = PAIR ? (int)ptx::cluster_rank() : 0, worker = PAIR ? blockIdx.x >> 1 : blockIdx.x;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::bars);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::misc + 4);
@@ -243,184 +265,229 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     ptx::prefetch_tensormap(&map_q);
     ptx::prefetch_tensormap(&map_k);
     ptx::prefetch_tensormap(&map_v);
-    // arrivals: P and the freed accumulator come from softmax warps (4 a query tile, 8 when two threads share a row)
+    // Arrivals.  P and the freed accumulator: one a softmax warp (4 a query tile; 8 in each CTA of a pair).  Values: the
+    // loading lane of each CTA.  A pair's leader has the barriers that its issuing lanes wait for.
     for (int i = 0; i < C::n_bars; ++i) {
       const bool soft = (i >= C::b_p_full && i < C::b_p_full + 2) || (i >= C::b_o_free && i < C::b_o_free + 2);
-      ptx::mbar_init(&bars[i], soft ? (NQ == 2 ? 4 : 8) : 1);
+      const bool val = i >= C::b_v_full && i < C::b_v_full + VS;
+      ptx::mbar_init(&bars[i], soft ? (PAIR ? 16 : 4) : (val && PAIR ? 2 : 1));
     }
-    *abort_flag = 0;
+    *abort_flag = (ptx::smem_u32(sm) & 1023u) != 0u;      // swizzled tiles need 1024-byte alignment; never seen violated
+    if (*abort_flag) atomicExch(a.status, kStatusSmemAlign);
     ptx::fence_mbar_init();
   }
   if (warp == 2) {
-    ptx::tmem_alloc(tmem_slot, 512);
-    ptx::tmem_relinquish();
+    if constexpr (PAIR) {
+      ptx::tmem_alloc_pair(tmem_slot, 512);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(tmem_slot, 512);
+      ptx::tmem_relinquish();
+    }
   }
   ptx::tc_fence_before();
+  if constexpr (PAIR) ptx::cluster_sync();
   __syncthreads();
   ptx::tc_fence_after();
   asm volatile("griddepcontrol.wait;" ::: "memory");     // the plan
   const uint32_t tmem = *tmem_slot;
-  // A wait that gives up raises the CTA's abort flag, after which every wait returns at once: the roles run through
-  // their loops without results, meet at the end and leave.
-  auto wait = [&](int bar, uint32_t parity) { return ptx::mbar_wait_or_abort(&bars[bar], parity, abort_flag, a.status, kStatusMbarWait); };
+  // A wait that gives up raises the abort flags, after which every wait of the CTA (or pair) returns at once: the roles run
+  // through their loops without results, meet at the end and leave.
+  auto wait_as = [&](int bar, uint32_t parity, bool cluster) {
+    for (uint32_t i = 0; i < ptx::kWaitPolls; ++i) {
+      if (PAIR && cluster ? ptx::mbar_try_wait_cluster(&bars[bar], parity) : ptx::mbar_try_wait(&bars[bar], parity)) return true;
+      if ((i & 63u) == 63u) {
+        if (*abort_flag) return false;
+        __nanosleep(40);
+      }
+    }
+    *abort_flag = 1;
+    if constexpr (PAIR) ptx::cluster_store(ptx::cluster_addr(const_cast<int*>(abort_flag), rank ^ 1), 1);
+    atomicExch(a.status, kStatusMbarWait);
+    return false;
+  };
+  auto wait = [&](int bar, uint32_t parity) { return wait_as(bar, parity, false); };
+  auto wait_pair = [&](int bar, uint32_t parity) { return wait_as(bar, parity, true); };   // arrivals of both CTAs
+  auto commit = [&](int bar) {
+    if constexpr (PAIR) ptx::umma_commit_pair(&bars[bar]);
+    else ptx::umma_commit(&bars[bar]);
+  };
+  // the leader's barrier, for arrivals and copies of both CTAs
+  auto arrive_leader = [&](int bar) {
+    if (PAIR) ptx::cluster_arrive(ptx::cluster_addr(&bars[bar], 0));
+    else ptx::mbar_arrive(&bars[bar]);
+  };
+  auto load = [&](void* dst, const CUtensorMap* m, int x, int y, int z, int w, int bar) {
+    if constexpr (PAIR) ptx::tma_load_4d_pair(dst, m, x, y, z, w, ptx::cluster_addr(&bars[bar], 0));
+    else ptx::tma_load_4d(dst, m, x, y, z, w, &bars[bar]);
+  };
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsHelper));
-    Walker<NQ> walk(p);
+    Walker walk(p, worker);
     Segment s;
     if (warp == 0) {
       // ------------------------------ queries and keys ------------------------------
       uint32_t fill = 0, seg = 0;
-      bool ok = true;
+      bool ok = !*abort_flag;
       while (ok && walk.next(s)) {
-        if (seg > 0) ok = wait(C::b_q_empty, (seg - 1) & 1);
-        ok = __all_sync(0xffffffffu, ok);
+        if (seg > 0) ok = __all_sync(0xffffffffu, wait(C::b_q_empty, (seg - 1) & 1));
         if (!ok) break;
         if (lane == 0) {
-          ptx::mbar_arrive_expect_tx(&bars[C::b_q_full], s.nq * NC * p.t.Gt * p.t.Tt * 128);
-          for (int qi = 0; qi < s.nq; ++qi)
+          const int tiles = PAIR ? 2 : s.nq;                  // a pair's tile without rows in use reads as zeros
+          if (rank == 0) ptx::mbar_arrive_expect_tx(&bars[C::b_q_full], tiles * NC * p.t.Gt * p.t.Tt * 128);
+          for (int qi = 0; qi < (PAIR ? 1 : tiles); ++qi)
             for (int c = 0; c < NC; ++c)
-              ptx::tma_load_4d(sm + C::q + (qi * NC + c) * kChunk, &map_q, c * 64, s.u.gc * p.t.Gt, s.u.t0 + qi * p.t.Tt,
-                               s.u.b * a.Hkv + s.u.h, &bars[C::b_q_full]);
+              load(sm + C::q + (qi * NC + c) * kChunk, &map_q, c * 64, s.u.gc * p.t.Gt, s.u.t0 + (PAIR ? rank : qi) * p.t.Tt,
+                   s.u.b * a.Hkv + s.u.h, C::b_q_full);
         }
         __syncwarp();
-        for (int j = s.lo; ok && j < s.hi; ++j) {
-          const int n0 = tile_key(s.u.k, j);
-          for (int c = 0; ok && c < NC; ++c, ++fill) {
-            const uint32_t st = fill % KS;
-            if (fill >= KS) ok = wait(C::b_kv_empty + st, (fill / KS - 1) & 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok) load_chunk(sm + C::kv + st * kChunk, &map_k, a, p.box, s.u.b, s.u.h, n0, s.u.len.keys, c * 64, &bars[C::b_kv_full + st], lane);
+        for (int j = s.lo; j < s.hi; ++j, ++fill) {
+          const int n0 = tile_key(s.u.k, j) + rank * 64;
+          const uint32_t st = fill % KS;
+          if (fill >= KS) ok = __all_sync(0xffffffffu, wait(C::b_k_empty + st, (fill / KS - 1) & 1));
+          if (!ok) break;
+          if (lane == 0 && rank == 0) ptx::mbar_arrive_expect_tx(&bars[C::b_k_full + st], (PAIR ? 2 : 1) * C::k_stage);
+          __syncwarp();
+          const int box = p.box < C::k_rows ? p.box : C::k_rows, pieces = C::k_rows / box;
+          for (int i = lane; i < NC * pieces; i += 32) {
+            const int c = i / pieces, n = n0 + (i - c * pieces) * box;
+            const TilePlace at = place_of(a, s.u.b, n, s.u.len.keys);
+            load(sm + C::k + st * C::k_stage + c * C::k_chunk + (n - n0) * 128, &map_k, c * 64, at.row, s.u.h, at.outer, C::b_k_full + st);
           }
+          __syncwarp();
         }
         ++seg;
       }
     } else if (warp == 1) {
       // ----------------------------------- values -----------------------------------
-      uint32_t fill = 0;
-      bool ok = true;
+      uint32_t fill = 0, tails = 0;
+      bool ok = !*abort_flag;
       while (ok && walk.next(s)) {
-        for (int j = s.lo; ok && j < s.hi; ++j) {
-          const int n0 = tile_key(s.u.k, j);
-          for (int c = 0; ok && c < NC; ++c, ++fill) {
-            const uint32_t st = KS + fill % VS;
-            if (fill >= VS) ok = wait(C::b_kv_empty + st, (fill / VS - 1) & 1);
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok) load_chunk(sm + C::kv + st * kChunk, &map_v, a, p.box, s.u.b, s.u.h, n0, s.u.len.keys, c * 64, &bars[C::b_kv_full + st], lane);
+        for (int j = s.lo; j < s.hi; ++j, ++fill) {
+          const int n0 = tile_key(s.u.k, j), rows = s.u.len.keys - n0;
+          const uint32_t st = fill % VS;
+          if (fill >= VS) ok = __all_sync(0xffffffffu, wait(C::b_v_empty + st, (fill / VS - 1) & 1));
+          if (!ok) break;
+          // Rows behind the sequence's length: a weight of zero times whatever the cache holds there would not be zero, so
+          // such a tile lands under a barrier of its own and the rows are cleared before the tile is announced.
+          const bool tail = rows < kKeys;
+          if (lane == 0) {
+            if (tail) ptx::mbar_arrive_expect_tx(&bars[C::b_tail], C::v_stage);
+            else if (rank == 0) ptx::mbar_arrive_expect_tx(&bars[C::b_v_full + st], (PAIR ? 2 : 1) * C::v_stage);
+            else arrive_leader(C::b_v_full + st);
+          }
+          __syncwarp();
+          uint8_t* dst = sm + C::v + st * C::v_stage;
+          const int pieces = kKeys / p.box;
+          for (int i = lane; i < C::v_chunks * pieces; i += 32) {
+            const int c = i / pieces, n = n0 + (i - c * pieces) * p.box;
+            const TilePlace at = place_of(a, s.u.b, n, s.u.len.keys);
+            uint8_t* d = dst + c * kChunk + (n - n0) * 128;
+            const int col = (rank * C::v_chunks + c) * 64;
+            if (tail) ptx::tma_load_4d(d, &map_v, col, at.row, s.u.h, at.outer, &bars[C::b_tail]);
+            else load(d, &map_v, col, at.row, s.u.h, at.outer, C::b_v_full + st);
+          }
+          __syncwarp();
+          if (tail) {
+            ok = __all_sync(0xffffffffu, wait(C::b_tail, tails++ & 1));
+            if (!ok) break;
+            for (int c = 0; c < C::v_chunks; ++c)
+              for (int e = (rows > 0 ? rows : 0) * 8 + lane; e < kKeys * 8; e += 32)
+                *reinterpret_cast<uint4*>(dst + c * kChunk + e * 16) = make_uint4(0, 0, 0, 0);
+            ptx::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) arrive_leader(C::b_v_full + st);
           }
         }
       }
     } else if (warp == 2) {
       // --------------------------------- S = Q K^T ----------------------------------
-      constexpr uint32_t kI = idesc<T>(kRows, kKeys, false);
-      if (lane == 0) {
+      constexpr uint32_t kI = idesc<T>(PAIR ? 256 : 128, kKeys, false);
+      if (lane == 0 && rank == 0) {
         uint32_t drain = 0, seg = 0, n_s[2] = {0, 0};       // n_s: score tiles issued per buffer
-        const uint32_t q_addr = ptx::smem_u32(sm + C::q), kv_addr = ptx::smem_u32(sm + C::kv);
+        const uint32_t q_addr = ptx::smem_u32(sm + C::q), k_addr = ptx::smem_u32(sm + C::k);
         bool ok = true;
         while (ok && walk.next(s)) {
           ok = wait(C::b_q_full, seg & 1);
-          ptx::tc_fence_after();
-          for (int j = s.lo; ok && j < s.hi; ++j) {
-            for (int qi = 0; ok && qi < s.nq; ++qi) {
+          const int nq = PAIR ? 1 : s.nq;
+          for (int j = s.lo; ok && j < s.hi; ++j, ++drain) {
+            const uint32_t st = drain % KS;
+            ok = wait(C::b_k_full + st, (drain / KS) & 1);
+            for (int qi = 0; ok && qi < nq; ++qi) {
               // the buffer is free once the product that read P from it has retired
-              const int buf = NQ == 2 ? qi : (int)((n_s[0] + n_s[1]) & 1);
+              const int buf = PAIR ? (int)(drain & 1) : qi;
               if (n_s[buf] > 0) ok = wait(C::b_s_free + buf, (n_s[buf] - 1) & 1);
               if (!ok) break;
               ptx::tc_fence_after();
               const uint32_t d = tmem + C::col_s(buf);
-              for (int c = 0; ok && c < NC; ++c) {
-                const uint32_t f = drain + c, st = f % KS;
-                if (qi == 0) {
-                  ok = wait(C::b_kv_full + st, (f / KS) & 1);
-                  ptx::tc_fence_after();
+#pragma unroll
+              for (int c = 0; c < NC; ++c) {
+                const uint64_t da = make_desc(q_addr + (qi * NC + c) * kChunk, 16, 1024);
+                const uint64_t db = make_desc(k_addr + st * C::k_stage + c * C::k_chunk, 16, 1024);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  if constexpr (PAIR) ptx::umma_ss_pair(d, da + 2 * k, db + 2 * k, kI, c + k > 0);
+                  else ptx::umma_ss(d, da + 2 * k, db + 2 * k, kI, c + k > 0);
                 }
-                const uint64_t da = make_desc(q_addr + (qi * NC + c) * kChunk, 16, 1024), db = make_desc(kv_addr + st * kChunk, 16, 1024);
-                if (c == 0) ptx::umma_ss_first(d, da, db, kI);
-                else ptx::umma_ss_acc(d, da, db, kI);
-                ptx::umma_ss_acc(d, da + 2, db + 2, kI);
-                ptx::umma_ss_acc(d, da + 4, db + 4, kI);
-                ptx::umma_ss_acc(d, da + 6, db + 6, kI);
-                if (qi == s.nq - 1) ptx::umma_commit(&bars[C::b_kv_empty + st]);
               }
-              ptx::umma_commit(&bars[C::b_s_full + buf]);
+              commit(C::b_s_full + buf);
+              if (qi == nq - 1) commit(C::b_k_empty + st);
               ++n_s[buf];
             }
-            drain += NC;
           }
-          ptx::umma_commit(&bars[C::b_q_empty]);
+          commit(C::b_q_empty);
           ++seg;
         }
       }
     } else {
       // --------------------------------- O += P V -----------------------------------
-      constexpr int kN = D == 64 ? 64 : 128;                 // columns of one product: one or two chunks
-      constexpr uint32_t kI = idesc<T>(kRows, kN, true);
-      uint32_t drain = 0, n_p[2] = {0, 0}, n_seg[2] = {0, 0};
-      bool ok = true;
-      while (ok && walk.next(s)) {
-        for (int j = s.lo; ok && j < s.hi; ++j) {
-          // value rows behind the sequence's length: zero, whatever the cache holds there
-          const int n0 = tile_key(s.u.k, j), rows = s.u.len.keys - n0;
-          if (rows < kKeys) {
-            for (int c = 0; c < NC; ++c) {
-              const uint32_t f = drain + c, st = KS + f % VS;
-              ok = __all_sync(0xffffffffu, wait(C::b_kv_full + st, (f / VS) & 1)) && ok;
-              uint8_t* v = sm + C::kv + st * kChunk;
-              for (int e = (rows > 0 ? rows : 0) * 8 + lane; e < kKeys * 8; e += 32) *reinterpret_cast<uint4*>(v + e * 16) = make_uint4(0, 0, 0, 0);
-            }
-            ptx::fence_proxy_async();
-            __syncwarp();
-          }
-          if (lane == 0) {
-            for (int qi = 0; ok && qi < s.nq; ++qi) {
-              const int buf = NQ == 2 ? qi : (int)((n_p[0] + n_p[1]) & 1);
+      constexpr uint32_t kI = idesc<T>(PAIR ? 256 : 128, D, true);
+      if (lane == 0 && rank == 0) {
+        uint32_t drain = 0, n_p[2] = {0, 0}, n_seg[2] = {0, 0};
+        const uint32_t v_addr = ptx::smem_u32(sm + C::v);
+        bool ok = true;
+        while (ok && walk.next(s)) {
+          const int nq = PAIR ? 1 : s.nq;
+          for (int j = s.lo; ok && j < s.hi; ++j, ++drain) {
+            const uint32_t st = drain % VS;
+            ok = wait_pair(C::b_v_full + st, (drain / VS) & 1);
+            for (int qi = 0; ok && qi < nq; ++qi) {
+              const int buf = PAIR ? (int)(drain & 1) : qi;
               // the first product of a segment overwrites the accumulator: the last segment's result must be out
-              if (j == s.lo && n_seg[qi] > 0) ok = wait(C::b_o_free + qi, (n_seg[qi] - 1) & 1);
-              ok = ok && wait(C::b_p_full + buf, n_p[buf] & 1);
+              if (j == s.lo && n_seg[qi] > 0) ok = wait_pair(C::b_o_free + qi, (n_seg[qi] - 1) & 1);
+              ok = ok && wait_pair(C::b_p_full + buf, n_p[buf] & 1);
               if (!ok) break;
               ptx::tc_fence_after();
-              const uint32_t pt = tmem + C::col_s(buf);
-              for (int c = 0; ok && c < NC; c += kN / 64) {
-                const uint32_t f = drain + c, st = KS + f % VS;
-                if (qi == 0) {
-                  ok = wait(C::b_kv_full + st, (f / VS) & 1);
-                  if (kN == 128) ok = ok && wait(C::b_kv_full + st + 1, (f / VS) & 1);
-                  ptx::tc_fence_after();
-                }
-                // 16 keys a step: 2048 bytes of values, 8 columns of P; the second chunk of a pair lies 16 KiB on
-                const uint64_t db = make_desc(ptx::smem_u32(sm + C::kv + st * kChunk), kChunk, 1024);
-                const uint32_t d = tmem + C::col_o(qi) + c * 64;
-                if (j == s.lo) ptx::umma_ts_first(d, pt, db, kI);
-                else ptx::umma_ts_acc(d, pt, db, kI);
+              // 16 keys a step: 2048 bytes of values, 8 columns of P; 64-column chunks lie 16 KiB apart
+              const uint64_t db = make_desc(v_addr + st * C::v_stage, kChunk, 1024);
+              const uint32_t d = tmem + C::col_o(qi), pt = tmem + C::col_s(buf);
 #pragma unroll
-                for (int k = 1; k < kKeys / 16; ++k) ptx::umma_ts_acc(d, pt + k * 8, db + (uint64_t)k * 128, kI);
-                if (qi == s.nq - 1) {
-                  ptx::umma_commit(&bars[C::b_kv_empty + st]);
-                  if (kN == 128) ptx::umma_commit(&bars[C::b_kv_empty + st + 1]);
-                }
+              for (int k = 0; k < kKeys / 16; ++k) {
+                if constexpr (PAIR) ptx::umma_ts_pair(d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || k > 0);
+                else ptx::umma_ts(d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || k > 0);
               }
-              ptx::umma_commit(&bars[C::b_s_free + buf]);
-              ptx::umma_commit(&bars[C::b_pv_done + qi]);
+              commit(C::b_pv_done + qi);
+              commit(C::b_s_free + buf);
+              if (qi == nq - 1) commit(C::b_v_empty + st);
               ++n_p[buf];
             }
-            for (int qi = 0; j == s.hi - 1 && qi < s.nq; ++qi) ++n_seg[qi];
           }
-          drain += NC;
-          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+          for (int qi = 0; qi < nq; ++qi) ++n_seg[qi];
         }
       }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     // ----------------------------------- softmax ------------------------------------
-    Walker<NQ> walk(p);
+    Walker walk(p, worker);
     Segment s;
     const int wq = warp & 3, grp = (warp - 4) >> 2;           // tensor-memory lane quarter; query tile, or half of the row
     const int r = wq * 32 + lane;
     const uint32_t lane_addr = tmem + ((uint32_t)(wq * 32) << 16);
-    const int qi = NQ == 2 ? grp : 0;
-    constexpr int NS = NQ == 2 ? 128 : 64;                    // score columns of this thread
-    const int col0 = NQ == 2 ? 0 : grp * 64;
+    const int qi = PAIR ? 0 : grp, tile = PAIR ? rank : grp;  // query tile of this CTA, of the unit
+    constexpr int NS = PAIR ? 64 : 128;                       // score columns of this thread
+    const int col0 = PAIR ? grp * 64 : 0;
     float* xch = reinterpret_cast<float*>(sm + C::xch);
     uint32_t n_s = 0, n_x = 0;                                // score tiles and exchanges done
     // value of the thread that has the other half of this row; the two warps always meet the same number of times
@@ -431,17 +498,16 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       return x[(grp ^ 1) * 128 + r];
     };
     while (walk.next(s)) {
-      if (NQ == 2 && qi >= s.nq) continue;
+      if (!PAIR && qi >= s.nq) continue;
       int t;
       long long row;
-      const bool used = row_of(p, s.u, qi, r, t, row);
+      const bool used = row_of(p, s.u, tile, r, t, row);
       const int pos = s.u.len.keys - s.u.len.rows + t;       // of an unused row too: it sees what it sees, nobody reads it
-      const int p_min = s.u.len.keys - s.u.len.rows + s.u.t0 + qi * p.t.Tt, p_max = p_min + p.t.Tt - 1;
+      const int p_min = s.u.len.keys - s.u.len.rows + s.u.t0 + tile * p.t.Tt, p_max = p_min + p.t.Tt - 1;
       float m = -INFINITY, l = 0.f;
       for (int j = s.lo; j < s.hi; ++j, ++n_s) {
-        const int buf = NQ == 2 ? qi : (int)(n_s & 1);
-        const uint32_t par = NQ == 2 ? n_s & 1 : (n_s >> 1) & 1;
-        wait(C::b_s_full + buf, par);
+        const int buf = PAIR ? (int)(n_s & 1) : qi;
+        wait(C::b_s_full + buf, PAIR ? (n_s >> 1) & 1 : n_s & 1);
         __syncwarp();
         ptx::tc_fence_after();
         const uint32_t s_addr = lane_addr + C::col_s(buf);
@@ -463,9 +529,10 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < NS; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], __uint_as_float(sr[i / 32][i % 32]));
+        for (int i = 0; i < NS; i += 2)
+          mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(sr[i / 32][i % 32]), __uint_as_float(sr[i / 32][i % 32 + 1]));
         float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-        if (NQ == 1) mx = fmaxf(mx, other_half(mx));
+        if (PAIR) mx = fmaxf(mx, other_half(mx));
         float f = 1.f;
         const bool grow = mx > m && (m == -INFINITY || (mx - m) * p.scale_log2 > kRescale);
         if (grow) {
@@ -475,27 +542,33 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         }
         const bool rescale = j > s.lo && __any_sync(0xffffffffu, grow);
         const float neg = m == -INFINITY ? 0.f : -m * p.scale_log2;
-        uint32_t pr[NS / 2];
-        float add4[4] = {0.f, 0.f, 0.f, 0.f};
+        // P over the first columns of S, which both threads of the row have read
+        float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int i = 0; i < NS; i += 2) {
-          const float w0 = mma::exp2_approx(fmaf(__uint_as_float(sr[i / 32][i % 32]), p.scale_log2, neg));
-          const float w1 = mma::exp2_approx(fmaf(__uint_as_float(sr[i / 32][i % 32 + 1]), p.scale_log2, neg));
-          add4[(i >> 1) & 3] += w0 + w1;
-          pr[i / 2] = mma::pack<T>(w0, w1);
+        for (int g = 0; g < NS / 32; ++g) {
+          uint32_t pr[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float2 w = fma2(__uint_as_float(sr[g][i]), __uint_as_float(sr[g][i + 1]), p.scale_log2, neg);
+            w.x = mma::exp2_approx(w.x);
+            w.y = mma::exp2_approx(w.y);
+            add[(i >> 1) & 1] = add2(add[(i >> 1) & 1], w);
+            pr[i / 2] = mma::pack<T>(w.x, w.y);
+          }
+          ptx::tmem_st16(s_addr + col0 / 2 + g * 16, pr);
         }
-        l += (add4[0] + add4[1]) + (add4[2] + add4[3]);
+        l += (add[0].x + add[0].y) + (add[1].x + add[1].y);
         // the last product is done with the accumulator; waited for every time and in order (a parity wait that skips a
         // phase cannot tell "done" from "two phases behind"), after the exponentials, when it rarely waits
         if (n_s > 0) wait(C::b_pv_done + qi, (n_s - 1) & 1);
+        __syncwarp();
         if (rescale) {
-          constexpr int kCols = NQ == 2 ? D : D / 2;
-          __syncwarp();
+          constexpr int kCols = PAIR ? D / 2 : D;
           ptx::tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < kCols; c += 32) {
             uint32_t o[32];
-            const uint32_t o_addr = lane_addr + C::col_o(qi) + (NQ == 2 ? 0 : grp * kCols) + c;
+            const uint32_t o_addr = lane_addr + C::col_o(qi) + (PAIR ? grp * kCols : 0) + c;
             ptx::tmem_ld32(o_addr, o);
             ptx::tmem_ld_wait();
 #pragma unroll
@@ -503,24 +576,21 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             ptx::tmem_st32(o_addr, o);
           }
         }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < NS / 64; ++i) ptx::tmem_st32(s_addr + col0 / 2 + i * 32, *reinterpret_cast<uint32_t(*)[32]>(&pr[i * 32]));
         ptx::tmem_st_wait();
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&bars[C::b_p_full + buf]);
+        if (lane == 0) arrive_leader(C::b_p_full + buf);
       }
       // ---- the segment's result ----
       wait(C::b_pv_done + qi, (n_s - 1) & 1);
       __syncwarp();
       ptx::tc_fence_after();
-      if (NQ == 1) {                                           // the same order of the two halves in both threads
+      if (PAIR) {                                              // the same order of the two halves in both threads
         const float x = other_half(l);
         l = grp == 0 ? l + x : x + l;
       }
-      constexpr int kCols = NQ == 2 ? D : D / 2;
-      const int c0 = NQ == 2 ? 0 : grp * kCols;
+      constexpr int kCols = PAIR ? D / 2 : D;
+      const int c0 = PAIR ? grp * kCols : 0;
       const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll 1
       for (int c = 0; c < kCols; c += 32) {
@@ -542,17 +612,17 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
           }
         } else {
           // [D / 4][rows]: the 32 rows of a warp store 512 bytes in a row
-          float4* dst = p.part_o + ((long long)s.slot * (D / 4) + (c0 + c) / 4) * (128 * NQ) + qi * 128 + r;
+          float4* dst = p.part_o + ((long long)s.slot * (D / 4) + (c0 + c) / 4) * 256 + tile * 128 + r;
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
-            dst[(i / 4) * (128 * NQ)] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+            dst[(i / 4) * 256] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
         }
       }
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&bars[C::b_o_free + qi]);
-      if (NQ == 2 || grp == 0) {
-        if (s.slot >= 0) p.part_ml[(long long)s.slot * (128 * NQ) + qi * 128 + r] = make_float2(m * p.scale_log2, l);
+      if (lane == 0) arrive_leader(C::b_o_free + qi);
+      if (!PAIR || grp == 0) {
+        if (s.slot >= 0) p.part_ml[(long long)s.slot * 256 + tile * 128 + r] = make_float2(m * p.scale_log2, l);
         else if (used && a.lse) a.lse[row] = l > 0.f ? (m * p.scale_log2 + log2f(l)) * kLn2 : -INFINITY;
       }
     }
@@ -560,18 +630,23 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
   __syncwarp();
   __syncthreads();
   if (*abort_flag) __nanosleep(100000);        // copies that were still in flight land before the memory is given back
-  if (warp == 2) ptx::tmem_dealloc(tmem, 512);
+  if constexpr (PAIR) {
+    ptx::cluster_sync();                       // the other CTA's products and arrivals use this one's memory
+    if (warp == 2) ptx::tmem_dealloc_pair(tmem, 512);
+  } else {
+    if (warp == 2) ptx::tmem_dealloc(tmem, 512);
+  }
 }
 
 // Joins the pieces of a cut unit: 32 rows and 64 columns a block, weights 2^(m_i - max m), added in the order of the pieces.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) join_kernel(const PromptParams p) {
-  constexpr int NQ = Cfg<D>::NQ, R = 128 * NQ;
+  constexpr int R = 256;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Cut cut = p.cuts[blockIdx.x];
   if (cut.count == 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Unit u = unit_at(p, cut.unit, NQ * p.t.Tt);
+  const Unit u = unit_at(p, cut.unit, 2 * p.t.Tt);
   const int rr = blockIdx.y * 32 + lane, qi = rr / 128, r = rr % 128;
   const int col = blockIdx.z * 64 + warp * 16;
   int t;
@@ -613,22 +688,21 @@ size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 struct Plan {
   Tiling t;
-  int NQ, NTT, grid;
+  int NTT, grid;               // grid: workers, a CTA each (D <= 128) or a pair of CTAs
   size_t steps, bounds, cuts, part_ml, part_o, total;
 };
 Plan plan_of(int B, int Hq, int Hkv, int T, int D, int N) {
   Plan x;
   x.t = tiling_of(Hq, Hkv);
-  x.NQ = D == 256 ? 1 : 2;
-  x.NTT = (T + x.NQ * x.t.Tt - 1) / (x.NQ * x.t.Tt);
+  x.NTT = (T + 2 * x.t.Tt - 1) / (2 * x.t.Tt);
   const long long tiles = (long long)B * Hkv * x.t.GC * x.NTT * ((N + kKeys - 1) / kKeys);
-  const int n_sm = sm_count();
-  x.grid = (int)(tiles < n_sm ? tiles : n_sm);
+  const int most = D == 256 ? sm_count() / 2 : sm_count();
+  x.grid = (int)(tiles < most ? tiles : most);
   x.steps = up256(((size_t)B * x.NTT + 1) * 8);
   x.bounds = up256((size_t)(x.grid + 1) * sizeof(Boundary));
   x.cuts = up256((size_t)x.grid * sizeof(Cut));
-  x.part_ml = up256((size_t)2 * x.grid * 128 * x.NQ * sizeof(float2));
-  x.part_o = up256((size_t)2 * x.grid * 128 * x.NQ * D * 4);
+  x.part_ml = up256((size_t)2 * x.grid * 256 * sizeof(float2));
+  x.part_o = up256((size_t)2 * x.grid * 256 * D * 4);
   x.total = x.steps + x.bounds + x.cuts + x.part_ml + x.part_o;
   return x;
 }
@@ -655,7 +729,7 @@ int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
   p.part_o = reinterpret_cast<float4*>(ws += x.part_ml);
   CUtensorMap mq, mk, mv;
   CUresult r = encode_q(&mq, a, x.t);
-  if (r == CUDA_SUCCESS) r = encode_kv(&mk, a.k, a, p.box);
+  if (r == CUDA_SUCCESS) r = encode_kv(&mk, a.k, a, p.box < C::k_rows ? p.box : C::k_rows);
   if (r == CUDA_SUCCESS) r = encode_kv(&mv, a.v, a, p.box);
   if (r != CUDA_SUCCESS) { set_error("prompt_sdpa: cuTensorMapEncodeTiled failed with CUresult %d", (int)r); return DFLASH_ERR_CUDA; }
   auto kernel = prompt_kernel<T, D>;
@@ -663,20 +737,24 @@ int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
   // the register hand-over waits for good if the launch gives the CTA fewer than it takes
   static const int regs = [&] { cudaFuncAttributes f; return cudaFuncGetAttributes(&f, kernel) == cudaSuccess ? f.numRegs : 0; }();
   if (regs != kRegsLaunch) { set_error("prompt_sdpa: the kernel is launched with %d registers a thread, %d expected", regs, kRegsLaunch); return DFLASH_ERR_CUDA; }
-  plan_kernel<<<1, 1024, 0, stream>>>(p, C::NQ * x.t.Tt);
+  plan_kernel<<<1, 1024, 0, stream>>>(p, 2 * x.t.Tt);
   DFLASH_LAUNCH_CHECK();
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = C::PAIR ? 2 : 1;
   cfg.stream = stream;
-  cfg.gridDim = dim3(x.grid);
+  cfg.gridDim = dim3(x.grid * (C::PAIR ? 2 : 1));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = C::total;
   DFLASH_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, p));
-  cfg.gridDim = dim3(x.grid, 4 * C::NQ, D / 64);
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3(x.grid, 8, D / 64);
   cfg.blockDim = dim3(128);
   cfg.dynamicSmemBytes = 0;
   DFLASH_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel<T, D>, p));

@@ -90,26 +90,18 @@ inline CUresult encode_q(CUtensorMap* m, const CacheArgs& a, const Tiling& t) {
                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 
-// One 64-column chunk of the 128 keys from n0 on into `dst`, by the lanes of one warp (one copy of `box` rows a lane).
-// Keys at and behind `len` may be anything that was in the cache.  Lane 0 announces the bytes.
-__device__ __forceinline__ void load_chunk(uint8_t* dst, const CUtensorMap* map, const CacheArgs& a, int box, int b, int h, int n0, int len,
-                                           int col, void* bar, int lane) {
-  if (lane == 0) ptx::mbar_arrive_expect_tx(bar, kChunk);
-  __syncwarp();
-  if (lane < kKeys / box) {
-    const int n = n0 + lane * box;
-    int outer = b, row = n;
-    if (a.page_table) {
-      outer = a.num_pages;                                // behind the pool: zeros
-      row = n % a.page_tokens;
-      if (n < len) {
-        const int page = a.page_table[(long long)b * a.max_pages + n / a.page_tokens];
-        if ((unsigned)page < (unsigned)a.num_pages) outer = page;
-        else atomicExch(a.status, kStatusKvRange);
-      }
-    }
-    ptx::tma_load_4d(dst + lane * box * 128, map, col, row, h, outer, bar);
+// Where the copy that starts at token n of sequence b begins.  Tokens at and behind `len` may be anything that was in the
+// cache; their pages are not looked up.
+struct TilePlace { int row, outer; };
+__device__ __forceinline__ TilePlace place_of(const CacheArgs& a, int b, int n, int len) {
+  if (!a.page_table) return TilePlace{n, b};
+  TilePlace t{n % a.page_tokens, a.num_pages};            // behind the pool: zeros
+  if (n < len) {
+    const int page = a.page_table[(long long)b * a.max_pages + n / a.page_tokens];
+    if ((unsigned)page < (unsigned)a.num_pages) t.outer = page;
+    else atomicExch(a.status, kStatusKvRange);
   }
+  return t;
 }
 
 }  // namespace tc
