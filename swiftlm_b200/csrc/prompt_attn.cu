@@ -227,6 +227,9 @@ __device__ __forceinline__ bool row_of(const PromptParams& p, const Unit& u, int
   return r < p.t.Gt * p.t.Tt && g < p.t.G && t < u.len.rows;
 }
 
+__device__ __forceinline__ uint32_t low_bits(int n) {      // bits [0, n), n clamped to [0, 32]
+  return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u);
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -307,14 +310,14 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     return false;
   };
   auto wait = [&](int bar, uint32_t parity) { return wait_as(bar, parity, false); };
-  auto wait_pair = [&](int bar, uint32_t parity) { return wait_as(bar, parity, true); };   // arrivals of both CTAs
+  auto wait_pair = [&](int bar, uint32_t parity) { return wait_as(bar, parity, true); };   // the other CTA's stores among what is waited for
   auto commit = [&](int bar) {
     if constexpr (PAIR) ptx::umma_commit_pair(&bars[bar]);
     else ptx::umma_commit(&bars[bar]);
   };
   // the leader's barrier, for arrivals and copies of both CTAs
   auto arrive_leader = [&](int bar) {
-    if (PAIR) ptx::cluster_arrive(ptx::cluster_addr(&bars[bar], 0));
+    if (PAIR) ptx::cluster_arrive_tc(ptx::cluster_addr(&bars[bar], 0));
     else ptx::mbar_arrive(&bars[bar]);
   };
   auto load = [&](void* dst, const CUtensorMap* m, int x, int y, int z, int w, int bar) {
@@ -397,7 +400,10 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 *reinterpret_cast<uint4*>(dst + c * kChunk + e * 16) = make_uint4(0, 0, 0, 0);
             ptx::fence_proxy_async();
             __syncwarp();
-            if (lane == 0) arrive_leader(C::b_v_full + st);
+            if (lane == 0) {
+              if (PAIR) ptx::cluster_arrive(ptx::cluster_addr(&bars[C::b_v_full + st], 0));
+              else arrive_leader(C::b_v_full + st);
+            }
           }
         }
       }
@@ -455,8 +461,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             for (int qi = 0; ok && qi < nq; ++qi) {
               const int buf = PAIR ? (int)(drain & 1) : qi;
               // the first product of a segment overwrites the accumulator: the last segment's result must be out
-              if (j == s.lo && n_seg[qi] > 0) ok = wait_pair(C::b_o_free + qi, (n_seg[qi] - 1) & 1);
-              ok = ok && wait_pair(C::b_p_full + buf, n_p[buf] & 1);
+              if (j == s.lo && n_seg[qi] > 0) ok = wait(C::b_o_free + qi, (n_seg[qi] - 1) & 1);
+              ok = ok && wait(C::b_p_full + buf, n_p[buf] & 1);
               if (!ok) break;
               ptx::tc_fence_after();
               // 16 keys a step: 2048 bytes of values, 8 columns of P; 64-column chunks lie 16 KiB apart
@@ -522,10 +528,14 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         }
         const bool whole = n0 + kKeys - 1 <= p_min && (a.window == 0 || n0 > p_max - a.window || n0 + kKeys <= a.sinks);
         if (!whole) {
-          const int hi = pos - n0 - col0, lo = a.window > 0 ? hi - a.window : -1, sink = a.sinks - n0 - col0;
+          const int hi = pos - n0 - col0 + 1, lo = a.window > 0 ? hi - a.window : 0, sink = a.sinks - n0 - col0;
 #pragma unroll
-          for (int i = 0; i < NS; ++i)
-            if (i > hi || (i <= lo && i >= sink)) sr[i / 32][i % 32] = __float_as_uint(-INFINITY);
+          for (int g = 0; g < NS / 32; ++g) {
+            const uint32_t seen = low_bits(hi - g * 32) & (~low_bits(lo - g * 32) | low_bits(sink - g * 32));
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((seen >> i) & 1u)) sr[g][i] = __float_as_uint(-INFINITY);
+          }
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll

@@ -220,6 +220,11 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void cluster_arrive(uint32_t remote_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote_bar) : "memory");
 }
+// the same without making this thread's earlier stores visible there (1200 clocks less): behind tensor-memory accesses that
+// tcgen05.fence::before_thread_sync has ordered, or nothing
+__device__ __forceinline__ void cluster_arrive_tc(uint32_t remote_bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote_bar) : "memory");
+}
 __device__ __forceinline__ void cluster_store(uint32_t remote, int x) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(x) : "memory");
 }
