@@ -311,9 +311,9 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
   };
   auto wait = [&](int bar, uint32_t parity) { return wait_as(bar, parity, false); };
   auto wait_pair = [&](int bar, uint32_t parity) { return wait_as(bar, parity, true); };   // the other CTA's stores among what is waited for
-  auto commit = [&](int bar) {
-    if constexpr (PAIR) ptx::umma_commit_pair(&bars[bar]);
-    else ptx::umma_commit(&bars[bar]);
+  auto commit = [&](uint32_t leader, int bar) {
+    if constexpr (PAIR) ptx::umma_commit_pair_if(leader, &bars[bar]);
+    else ptx::umma_commit_if(leader, &bars[bar]);
   };
   // the leader's barrier, for arrivals and copies of both CTAs
   auto arrive_leader = [&](int bar) {
@@ -325,6 +325,9 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     else ptx::tma_load_4d(dst, m, x, y, z, w, &bars[bar]);
   };
 
+  // The issuing warps run converged, every lane with the same operands, and one lane issues: operands of a diverged lane
+  // would each be moved to uniform registers first.
+  const uint32_t leader = lane == 0;
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsHelper));
     Walker walk(p, worker);
@@ -410,7 +413,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     } else if (warp == 2) {
       // --------------------------------- S = Q K^T ----------------------------------
       constexpr uint32_t kI = idesc<T>(PAIR ? 256 : 128, kKeys, false);
-      if (lane == 0 && rank == 0) {
+      if (rank == 0) {
         uint32_t drain = 0, seg = 0, n_s[2] = {0, 0};       // n_s: score tiles issued per buffer
         const uint32_t q_addr = ptx::smem_u32(sm + C::q), k_addr = ptx::smem_u32(sm + C::k);
         bool ok = true;
@@ -433,23 +436,23 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 const uint64_t db = make_desc(k_addr + st * C::k_stage + c * C::k_chunk, 16, 1024);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                  if constexpr (PAIR) ptx::umma_ss_pair(d, da + 2 * k, db + 2 * k, kI, c + k > 0);
-                  else ptx::umma_ss(d, da + 2 * k, db + 2 * k, kI, c + k > 0);
+                  if constexpr (PAIR) ptx::umma_ss_pair_if(leader, d, da + 2 * k, db + 2 * k, kI, c + k > 0);
+                  else ptx::umma_ss_if(leader, d, da + 2 * k, db + 2 * k, kI, c + k > 0);
                 }
               }
-              commit(C::b_s_full + buf);
-              if (qi == nq - 1) commit(C::b_k_empty + st);
+              commit(leader, C::b_s_full + buf);
+              if (qi == nq - 1) commit(leader, C::b_k_empty + st);
               ++n_s[buf];
             }
           }
-          commit(C::b_q_empty);
+          commit(leader, C::b_q_empty);
           ++seg;
         }
       }
     } else {
       // --------------------------------- O += P V -----------------------------------
       constexpr uint32_t kI = idesc<T>(PAIR ? 256 : 128, D, true);
-      if (lane == 0 && rank == 0) {
+      if (rank == 0) {
         uint32_t drain = 0, n_p[2] = {0, 0}, n_seg[2] = {0, 0};
         const uint32_t v_addr = ptx::smem_u32(sm + C::v);
         bool ok = true;
@@ -470,12 +473,12 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
               const uint32_t d = tmem + C::col_o(qi), pt = tmem + C::col_s(buf);
 #pragma unroll
               for (int k = 0; k < kKeys / 16; ++k) {
-                if constexpr (PAIR) ptx::umma_ts_pair(d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || k > 0);
-                else ptx::umma_ts(d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || k > 0);
+                if constexpr (PAIR) ptx::umma_ts_pair_if(leader, d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || k > 0);
+                else ptx::umma_ts_if(leader, d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || k > 0);
               }
-              commit(C::b_pv_done + qi);
-              commit(C::b_s_free + buf);
-              if (qi == nq - 1) commit(C::b_v_empty + st);
+              commit(leader, C::b_pv_done + qi);
+              commit(leader, C::b_s_free + buf);
+              if (qi == nq - 1) commit(leader, C::b_v_empty + st);
               ++n_p[buf];
             }
           }
