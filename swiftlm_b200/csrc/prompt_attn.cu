@@ -61,12 +61,14 @@ template <int D> struct Cfg {
   static constexpr int k_rows = PAIR ? 64 : 128;            // this CTA's share of a key tile: rows ...
   static constexpr int v_chunks = PAIR ? NC / 2 : NC;       // ... and of a value tile: columns
   static constexpr int k_chunk = k_rows * 128, k_stage = NC * k_chunk, v_stage = v_chunks * kChunk;
-  static constexpr int KS = D == 64 ? 4 : 2, VS = D == 64 ? 6 : 3;
+  // A pair's key stages: the next tile's keys are wanted a period after the stage's last use, its values two; copies take
+  // about 2000 clocks under load (two key and three value stages waited 500 clocks a tile for keys).
+  static constexpr int KS = D == 64 ? 4 : (PAIR ? 3 : 2), VS = D == 64 ? 6 : (PAIR ? 2 : 3);
   static constexpr int q = 0;
   static constexpr int k = QT * NC * kChunk, v = k + KS * k_stage;
   static constexpr int bars = v + VS * v_stage;
   // barriers
-  static constexpr int b_q_full = 0, b_q_empty = 1, b_s_full = 2, b_p_full = 4, b_s_free = 6, b_pv_done = 8, b_o_free = 10,
+  static constexpr int b_q_full = 0, b_q_empty = 1, b_s_full = 2, b_p_half = 4, b_p_full = 6, b_s_free = 8, b_pv_done = 10,
                        b_tail = 12, b_k_full = 13, b_k_empty = b_k_full + KS, b_v_full = b_k_empty + KS, b_v_empty = b_v_full + VS,
                        n_bars = b_v_empty + VS;
   static constexpr int misc = bars + (8 * n_bars + 15) / 16 * 16;   // tensor-memory base, abort flag
@@ -268,10 +270,10 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     ptx::prefetch_tensormap(&map_q);
     ptx::prefetch_tensormap(&map_k);
     ptx::prefetch_tensormap(&map_v);
-    // Arrivals.  P and the freed accumulator: one a softmax warp (4 a query tile; 8 in each CTA of a pair).  Values: the
+    // Arrivals.  P, in two halves: one a softmax warp (4 a query tile; 8 in each CTA of a pair).  Values: the
     // loading lane of each CTA.  A pair's leader has the barriers that its issuing lanes wait for.
     for (int i = 0; i < C::n_bars; ++i) {
-      const bool soft = (i >= C::b_p_full && i < C::b_p_full + 2) || (i >= C::b_o_free && i < C::b_o_free + 2);
+      const bool soft = i >= C::b_p_half && i < C::b_p_full + 2;
       const bool val = i >= C::b_v_full && i < C::b_v_full + VS;
       ptx::mbar_init(&bars[i], soft ? (PAIR ? 16 : 4) : (val && PAIR ? 2 : 1));
     }
@@ -453,7 +455,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       // --------------------------------- O += P V -----------------------------------
       constexpr uint32_t kI = idesc<T>(PAIR ? 256 : 128, D, true);
       if (rank == 0) {
-        uint32_t drain = 0, n_p[2] = {0, 0}, n_seg[2] = {0, 0};
+        uint32_t drain = 0, n_p[2] = {0, 0};
         const uint32_t v_addr = ptx::smem_u32(sm + C::v);
         bool ok = true;
         while (ok && walk.next(s)) {
@@ -463,26 +465,31 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             ok = wait_pair(C::b_v_full + st, (drain / VS) & 1);
             for (int qi = 0; ok && qi < nq; ++qi) {
               const int buf = PAIR ? (int)(drain & 1) : qi;
-              // the first product of a segment overwrites the accumulator: the last segment's result must be out
-              if (j == s.lo && n_seg[qi] > 0) ok = wait(C::b_o_free + qi, (n_seg[qi] - 1) & 1);
-              ok = ok && wait(C::b_p_full + buf, n_p[buf] & 1);
-              if (!ok) break;
-              ptx::tc_fence_after();
-              // 16 keys a step: 2048 bytes of values, 8 columns of P; 64-column chunks lie 16 KiB apart
+              // The weights come in two halves (of every thread's columns), so that the first products run under the
+              // second half's exponentials.  The first half of a segment's first tile also says that the last
+              // segment's accumulator has been read.
               const uint64_t db = make_desc(v_addr + st * C::v_stage, kChunk, 1024);
               const uint32_t d = tmem + C::col_o(qi), pt = tmem + C::col_s(buf);
 #pragma unroll
-              for (int k = 0; k < kKeys / 16; ++k) {
-                if constexpr (PAIR) ptx::umma_ts_pair_if(leader, d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || k > 0);
-                else ptx::umma_ts_if(leader, d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || k > 0);
+              for (int half = 0; half < 2; ++half) {
+                ok = ok && wait((half ? C::b_p_full : C::b_p_half) + buf, n_p[buf] & 1);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                // 16 keys a step: 2048 bytes of values, 8 columns of P; 64-column chunks lie 16 KiB apart
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int k = PAIR ? 4 * (i / 2) + 2 * half + i % 2 : 4 * half + i;
+                  if constexpr (PAIR) ptx::umma_ts_pair_if(leader, d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || half + i > 0);
+                  else ptx::umma_ts_if(leader, d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || half + i > 0);
+                }
               }
+              if (!ok) break;
               commit(leader, C::b_pv_done + qi);
               commit(leader, C::b_s_free + buf);
               if (qi == nq - 1) commit(leader, C::b_v_empty + st);
               ++n_p[buf];
             }
           }
-          for (int qi = 0; qi < nq; ++qi) ++n_seg[qi];
         }
       }
     }
@@ -555,28 +562,11 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         }
         const bool rescale = j > s.lo && __any_sync(0xffffffffu, grow);
         const float neg = m == -INFINITY ? 0.f : -m * p.scale_log2;
-        // P over the first columns of S, which both threads of the row have read
-        float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-        for (int g = 0; g < NS / 32; ++g) {
-          uint32_t pr[16];
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float2 w = fma2(__uint_as_float(sr[g][i]), __uint_as_float(sr[g][i + 1]), p.scale_log2, neg);
-            w.x = mma::exp2_approx(w.x);
-            w.y = mma::exp2_approx(w.y);
-            add[(i >> 1) & 1] = add2(add[(i >> 1) & 1], w);
-            pr[i / 2] = mma::pack<T>(w.x, w.y);
-          }
-          ptx::tmem_st16(s_addr + col0 / 2 + g * 16, pr);
-        }
-        l += (add[0].x + add[0].y) + (add[1].x + add[1].y);
-        // the last product is done with the accumulator; waited for every time and in order (a parity wait that skips a
-        // phase cannot tell "done" from "two phases behind"), after the exponentials, when it rarely waits
-        if (n_s > 0) wait(C::b_pv_done + qi, (n_s - 1) & 1);
-        __syncwarp();
+        // the last product is done with the accumulator
         if (rescale) {
           constexpr int kCols = PAIR ? D / 2 : D;
+          wait(C::b_pv_done + qi, (n_s - 1) & 1);
+          __syncwarp();
           ptx::tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < kCols; c += 32) {
@@ -589,10 +579,32 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             ptx::tmem_st32(o_addr, o);
           }
         }
-        ptx::tmem_st_wait();
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_leader(C::b_p_full + buf);
+        // P over the first columns of S, which both threads of the row have read
+        float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int g = half * (NS / 64); g < (half + 1) * (NS / 64); ++g) {
+            uint32_t pr[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float2 w = fma2(__uint_as_float(sr[g][i]), __uint_as_float(sr[g][i + 1]), p.scale_log2, neg);
+              w.x = mma::exp2_approx(w.x);
+              w.y = mma::exp2_approx(w.y);
+              add[(i >> 1) & 1] = add2(add[(i >> 1) & 1], w);
+              pr[i / 2] = mma::pack<T>(w.x, w.y);
+            }
+            ptx::tmem_st16(s_addr + col0 / 2 + g * 16, pr);
+          }
+          ptx::tmem_st_wait();
+          ptx::tc_fence_before();
+          // Every phase is waited for, in order (a parity wait that skips one cannot tell "done" from "two phases behind"),
+          // and before the next one can end, which takes this warp's arrival.
+          if (half && n_s > 0) wait(C::b_pv_done + qi, (n_s - 1) & 1);
+          __syncwarp();
+          if (lane == 0) arrive_leader((half ? C::b_p_full : C::b_p_half) + buf);
+        }
+        l += (add[0].x + add[0].y) + (add[1].x + add[1].y);
       }
       // ---- the segment's result ----
       wait(C::b_pv_done + qi, (n_s - 1) & 1);
@@ -631,9 +643,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             dst[(i / 4) * 256] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
         }
       }
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_leader(C::b_o_free + qi);
+      ptx::tc_fence_before();              // the next segment's first half of P says that the accumulator has been read
       if (!PAIR || grp == 0) {
         if (s.slot >= 0) p.part_ml[(long long)s.slot * 256 + tile * 128 + r] = make_float2(m * p.scale_log2, l);
         else if (used && a.lse) a.lse[row] = l > 0.f ? (m * p.scale_log2 + log2f(l)) * kLn2 : -INFINITY;
