@@ -7,14 +7,15 @@
 // exponentials of a tile (16 a clock per SM, 1024 clocks; a tile's two products take 1024 at D = 128, 2048 at 256).
 //
 // * A query tile is 128 rows: the heads of one KV head for consecutive tokens (tc_common.cuh); a unit of work has two.
-//   D <= 128: one CTA takes both, each with its score columns and accumulator in tensor memory and a softmax warpgroup
-//   (one thread a row); the tiles take turns, one's products run under the other's exponentials, and a key tile is
+//   D <= 128: one CTA takes both, each with its score columns and accumulator in tensor memory and two softmax
+//   warpgroups; the tiles take turns, one's products run under the other's exponentials, and a key tile is
 //   loaded once for both.  D = 256: the accumulator takes half of the tensor memory, so a pair of CTAs takes a unit with
 //   products of 256 rows across the two SMs (cta_group::2), each holding its query tile, two score buffers, half of the
-//   keys of a tile and half of the value columns; two threads share a row.  One CTA alone would read 128 KiB of keys and
+//   keys of a tile and half of the value columns.  One CTA alone would read 128 KiB of keys and
 //   values from L2 for each 128 x 128 tile: that ran at 4600 clocks a tile, waiting for L2 and for shared memory.
 // * Warps: 0 loads queries and keys, 1 values, 2 issues S = Q K^T, 3 issues O += P V (P replaces S in tensor memory,
-//   in the inputs' type: the product needs a 16-bit operand), 4-11 softmax.
+//   in the inputs' type: the product needs a 16-bit operand), the others softmax, two threads a row: with one
+//   the row's 128 exponentials were a chain of 4000 clocks.
 // * Only the key tiles that some row of the unit sees are visited; only those that some row does not see whole are masked.
 //   Value rows behind the sequence's length are zeroed in shared memory before the product, whatever the cache holds there.
 // * Persistent CTAs, one per SM.  plan_kernel lays the key tiles of all units in a row and cuts them into equal ranges, so
@@ -30,11 +31,7 @@ using namespace tc;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescale = 8.f;              // in log2 units
-constexpr int kThreads = 384;
 constexpr int kMinCut = 4;
-// registers: 384 threads launched with 168 each; what the four helper warps give up the softmax warps take
-constexpr int kRegsLaunch = 168, kRegsHelper = 56, kRegsSoftmax = 216;
-static_assert(128 * kRegsHelper + 256 * kRegsSoftmax <= kThreads * kRegsLaunch, "register split");
 
 struct Boundary { long long unit; int off, pad; long long pos; };
 struct Cut { long long unit; int first, count; };
@@ -58,6 +55,10 @@ template <int D> struct Cfg {
   static constexpr bool PAIR = D == 256;                    // two CTAs on one unit, a query tile each
   static constexpr int NC = D / 64;                         // 64-column chunks of a row
   static constexpr int QT = PAIR ? 1 : 2;                   // query tiles of one CTA (a unit has two)
+  static constexpr int threads = 128 + QT * 256;            // four helper warps, eight softmax warps a query tile
+  // registers a thread at launch; what the helper warps give up the softmax warps take
+  static constexpr int regs_launch = PAIR ? 168 : 96, regs_helper = 56, regs_softmax = PAIR ? 216 : 104;
+  static_assert(128 * regs_helper + (threads - 128) * regs_softmax <= threads * regs_launch, "register split");
   static constexpr int k_rows = PAIR ? 64 : 128;            // this CTA's share of a key tile: rows ...
   static constexpr int v_chunks = PAIR ? NC / 2 : NC;       // ... and of a value tile: columns
   static constexpr int k_chunk = k_rows * 128, k_stage = NC * k_chunk, v_stage = v_chunks * kChunk;
@@ -72,8 +73,9 @@ template <int D> struct Cfg {
                        b_tail = 12, b_k_full = 13, b_k_empty = b_k_full + KS, b_v_full = b_k_empty + KS, b_v_empty = b_v_full + VS,
                        n_bars = b_v_empty + VS;
   static constexpr int misc = bars + (8 * n_bars + 15) / 16 * 16;   // tensor-memory base, abort flag
-  static constexpr int xch = misc + 16;                     // [2][2][128] row maxima of the two halves (D = 256)
-  static constexpr int total = xch + (PAIR ? 2 * 2 * 128 * 4 : 0);
+  static constexpr int xch = misc + 16;                     // row maxima (sums) of the two halves: [QT][slots][2][128]
+  static constexpr int slots = PAIR ? 2 : 1;
+  static constexpr int total = xch + QT * slots * 2 * 128 * 4;
   // tensor-memory columns: accumulators first, score buffers in the upper half
   __host__ __device__ static constexpr int col_o(int qi) { return qi * 128; }
   __host__ __device__ static constexpr int col_s(int i) { return 256 + i * 128; }
@@ -252,7 +254,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Cfg<D>::threads, 1)
 prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
               const __grid_constant__ CUtensorMap map_v, const PromptParams p) {
   using C = Cfg<D>;
@@ -275,7 +277,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     for (int i = 0; i < C::n_bars; ++i) {
       const bool soft = i >= C::b_p_half && i < C::b_p_full + 2;
       const bool val = i >= C::b_v_full && i < C::b_v_full + VS;
-      ptx::mbar_init(&bars[i], soft ? (PAIR ? 16 : 4) : (val && PAIR ? 2 : 1));
+      ptx::mbar_init(&bars[i], soft ? (PAIR ? 16 : 8) : (val && PAIR ? 2 : 1));
     }
     *abort_flag = (ptx::smem_u32(sm) & 1023u) != 0u;      // swizzled tiles need 1024-byte alignment; never seen violated
     if (*abort_flag) atomicExch(a.status, kStatusSmemAlign);
@@ -313,9 +315,9 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
   };
   auto wait = [&](int bar, uint32_t parity) { return wait_as(bar, parity, false); };
   auto wait_pair = [&](int bar, uint32_t parity) { return wait_as(bar, parity, true); };   // the other CTA's stores among what is waited for
-  auto commit = [&](uint32_t leader, int bar) {
-    if constexpr (PAIR) ptx::umma_commit_pair_if(leader, &bars[bar]);
-    else ptx::umma_commit_if(leader, &bars[bar]);
+  auto commit = [&](int bar) {
+    if constexpr (PAIR) ptx::umma_commit_pair(&bars[bar]);
+    else ptx::umma_commit(&bars[bar]);
   };
   // the leader's barrier, for arrivals and copies of both CTAs
   auto arrive_leader = [&](int bar) {
@@ -327,11 +329,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     else ptx::tma_load_4d(dst, m, x, y, z, w, &bars[bar]);
   };
 
-  // The issuing warps run converged, every lane with the same operands, and one lane issues: operands of a diverged lane
-  // would each be moved to uniform registers first.
-  const uint32_t leader = lane == 0;
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsHelper));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::regs_helper));
     Walker walk(p, worker);
     Segment s;
     if (warp == 0) {
@@ -431,23 +430,26 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
               if (n_s[buf] > 0) ok = wait(C::b_s_free + buf, (n_s[buf] - 1) & 1);
               if (!ok) break;
               ptx::tc_fence_after();
-              const uint32_t d = tmem + C::col_s(buf);
+              if (ptx::elect_one()) {
+                const uint32_t d = tmem + C::col_s(buf);
 #pragma unroll
-              for (int c = 0; c < NC; ++c) {
-                const uint64_t da = make_desc(q_addr + (qi * NC + c) * kChunk, 16, 1024);
-                const uint64_t db = make_desc(k_addr + st * C::k_stage + c * C::k_chunk, 16, 1024);
+                for (int c = 0; c < NC; ++c) {
+                  const uint64_t da = make_desc(q_addr + (qi * NC + c) * kChunk, 16, 1024);
+                  const uint64_t db = make_desc(k_addr + st * C::k_stage + c * C::k_chunk, 16, 1024);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  if constexpr (PAIR) ptx::umma_ss_pair_if(leader, d, da + 2 * k, db + 2 * k, kI, c + k > 0);
-                  else ptx::umma_ss_if(leader, d, da + 2 * k, db + 2 * k, kI, c + k > 0);
+                  for (int k = 0; k < 4; ++k) {
+                    if constexpr (PAIR) ptx::umma_ss_pair(d, da + 2 * k, db + 2 * k, kI, c + k > 0);
+                    else ptx::umma_ss(d, da + 2 * k, db + 2 * k, kI, c + k > 0);
+                  }
                 }
+                commit(C::b_s_full + buf);
+                if (qi == nq - 1) commit(C::b_k_empty + st);
+                if (qi == nq - 1 && j == s.hi - 1) commit(C::b_q_empty);
               }
-              commit(leader, C::b_s_full + buf);
-              if (qi == nq - 1) commit(leader, C::b_k_empty + st);
+              __syncwarp();
               ++n_s[buf];
             }
           }
-          commit(leader, C::b_q_empty);
           ++seg;
         }
       }
@@ -475,18 +477,23 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 ok = ok && wait((half ? C::b_p_full : C::b_p_half) + buf, n_p[buf] & 1);
                 if (!ok) break;
                 ptx::tc_fence_after();
-                // 16 keys a step: 2048 bytes of values, 8 columns of P; 64-column chunks lie 16 KiB apart
+                if (ptx::elect_one()) {
+                  // 16 keys a step: 2048 bytes of values, 8 columns of P; 64-column chunks lie 16 KiB apart
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const int k = PAIR ? 4 * (i / 2) + 2 * half + i % 2 : 4 * half + i;
-                  if constexpr (PAIR) ptx::umma_ts_pair_if(leader, d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || half + i > 0);
-                  else ptx::umma_ts_if(leader, d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || half + i > 0);
+                  for (int i = 0; i < 4; ++i) {
+                    const int k = 4 * (i / 2) + 2 * half + i % 2;
+                    if constexpr (PAIR) ptx::umma_ts_pair(d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || half + i > 0);
+                    else ptx::umma_ts(d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || half + i > 0);
+                  }
+                  if (half) {
+                    commit(C::b_pv_done + qi);
+                    commit(C::b_s_free + buf);
+                    if (qi == nq - 1) commit(C::b_v_empty + st);
+                  }
                 }
+                __syncwarp();
               }
               if (!ok) break;
-              commit(leader, C::b_pv_done + qi);
-              commit(leader, C::b_s_free + buf);
-              if (qi == nq - 1) commit(leader, C::b_v_empty + st);
               ++n_p[buf];
             }
           }
@@ -494,23 +501,24 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::regs_softmax));
     // ----------------------------------- softmax ------------------------------------
     Walker walk(p, worker);
     Segment s;
-    const int wq = warp & 3, grp = (warp - 4) >> 2;           // tensor-memory lane quarter; query tile, or half of the row
+    const int wq = warp & 3, grp = ((warp - 4) >> 2) & 1;     // tensor-memory lane quarter; half of the row
     const int r = wq * 32 + lane;
     const uint32_t lane_addr = tmem + ((uint32_t)(wq * 32) << 16);
-    const int qi = PAIR ? 0 : grp, tile = PAIR ? rank : grp;  // query tile of this CTA, of the unit
-    constexpr int NS = PAIR ? 64 : 128;                       // score columns of this thread
-    const int col0 = PAIR ? grp * 64 : 0;
-    float* xch = reinterpret_cast<float*>(sm + C::xch);
+    const int qi = (warp - 4) >> 3, tile = PAIR ? rank : qi;  // query tile of this CTA, of the unit
+    constexpr int NS = 64;                                    // score columns of this thread
+    const int col0 = grp * 64;
+    float* xch = reinterpret_cast<float*>(sm + C::xch) + qi * C::slots * 256;
     uint32_t n_s = 0, n_x = 0;                                // score tiles and exchanges done
-    // value of the thread that has the other half of this row; the two warps always meet the same number of times
+    // Value of the thread that has the other half of this row; the two warps always meet the same number of times.  With
+    // one slot the next value is written only after this one has been read: the next tile's scores take both threads' P.
     auto other_half = [&](float mine) {
-      float* x = xch + (n_x++ & 1) * 256;
+      float* x = xch + n_x++ % C::slots * 256;
       x[grp * 128 + r] = mine;
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + wq) : "memory");
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + qi * 4 + wq) : "memory");
       return x[(grp ^ 1) * 128 + r];
     };
     while (walk.next(s)) {
@@ -552,7 +560,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         for (int i = 0; i < NS; i += 2)
           mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(sr[i / 32][i % 32]), __uint_as_float(sr[i / 32][i % 32 + 1]));
         float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-        if (PAIR) mx = fmaxf(mx, other_half(mx));
+        mx = fmaxf(mx, other_half(mx));
         float f = 1.f;
         const bool grow = mx > m && (m == -INFINITY || (mx - m) * p.scale_log2 > kRescale);
         if (grow) {
@@ -564,14 +572,14 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         const float neg = m == -INFINITY ? 0.f : -m * p.scale_log2;
         // the last product is done with the accumulator
         if (rescale) {
-          constexpr int kCols = PAIR ? D / 2 : D;
+          constexpr int kCols = D / 2;
           wait(C::b_pv_done + qi, (n_s - 1) & 1);
           __syncwarp();
           ptx::tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < kCols; c += 32) {
             uint32_t o[32];
-            const uint32_t o_addr = lane_addr + C::col_o(qi) + (PAIR ? grp * kCols : 0) + c;
+            const uint32_t o_addr = lane_addr + C::col_o(qi) + grp * kCols + c;
             ptx::tmem_ld32(o_addr, o);
             ptx::tmem_ld_wait();
 #pragma unroll
@@ -610,12 +618,13 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       wait(C::b_pv_done + qi, (n_s - 1) & 1);
       __syncwarp();
       ptx::tc_fence_after();
-      if (PAIR) {                                              // the same order of the two halves in both threads
+      {                                                        // the same order of the two halves in both threads
         const float x = other_half(l);
         l = grp == 0 ? l + x : x + l;
+        if (C::slots == 1) asm volatile("bar.sync %0, 64;" ::"r"(1 + qi * 4 + wq) : "memory");
       }
-      constexpr int kCols = PAIR ? D / 2 : D;
-      const int c0 = PAIR ? grp * kCols : 0;
+      constexpr int kCols = D / 2;
+      const int c0 = grp * kCols;
       const float inv = l > 0.f ? 1.f / l : 0.f;
 #pragma unroll 1
       for (int c = 0; c < kCols; c += 32) {
@@ -644,7 +653,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         }
       }
       ptx::tc_fence_before();              // the next segment's first half of P says that the accumulator has been read
-      if (!PAIR || grp == 0) {
+      if (grp == 0) {
         if (s.slot >= 0) p.part_ml[(long long)s.slot * 256 + tile * 128 + r] = make_float2(m * p.scale_log2, l);
         else if (used && a.lse) a.lse[row] = l > 0.f ? (m * p.scale_log2 + log2f(l)) * kLn2 : -INFINITY;
       }
@@ -759,7 +768,7 @@ int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
   DFLASH_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::total));
   // the register hand-over waits for good if the launch gives the CTA fewer than it takes
   static const int regs = [&] { cudaFuncAttributes f; return cudaFuncGetAttributes(&f, kernel) == cudaSuccess ? f.numRegs : 0; }();
-  if (regs != kRegsLaunch) { set_error("prompt_sdpa: the kernel is launched with %d registers a thread, %d expected", regs, kRegsLaunch); return DFLASH_ERR_CUDA; }
+  if (regs != C::regs_launch) { set_error("prompt_sdpa: the kernel is launched with %d registers a thread, %d expected", regs, C::regs_launch); return DFLASH_ERR_CUDA; }
   plan_kernel<<<1, 1024, 0, stream>>>(p, 2 * x.t.Tt);
   DFLASH_LAUNCH_CHECK();
   cudaLaunchConfig_t cfg = {};
@@ -773,7 +782,7 @@ int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
   cfg.numAttrs = C::PAIR ? 2 : 1;
   cfg.stream = stream;
   cfg.gridDim = dim3(x.grid * (C::PAIR ? 2 : 1));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(C::threads);
   cfg.dynamicSmemBytes = C::total;
   DFLASH_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, p));
   cfg.numAttrs = 1;
