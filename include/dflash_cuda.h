@@ -246,6 +246,7 @@ int32_t dflash_kv_commit(int32_t* kv_len, const int32_t* commit, int32_t B, int3
  *   lse        fp32, natural logarithm of the sum of exp(scale * q.k) over the visible tokens.
  *   mass       fp32 [B,Hkv,mass_stride], mass_stride >= N: the weight every cached token has received, summed over
  *              the query heads of its KV head.  Always added to, in an order that does not change from run to run.
+ *   scale      positive, 1e-30 .. 1e30.
  *   Supported: dtype bf16 / f16, D in {64, 128, 256}, Hq % Hkv == 0.  Neither outputs nor workspace may overlap
  *   another argument unless it is said.
  */

@@ -19,7 +19,7 @@ int32_t check(const char* op, CacheArgs& a) {
   if (a.D != 64 && a.D != 128 && a.D != 256) { set_error("%s: unsupported head_dim %d (64, 128 or 256)", op, a.D); return DFLASH_ERR_UNSUPPORTED; }
   if (a.Hq % a.Hkv != 0) { set_error("%s: unsupported heads: Hq=%d not a multiple of Hkv=%d", op, a.Hq, a.Hkv); return DFLASH_ERR_UNSUPPORTED; }
   if (a.window < 0 || a.sinks < 0) return invalid(op, "negative window or sinks");
-  if (!(a.scale - a.scale == 0.f)) return invalid(op, "scale is not finite");
+  if (!(a.scale >= 1e-30f && a.scale <= 1e30f)) return invalid(op, "scale must be positive and finite");   // running maxima assume its sign
   if (a.page_table) {
     if (a.page_tokens <= 0 || a.max_pages <= 0 || a.num_pages <= 0 || (long long)a.max_pages * a.page_tokens < a.N)
       return invalid(op, "paged KV needs page_tokens, num_pages and max_pages * page_tokens >= N");

@@ -43,7 +43,6 @@ struct PromptParams {
   int box;
   int grid;
   float scale_log2;
-  int negate;                  // scale < 0: the scores change sign first
   long long* steps;            // [B * NTT + 1] key tiles in front of every (sequence, unit)
   Boundary* bounds;            // [grid + 1]
   Cut* cuts;                   // [grid]
@@ -69,7 +68,7 @@ template <int D> struct Cfg {
   static constexpr int k = QT * NC * kChunk, v = k + KS * k_stage;
   static constexpr int bars = v + VS * v_stage;
   // barriers
-  static constexpr int b_q_full = 0, b_q_empty = 1, b_s_full = 2, b_p_half = 4, b_p_full = 6, b_s_free = 8, b_pv_done = 10,
+  static constexpr int b_q_full = 0, b_q_empty = 1, b_s_full = 2, b_p_half = 4, b_s_free = 8, b_pv_done = 10,
                        b_tail = 12, b_k_full = 13, b_k_empty = b_k_full + KS, b_v_full = b_k_empty + KS, b_v_empty = b_v_full + VS,
                        n_bars = b_v_empty + VS;
   static constexpr int misc = bars + (8 * n_bars + 15) / 16 * 16;   // tensor-memory base, abort flag
@@ -275,7 +274,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     // Arrivals.  P, in two halves: one a softmax warp (4 a query tile; 8 in each CTA of a pair).  Values: the
     // loading lane of each CTA.  A pair's leader has the barriers that its issuing lanes wait for.
     for (int i = 0; i < C::n_bars; ++i) {
-      const bool soft = i >= C::b_p_half && i < C::b_p_full + 2;
+      const bool soft = i >= C::b_p_half && i < C::b_p_half + 4;
       const bool val = i >= C::b_v_full && i < C::b_v_full + VS;
       ptx::mbar_init(&bars[i], soft ? (PAIR ? 16 : 8) : (val && PAIR ? 2 : 1));
     }
@@ -301,6 +300,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
   // A wait that gives up raises the abort flags, after which every wait of the CTA (or pair) returns at once: the roles run
   // through their loops without results, meet at the end and leave.
   auto wait_as = [&](int bar, uint32_t parity, bool cluster) {
+#pragma unroll 1
     for (uint32_t i = 0; i < ptx::kWaitPolls; ++i) {
       if (PAIR && cluster ? ptx::mbar_try_wait_cluster(&bars[bar], parity) : ptx::mbar_try_wait(&bars[bar], parity)) return true;
       if ((i & 63u) == 63u) {
@@ -432,7 +432,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
               ptx::tc_fence_after();
               if (ptx::elect_one()) {
                 const uint32_t d = tmem + C::col_s(buf);
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < NC; ++c) {
                   const uint64_t da = make_desc(q_addr + (qi * NC + c) * kChunk, 16, 1024);
                   const uint64_t db = make_desc(k_addr + st * C::k_stage + c * C::k_chunk, 16, 1024);
@@ -472,18 +472,19 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
               // segment's accumulator has been read.
               const uint64_t db = make_desc(v_addr + st * C::v_stage, kChunk, 1024);
               const uint32_t d = tmem + C::col_o(qi), pt = tmem + C::col_s(buf);
-#pragma unroll
+#pragma unroll 1
               for (int half = 0; half < 2; ++half) {
-                ok = ok && wait((half ? C::b_p_full : C::b_p_half) + buf, n_p[buf] & 1);
+                ok = ok && wait(C::b_p_half + 2 * half + buf, n_p[buf] & 1);
                 if (!ok) break;
                 ptx::tc_fence_after();
                 if (ptx::elect_one()) {
-                  // 16 keys a step: 2048 bytes of values, 8 columns of P; 64-column chunks lie 16 KiB apart
+                  // 16 keys a step: 2048 bytes of values, 8 columns of P (those of the second 64 keys start at column 64); 64-column
+                  // chunks of values lie 16 KiB apart
 #pragma unroll
                   for (int i = 0; i < 4; ++i) {
-                    const int k = 4 * (i / 2) + 2 * half + i % 2;
-                    if constexpr (PAIR) ptx::umma_ts_pair(d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || half + i > 0);
-                    else ptx::umma_ts(d, pt + k * 8, db + (uint64_t)k * 128, kI, j > s.lo || half + i > 0);
+                    const int k = 4 * (i / 2) + 2 * half + i % 2, pc = 64 * (i / 2) + 16 * half + 8 * (i % 2);
+                    if constexpr (PAIR) ptx::umma_ts_pair(d, pt + pc, db + (uint64_t)k * 128, kI, j > s.lo || half + i > 0);
+                    else ptx::umma_ts(d, pt + pc, db + (uint64_t)k * 128, kI, j > s.lo || half + i > 0);
                   }
                   if (half) {
                     commit(C::b_pv_done + qi);
@@ -534,32 +535,31 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         wait(C::b_s_full + buf, PAIR ? (n_s >> 1) & 1 : n_s & 1);
         __syncwarp();
         ptx::tc_fence_after();
-        const uint32_t s_addr = lane_addr + C::col_s(buf);
-        uint32_t sr[NS / 32][32];
-#pragma unroll
-        for (int i = 0; i < NS / 32; ++i) ptx::tmem_ld32(s_addr + col0 + i * 32, sr[i]);
-        ptx::tmem_ld_wait();
+        const uint32_t s_addr = lane_addr + C::col_s(buf) + col0;
         const int n0 = tile_key(s.u.k, j);
-        if (p.negate) {
-#pragma unroll
-          for (int i = 0; i < NS; ++i) sr[i / 32][i % 32] ^= 0x80000000u;
-        }
         const bool whole = n0 + kKeys - 1 <= p_min && (a.window == 0 || n0 > p_max - a.window || n0 + kKeys <= a.sinks);
-        if (!whole) {
-          const int hi = pos - n0 - col0 + 1, lo = a.window > 0 ? hi - a.window : 0, sink = a.sinks - n0 - col0;
-#pragma unroll
-          for (int g = 0; g < NS / 32; ++g) {
-            const uint32_t seen = low_bits(hi - g * 32) & (~low_bits(lo - g * 32) | low_bits(sink - g * 32));
+        // Loops of 32 scores, not unrolled further, and read from tensor memory a second time for the exponentials: the
+        // loop of 64 unrolled scores ran at half the speed, a fifth of the instruction fetches missing.
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int g = 0; g < NS; g += 32) {
+          uint32_t x[32];
+          ptx::tmem_ld32(s_addr + g, x);
+          ptx::tmem_ld_wait();
+          if (!whole) {                                       // hidden scores go back as -infinity
+            const int hi = pos - n0 - col0 - g + 1, lo = a.window > 0 ? hi - a.window : 0, sink = a.sinks - n0 - col0 - g;
+            const uint32_t seen = low_bits(hi) & (~low_bits(lo) | low_bits(sink));
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (!((seen >> i) & 1u)) sr[g][i] = __float_as_uint(-INFINITY);
+              if (!((seen >> i) & 1u)) x[i] = __float_as_uint(-INFINITY);
+            ptx::tmem_st32(s_addr + g, x);
           }
-        }
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < NS; i += 2)
-          mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(sr[i / 32][i % 32]), __uint_as_float(sr[i / 32][i % 32 + 1]));
-        float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+          for (int i = 0; i < 32; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        }
+        if (!whole) ptx::tmem_st_wait();
         mx = fmaxf(mx, other_half(mx));
         float f = 1.f;
         const bool grow = mx > m && (m == -INFINITY || (mx - m) * p.scale_log2 > kRescale);
@@ -587,30 +587,29 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             ptx::tmem_st32(o_addr, o);
           }
         }
-        // P over the first columns of S, which both threads of the row have read
+        // P over the front half of this thread's own columns, in two halves
         float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
+#pragma unroll 1
         for (int half = 0; half < 2; ++half) {
+          uint32_t x[32], pr[16];
+          ptx::tmem_ld32(s_addr + half * 32, x);
+          ptx::tmem_ld_wait();
 #pragma unroll
-          for (int g = half * (NS / 64); g < (half + 1) * (NS / 64); ++g) {
-            uint32_t pr[16];
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float2 w = fma2(__uint_as_float(sr[g][i]), __uint_as_float(sr[g][i + 1]), p.scale_log2, neg);
-              w.x = mma::exp2_approx(w.x);
-              w.y = mma::exp2_approx(w.y);
-              add[(i >> 1) & 1] = add2(add[(i >> 1) & 1], w);
-              pr[i / 2] = mma::pack<T>(w.x, w.y);
-            }
-            ptx::tmem_st16(s_addr + col0 / 2 + g * 16, pr);
+          for (int i = 0; i < 32; i += 2) {
+            float2 w = fma2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), p.scale_log2, neg);
+            w.x = mma::exp2_approx(w.x);
+            w.y = mma::exp2_approx(w.y);
+            add[(i >> 1) & 1] = add2(add[(i >> 1) & 1], w);
+            pr[i / 2] = mma::pack<T>(w.x, w.y);
           }
+          ptx::tmem_st16(s_addr + half * 16, pr);
           ptx::tmem_st_wait();
           ptx::tc_fence_before();
           // Every phase is waited for, in order (a parity wait that skips one cannot tell "done" from "two phases behind"),
           // and before the next one can end, which takes this warp's arrival.
           if (half && n_s > 0) wait(C::b_pv_done + qi, (n_s - 1) & 1);
           __syncwarp();
-          if (lane == 0) arrive_leader((half ? C::b_p_full : C::b_p_half) + buf);
+          if (lane == 0) arrive_leader(C::b_p_half + 2 * half + buf);
         }
         l += (add[0].x + add[0].y) + (add[1].x + add[1].y);
       }
@@ -749,10 +748,7 @@ int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
   p.NTT = x.NTT;
   p.box = box_rows(a);
   p.grid = x.grid;
-  // a scale of zero as one too small to matter: -inf times it has to stay -inf
-  const float s = a.scale < 0.f ? -a.scale : a.scale;
-  p.scale_log2 = (s < 1e-30f ? 1e-30f : s) * kLog2e;
-  p.negate = a.scale < 0.f;
+  p.scale_log2 = a.scale * kLog2e;
   uint8_t* ws = reinterpret_cast<uint8_t*>(a.workspace);
   p.steps = reinterpret_cast<long long*>(ws);
   p.bounds = reinterpret_cast<Boundary*>(ws += x.steps);

@@ -37,6 +37,7 @@ def test_attention_refusals(op):
     assert call(op, Hq=15) == un
     assert call(op, window=-1) == bad and call(op, sinks=-1) == bad
     assert call(op, scale=float("nan")) == bad and call(op, scale=float("inf")) == bad
+    assert call(op, scale=0.0) == bad and call(op, scale=-0.1) == bad and call(op, scale=1e-38) == bad
     assert call(op, q=FAKE + 8) == bad and call(op, k=FAKE + 2) == bad
     assert call(op, page_table=FAKE, page_tokens=24, max_pages=9, num_pages=9) == un
     assert call(op, page_table=FAKE, page_tokens=16, max_pages=3, num_pages=9) == bad      # 48 < N
