@@ -31,9 +31,10 @@ using namespace tc;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescale = 8.f;              // in log2 units
-constexpr int kMinCut = 4;
+constexpr int kMinCut = 4;                   // key tiles of the smallest piece of a cut unit
+constexpr int kUnitCost = 3;                 // what a unit costs besides its key tiles (loading queries, storing rows), in tiles
 
-struct Boundary { long long unit; int off, pad; long long pos; };
+struct Boundary { long long unit; int off, pad; };   // in front of key tile `off` of a unit
 struct Cut { long long unit; int first, count; };
 
 struct PromptParams {
@@ -43,12 +44,15 @@ struct PromptParams {
   int box;
   int grid;
   float scale_log2;
-  long long* steps;            // [B * NTT + 1] key tiles in front of every (sequence, unit)
+  int out32;                   // `out` is 32-byte aligned
+  long long* cost;             // [B * NTT + 1] cost of what is in front of every (sequence, unit)
   Boundary* bounds;            // [grid + 1]
   Cut* cuts;                   // [grid]
   float4* part_o;              // [2 * grid][D / 4][256]
   float2* part_ml;             // [2 * grid][256]
 };
+
+constexpr int kMaxGrid = 1023;                // workers at most: a boundary for each thread of plan_kernel
 
 template <int D> struct Cfg {
   static constexpr bool PAIR = D == 256;                    // two CTAs on one unit, a query tile each
@@ -82,11 +86,11 @@ template <int D> struct Cfg {
 static_assert(Cfg<256>::total <= 232448 && Cfg<128>::total <= 232448 && Cfg<64>::total <= 232448, "shared memory");
 
 // ---- the plan ----
-__device__ __forceinline__ int unit_steps(const PromptParams& p, RowLens len, int tt, int tokens) {
+__device__ __forceinline__ int unit_cost(const PromptParams& p, RowLens len, int tt, int tokens) {
   const int t0 = tt * tokens;
   if (t0 >= len.rows) return 0;
   const int t1 = t0 + tokens < len.rows ? t0 + tokens : len.rows;
-  return key_tiles(p.a, len, t0, t1).count;
+  return kUnitCost + key_tiles(p.a, len, t0, t1).count;
 }
 
 __global__ void __launch_bounds__(1024) plan_kernel(const PromptParams p, int tokens) {
@@ -101,7 +105,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PromptParams p, int to
   for (long long e = e0; e < e1; ++e) {
     const int eb = (int)(e / p.NTT);
     if (eb != b) { b = eb; len = lens_of(p.a, b, true); }
-    mine += unit_steps(p, len, (int)(e - (long long)b * p.NTT), tokens);
+    mine += unit_cost(p, len, (int)(e - (long long)b * p.NTT), tokens);
   }
   long long x = mine;
 #pragma unroll
@@ -117,43 +121,61 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PromptParams p, int to
   for (long long e = e0; e < e1; ++e) {
     const int eb = (int)(e / p.NTT);
     if (eb != b) { b = eb; len = lens_of(p.a, b); }
-    p.steps[e] = at;
-    at += unit_steps(p, len, (int)(e - (long long)b * p.NTT), tokens);
+    p.cost[e] = at;
+    at += unit_cost(p, len, (int)(e - (long long)b * p.NTT), tokens);
   }
   long long all = 0;
   for (int w = 0; w < 32; ++w) all += warp_sums[w];
-  if (tid == 0) p.steps[E] = all;
+  if (tid == 0) p.cost[E] = all;
   __syncthreads();               // the table is read by other threads of this block below
   const long long total = all * HG;
-  long long per = (total + p.grid - 1) / p.grid;
-  if (per < kMinCut) per = kMinCut;
-  for (int c = tid; c <= p.grid; c += 1024) {
-    long long pos = c * per;
-    Boundary r{E * HG, 0, 0, total};
+  const long long per = total > p.grid ? (total + p.grid - 1) / p.grid : 1;
+  __shared__ Boundary raw[kMaxGrid + 1];
+  if (tid <= p.grid) {
+    const int c = tid;
+    const long long pos = c * per;
+    Boundary r{E * HG, 0, 0};
     if (pos < total) {
       int lo = 0, hi = p.a.B - 1;             // the last sequence that starts at or before pos
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (p.steps[(long long)mid * p.NTT] * HG <= pos) lo = mid; else hi = mid - 1;
+        if (p.cost[(long long)mid * p.NTT] * HG <= pos) lo = mid; else hi = mid - 1;
       }
-      const long long base = p.steps[(long long)lo * p.NTT], len_b = p.steps[(long long)(lo + 1) * p.NTT] - base;
+      const long long base = p.cost[(long long)lo * p.NTT], len_b = p.cost[(long long)(lo + 1) * p.NTT] - base;
       const long long hg = (pos - base * HG) / len_b, rem = pos - base * HG - hg * len_b;
       int ta = 0, tb = p.NTT - 1;             // the last unit that starts at or before rem
       while (ta < tb) {
         const int mid = (ta + tb + 1) >> 1;
-        if (p.steps[(long long)lo * p.NTT + mid] - base <= rem) ta = mid; else tb = mid - 1;
+        if (p.cost[(long long)lo * p.NTT + mid] - base <= rem) ta = mid; else tb = mid - 1;
       }
-      const long long s = p.steps[(long long)lo * p.NTT + ta] - base, e = p.steps[(long long)lo * p.NTT + ta + 1] - base;
+      const long long s = p.cost[(long long)lo * p.NTT + ta] - base, e = p.cost[(long long)lo * p.NTT + ta + 1] - base;
       const long long unit = ((long long)lo * HG + hg) * p.NTT + ta;
-      const int off = (int)(rem - s), size = (int)(e - s);
-      if (off < kMinCut) r = Boundary{unit, 0, 0, pos - off};
-      else if (size - off < kMinCut) r = Boundary{unit + 1, 0, 0, pos - off + size};
-      else r = Boundary{unit, off, 0, pos};
+      const int size = (int)(e - s) - kUnitCost;
+      int off = (int)(rem - s) - kUnitCost;
+      off = off < 0 ? 0 : off / kMinCut * kMinCut;
+      const bool back = size < kMinCut ? 2 * (rem - s) >= e - s : size - off < kMinCut;    // the unit's end is nearer
+      r = back ? Boundary{unit + 1, 0, 0} : Boundary{unit, off, 0};
     }
-    p.bounds[c] = r;
+    raw[c] = r;
   }
   __syncthreads();
-  for (int c = tid; c < p.grid; c += 1024) {
+  // equal boundaries become one, so that the pieces of a cut unit belong to workers in a row
+  {
+    const bool fresh = tid <= p.grid && (tid == 0 || raw[tid].unit != raw[tid - 1].unit || raw[tid].off != raw[tid - 1].off);
+    const uint32_t in_warp = __ballot_sync(0xffffffffu, fresh);
+    if (lane == 0) warp_sums[warp] = __popc(in_warp);
+    __syncthreads();
+    int before = 0, all_fresh = 0;
+    for (int w = 0; w < 32; ++w) {
+      before += w < warp ? (int)warp_sums[w] : 0;
+      all_fresh += (int)warp_sums[w];
+    }
+    if (fresh) p.bounds[before + __popc(in_warp & ((1u << lane) - 1u))] = raw[tid];
+    if (tid >= all_fresh && tid <= p.grid) p.bounds[tid] = Boundary{E * HG, 0, 0};
+  }
+  __syncthreads();
+  if (tid < p.grid) {
+    const int c = tid;
     Cut cut{0, 0, 0};
     if (c >= 1 && p.bounds[c].off > 0 && !(p.bounds[c - 1].off > 0 && p.bounds[c - 1].unit == p.bounds[c].unit)) {
       int n = 1;
@@ -169,20 +191,6 @@ struct Unit {
   RowLens len;
   KeyTiles k;
 };
-__device__ __forceinline__ Unit unit_at(const PromptParams& p, long long unit, int tokens) {
-  Unit u;
-  const int HG = p.a.Hkv * p.t.GC;
-  const long long bhg = unit / p.NTT;
-  u.t0 = (int)(unit - bhg * p.NTT) * tokens;
-  u.b = (int)(bhg / HG);
-  const int hg = (int)(bhg - (long long)u.b * HG);
-  u.h = hg / p.t.GC;
-  u.gc = hg - u.h * p.t.GC;
-  u.len = lens_of(p.a, u.b);
-  const int t1 = u.t0 + tokens < u.len.rows ? u.t0 + tokens : u.len.rows;
-  u.k = key_tiles(p.a, u.len, u.t0, t1);
-  return u;
-}
 
 struct Segment {
   Unit u;
@@ -190,35 +198,65 @@ struct Segment {
   int nq;                      // query tiles with rows in use
   int slot;                    // -1: the whole unit
 };
+// The units from number `unit` on, one after another; sequences' lengths are read once each.
+struct Cursor {
+  const PromptParams& p;
+  int b, hg, tt;
+  RowLens len;
+  __device__ Cursor(const PromptParams& p_, long long unit) : p(p_) {
+    const int HG = p.a.Hkv * p.t.GC;
+    const long long bhg = unit / p.NTT;
+    tt = (int)(unit - bhg * p.NTT);
+    b = (int)(bhg / HG);
+    hg = (int)(bhg - (long long)b * HG);
+    len = b < p.a.B ? lens_of(p.a, b) : RowLens{0, 0};
+  }
+  __device__ long long number() const { return ((long long)b * (p.a.Hkv * p.t.GC) + hg) * p.NTT + tt; }
+  __device__ bool live() const { return tt * (2 * p.t.Tt) < len.rows; }
+  __device__ void next_row() {                 // the next head: the rest of this one's units, if any, have no rows
+    tt = 0;
+    if (++hg == p.a.Hkv * p.t.GC) {
+      hg = 0;
+      ++b;
+      len = b < p.a.B ? lens_of(p.a, b) : RowLens{0, 0};
+    }
+  }
+  __device__ void next() { if (++tt == p.NTT) next_row(); }
+  __device__ Unit unit() const {
+    Unit u;
+    u.b = b;
+    u.h = p.t.GC == 1 ? hg : hg / p.t.GC;
+    u.gc = hg - u.h * p.t.GC;
+    u.t0 = tt * 2 * p.t.Tt;
+    u.len = len;
+    const int t1 = u.t0 + 2 * p.t.Tt;
+    u.k = key_tiles(p.a, len, u.t0, t1 < len.rows ? t1 : len.rows);
+    return u;
+  }
+};
 // the segments of one worker (a CTA or a pair of CTAs), in order; every role walks them for itself
 struct Walker {
-  const PromptParams& p;
-  long long unit, left;
-  int off;
-  int worker;
-  __device__ Walker(const PromptParams& p_, int worker_) : p(p_), worker(worker_) {
-    const Boundary x = p.bounds[worker], y = p.bounds[worker + 1];
-    unit = x.unit;
-    off = x.off;
-    left = y.pos - x.pos;
-  }
+  Cursor c;
+  long long last;              // unit in which the range ends, in front of key tile last_off
+  int off, last_off, worker;
+  __device__ Walker(const PromptParams& p, int worker_)
+      : c(p, p.bounds[worker_].unit), last(p.bounds[worker_ + 1].unit), off(p.bounds[worker_].off), last_off(p.bounds[worker_ + 1].off), worker(worker_) {}
   __device__ bool next(Segment& s) {
-    if (left <= 0) return false;
-    const int tokens = 2 * p.t.Tt;
     for (;;) {
-      s.u = unit_at(p, unit, tokens);
-      if (s.u.t0 < s.u.len.rows) break;
-      unit = (unit / p.NTT + 1) * p.NTT;       // the rest of this head's units has no rows either
+      const long long at = c.number();
+      if (at > last || (at == last && off >= last_off)) return false;
+      if (c.live()) {
+        s.u = c.unit();
+        s.lo = off;
+        s.hi = at == last ? last_off : s.u.k.count;
+        s.nq = s.u.t0 + c.p.t.Tt < c.len.rows ? 2 : 1;
+        s.slot = (s.lo == 0 && s.hi == s.u.k.count) ? -1 : 2 * worker + (s.lo > 0 ? 0 : 1);
+        off = 0;
+        c.next();
+        return true;
+      }
+      c.next_row();
     }
-    s.lo = off;
-    const int size = s.u.k.count;
-    s.hi = left < size - off ? off + (int)left : size;
-    s.nq = s.u.t0 + p.t.Tt < s.u.len.rows ? 2 : 1;
-    s.slot = (s.lo == 0 && s.hi == size) ? -1 : 2 * worker + (s.lo > 0 ? 0 : 1);
-    left -= s.hi - s.lo;
-    off = 0;
-    ++unit;
-    return true;
   }
 };
 
@@ -538,25 +576,31 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         const uint32_t s_addr = lane_addr + C::col_s(buf) + col0;
         const int n0 = tile_key(s.u.k, j);
         const bool whole = n0 + kKeys - 1 <= p_min && (a.window == 0 || n0 > p_max - a.window || n0 + kKeys <= a.sinks);
-        // Loops of 32 scores, not unrolled further, and read from tensor memory a second time for the exponentials: the
-        // loop of 64 unrolled scores ran at half the speed, a fifth of the instruction fetches missing.
+        // Loops of 32 scores, read from tensor memory a second time for the exponentials; a pair's CTA, with half as many
+        // warps, takes 64 at a time.  (Two query tiles with 64 scores a thread kept in registers: spills, a fifth of the
+        // instruction fetches missing, 500 instead of 458 us for two prompts of 8192 with a window.)
+        constexpr int kAt = PAIR ? 2 : 1;
         float mx = -INFINITY;
 #pragma unroll 1
-        for (int g = 0; g < NS; g += 32) {
-          uint32_t x[32];
-          ptx::tmem_ld32(s_addr + g, x);
-          ptx::tmem_ld_wait();
-          if (!whole) {                                       // hidden scores go back as -infinity
-            const int hi = pos - n0 - col0 - g + 1, lo = a.window > 0 ? hi - a.window : 0, sink = a.sinks - n0 - col0 - g;
-            const uint32_t seen = low_bits(hi) & (~low_bits(lo) | low_bits(sink));
+        for (int g = 0; g < NS; g += 32 * kAt) {
+          uint32_t x[kAt][32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!((seen >> i) & 1u)) x[i] = __float_as_uint(-INFINITY);
-            ptx::tmem_st32(s_addr + g, x);
-          }
+          for (int u = 0; u < kAt; ++u) ptx::tmem_ld32(s_addr + g + u * 32, x[u]);
+          ptx::tmem_ld_wait();
           float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+          for (int u = 0; u < kAt; ++u) {
+            if (!whole) {                                     // hidden scores go back as -infinity
+              const int at = col0 + g + u * 32, hi = pos - n0 - at + 1, lo = a.window > 0 ? hi - a.window : 0, sink = a.sinks - n0 - at;
+              const uint32_t seen = low_bits(hi) & (~low_bits(lo) | low_bits(sink));
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!((seen >> i) & 1u)) x[u][i] = __float_as_uint(-INFINITY);
+              ptx::tmem_st32(s_addr + g + u * 32, x[u]);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(x[u][i]), __uint_as_float(x[u][i + 1]));
+          }
           mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         }
         if (!whole) ptx::tmem_st_wait();
@@ -589,11 +633,16 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         }
         // P over the front half of this thread's own columns, in two halves
         float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll 1
+        uint32_t xs[kAt][32];
+#pragma unroll kAt
         for (int half = 0; half < 2; ++half) {
-          uint32_t x[32], pr[16];
-          ptx::tmem_ld32(s_addr + half * 32, x);
-          ptx::tmem_ld_wait();
+          uint32_t pr[16];
+          if (half % kAt == 0) {
+#pragma unroll
+            for (int u = 0; u < kAt; ++u) ptx::tmem_ld32(s_addr + (half + u) * 32, xs[u]);
+            ptx::tmem_ld_wait();
+          }
+          const uint32_t(&x)[32] = xs[half % kAt];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             float2 w = fma2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), p.scale_log2, neg);
@@ -632,15 +681,16 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         ptx::tmem_ld_wait();
         if (s.slot < 0) {
           if (used) {
-            uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + row * D + c0 + c);
+            T* dst = reinterpret_cast<T*>(a.out) + row * D + c0 + c;
+            uint32_t x[16];
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint4 x;
-              x.x = mma::pack<T>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-              x.y = mma::pack<T>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-              x.z = mma::pack<T>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
-              x.w = mma::pack<T>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
-              dst[i / 8] = x;
+            for (int i = 0; i < 32; i += 2) x[i / 2] = mma::pack<T>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+            if (p.out32) {                       // whole sectors; the rows of a warp are far apart
+              ptx::st_global_v8(dst, x);
+              ptx::st_global_v8(dst + 16, x + 8);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; i += 4) reinterpret_cast<uint4*>(dst)[i / 4] = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
             }
           }
         } else {
@@ -677,7 +727,7 @@ __global__ void __launch_bounds__(128) join_kernel(const PromptParams p) {
   const Cut cut = p.cuts[blockIdx.x];
   if (cut.count == 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Unit u = unit_at(p, cut.unit, 2 * p.t.Tt);
+  const Unit u = Cursor(p, cut.unit).unit();
   const int rr = blockIdx.y * 32 + lane, qi = rr / 128, r = rr % 128;
   const int col = blockIdx.z * 64 + warp * 16;
   int t;
@@ -729,6 +779,7 @@ Plan plan_of(int B, int Hq, int Hkv, int T, int D, int N) {
   const long long tiles = (long long)B * Hkv * x.t.GC * x.NTT * ((N + kKeys - 1) / kKeys);
   const int most = D == 256 ? sm_count() / 2 : sm_count();
   x.grid = (int)(tiles < most ? tiles : most);
+  if (x.grid > kMaxGrid) x.grid = kMaxGrid;
   x.steps = up256(((size_t)B * x.NTT + 1) * 8);
   x.bounds = up256((size_t)(x.grid + 1) * sizeof(Boundary));
   x.cuts = up256((size_t)x.grid * sizeof(Cut));
@@ -749,8 +800,9 @@ int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
   p.box = box_rows(a);
   p.grid = x.grid;
   p.scale_log2 = a.scale * kLog2e;
+  p.out32 = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
   uint8_t* ws = reinterpret_cast<uint8_t*>(a.workspace);
-  p.steps = reinterpret_cast<long long*>(ws);
+  p.cost = reinterpret_cast<long long*>(ws);
   p.bounds = reinterpret_cast<Boundary*>(ws += x.steps);
   p.cuts = reinterpret_cast<Cut*>(ws += x.bounds);
   p.part_ml = reinterpret_cast<float2*>(ws += x.cuts);

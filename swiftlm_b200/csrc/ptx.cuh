@@ -132,6 +132,11 @@ __device__ __forceinline__ void st_global_v8(float* p, float2 a, float2 b, float
                : "memory");
 }
 
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t* x) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]),
+               "r"(x[5]), "r"(x[6]), "r"(x[7]) : "memory");
+}
+
 // ---- tcgen05 / tensor memory ----------------------------------------------------------------
 __device__ __forceinline__ void tmem_alloc(void* smem_result, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_result)), "r"(ncols) : "memory");
