@@ -1,0 +1,406 @@
+// The weight that cached tokens receive from queries whose log-sum-exp is known:
+//     mass[b, h, n] += sum over the rows r of h's query heads that see n of 2^(scale log2(e) q_r . k_n - log2(e) lse_r)
+//
+// Computed as S^T = K Q^T on the tensor cores (tcgen05): 128 keys are the lanes of tensor memory and 128 query rows its
+// columns, so that the sum over rows stays inside a thread and nothing is reduced across lanes; four threads share a key.
+// A unit of work is one key tile, its steps are the query tiles that see it.  Few rows (a verify block, the last rows of a
+// prompt: one query tile): every key is read once and used by 128 rows, bound by HBM; the query tile stays in shared
+// memory.  Many rows: 2 D operations and one exponential a pair of row and key, bound by the 16 exponentials a clock of
+// an SM (1024 clocks a tile against 512 of products at D = 128), the key tile stays and query tiles stream.
+//
+// Warps: 0 loads key and query tiles (whichever changed), 1 the rows' -log2(e) lse, 2 issues the products, 4-19 sum.  Four
+// score buffers in tensor memory let the products run ahead.  Units are cut into equal ranges per CTA (ranges.cuh);
+// pieces of a cut unit leave 128 sums in the workspace, added in order by join_kernel: the order of every sum is fixed.
+#include "ranges.cuh"
+#include "tc_common.cuh"
+
+namespace dflash {
+namespace {
+
+using namespace tc;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kUnitCost = 1;                 // what a unit costs besides its query tiles
+constexpr int kSumWarps = 16, kThreads = 128 + kSumWarps * 32;
+constexpr int kBuffers = 4;
+
+struct MassParams {
+  CacheArgs a;
+  Tiling t;
+  Ranges ranges;               // rows of key tiles
+  int box, k_stages, q_stages; // tiles of keys and of queries in shared memory
+  float scale_log2;
+  float* part;                 // [2 * grid][128]
+};
+
+template <int D> struct Cfg {
+  static constexpr int NC = D / 64, tile = NC * kChunk;
+  static constexpr int tiles = D == 256 ? 3 : 6;            // tiles of keys and queries together
+  static constexpr int bars = tiles * tile;
+  static constexpr int b_k_full = 0, b_k_empty = tiles, b_q_full = 2 * tiles, b_q_empty = 3 * tiles, b_s_full = 4 * tiles,
+                       b_s_free = b_s_full + kBuffers, b_z_full = b_s_free + kBuffers, n_bars = b_z_full + kBuffers;
+  static constexpr int misc = bars + (8 * n_bars + 15) / 16 * 16;
+  static constexpr int z = misc + 16;                       // [kBuffers][128] -log2(e) lse of the rows
+  static constexpr int sums = z + kBuffers * 128 * 4;       // [2][4][128] of the four threads of a key
+  static constexpr int total = sums + 2 * 4 * 128 * 4;
+};
+static_assert(Cfg<256>::total <= 232448 && Cfg<128>::total <= 232448 && Cfg<64>::total <= 232448, "shared memory");
+
+// query tokens of sequence (len) that see some key of [n0, n0 + 128): first and last; last < first: none
+struct Seeing { int first, last; };
+__device__ __forceinline__ Seeing seeing(const CacheArgs& a, RowLens len, int n0) {
+  const int past = len.keys - len.rows, n1 = (n0 + kKeys < len.keys ? n0 + kKeys : len.keys) - 1;
+  Seeing s{n0 > past ? n0 - past : 0, len.rows - 1};
+  if (a.window > 0 && n0 >= a.sinks && n1 + a.window - 1 - past < s.last) s.last = n1 + a.window - 1 - past;
+  if (n1 < n0) s.last = -1;
+  return s;
+}
+// query tiles (times head groups) of a key tile
+__device__ __forceinline__ int tile_steps(const CacheArgs& a, const Tiling& t, RowLens len, int u) {
+  const Seeing s = seeing(a, len, u * kKeys);
+  return s.last < s.first ? 0 : t.GC * (s.last / t.Tt - s.first / t.Tt + 1);
+}
+// first key tile at or behind u that is seen
+__device__ __forceinline__ int next_tile(const CacheArgs& a, RowLens len, int u, int per_row) {
+  const int tiles = (len.keys + kKeys - 1) / kKeys;
+  if (len.rows == 0 || u >= tiles) return per_row;
+  const int past = len.keys - len.rows;
+  const int lo = a.window > 0 && past - a.window + 1 > 0 ? (past - a.window + 1) / kKeys : 0;      // of the first row's window
+  const int sinks = a.window > 0 ? (a.sinks + kKeys - 1) / kKeys : 0;
+  if (u >= sinks && u < lo) u = lo;
+  return u < tiles ? u : per_row;
+}
+
+__global__ void __launch_bounds__(1024) mass_plan_kernel(const MassParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  plan_ranges<kUnitCost>(p.ranges, p.a, [&](RowLens len, int u) { return tile_steps(p.a, p.t, len, u); });
+}
+
+// One step: a key tile against a query tile.
+struct Step {
+  int b, h, n0, gc, t0;        // t0: first token of the query tile
+  RowLens len;
+  bool new_k, new_q, last;     // the first step of a unit; another query tile than the step before; the last step of a unit
+  int slot;                    // of the unit (see RangeWalker::take)
+};
+struct Steps {
+  const MassParams& p;
+  RangeWalker w;
+  Step s;
+  int tt0, per_gc, i, hi;      // first query tile and query tiles per head group of the unit; step, end
+  bool any;
+  __device__ Steps(const MassParams& p_, int worker) : p(p_), w(p_.ranges, p_.a, worker), i(0), hi(0), any(false) {}
+  __device__ bool next() {
+    const int b = s.b, h = s.h, gc = s.gc, t0 = s.t0;
+    s.new_k = ++i >= hi || !any;
+    if (s.new_k) {
+      if (!w.find([&](RowLens len, int u) {
+            u = next_tile(p.a, len, u, p.ranges.per_row);
+            while (u < p.ranges.per_row && tile_steps(p.a, p.t, len, u) == 0) u = next_tile(p.a, len, u + 1, p.ranges.per_row);
+            return u;
+          }, i)) return false;
+      s.b = w.c.b;
+      s.h = w.c.hg;
+      s.len = w.c.len;
+      s.n0 = w.c.u * kKeys;
+      const Seeing x = seeing(p.a, s.len, s.n0);
+      tt0 = x.first / p.t.Tt;
+      per_gc = x.last / p.t.Tt - tt0 + 1;
+      hi = w.take(i, p.t.GC * per_gc, s.slot);
+    }
+    s.gc = p.t.GC == 1 ? 0 : i / per_gc;
+    s.t0 = (tt0 + i - s.gc * per_gc) * p.t.Tt;
+    s.new_q = !any || b != s.b || h != s.h || gc != s.gc || t0 != s.t0;
+    s.last = i == hi - 1;
+    any = true;
+    return true;
+  }
+};
+
+__device__ __forceinline__ uint32_t bits_below(int n) {     // bits [0, n), n clamped to [0, 32]
+  return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const MassParams p) {
+  using C = Cfg<D>;
+  constexpr int NC = C::NC;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  const CacheArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::bars);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::misc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::misc + 4);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) {
+    ptx::prefetch_tensormap(&map_q);
+    ptx::prefetch_tensormap(&map_k);
+    for (int i = 0; i < C::n_bars; ++i) ptx::mbar_init(&bars[i], i >= C::b_s_free && i < C::b_z_full ? kSumWarps : 1);
+    *abort_flag = (ptx::smem_u32(sm) & 1023u) != 0u;      // swizzled tiles need 1024-byte alignment; never seen violated
+    if (*abort_flag) atomicExch(a.status, kStatusSmemAlign);
+    ptx::fence_mbar_init();
+  }
+  // rows of a query tile behind Gt * Tt are never loaded: zeros, so that their scores are numbers
+  const int q0 = p.k_stages * C::tile;
+  if (p.t.Gt * p.t.Tt < kRows) {
+    for (int e = threadIdx.x; e < p.q_stages * C::tile / 16; e += kThreads) *reinterpret_cast<uint4*>(sm + q0 + e * 16) = make_uint4(0, 0, 0, 0);
+    ptx::fence_proxy_async();
+  }
+  if (warp == 2) {
+    ptx::tmem_alloc(tmem_slot, 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  asm volatile("griddepcontrol.wait;" ::: "memory");     // the plan
+  const uint32_t tmem = *tmem_slot;
+  // A wait that gives up raises the abort flag, after which every wait returns at once: the roles run through their loops
+  // without results, meet at the end and leave.
+  auto wait = [&](int bar, uint32_t parity) { return ptx::mbar_wait_or_abort(&bars[bar], parity, abort_flag, a.status, kStatusMbarWait); };
+  Steps st(p, blockIdx.x);
+  const Step& s = st.s;
+
+  if (warp == 0) {
+    // ------------------------------- keys and queries -------------------------------
+    uint32_t n_k = 0, n_q = 0;
+    bool ok = !*abort_flag;
+    while (ok && st.next()) {
+      if (s.new_k) {
+        const uint32_t at = n_k % p.k_stages;
+        if (n_k >= (uint32_t)p.k_stages) ok = __all_sync(0xffffffffu, wait(C::b_k_empty + at, (n_k / p.k_stages - 1) & 1));
+        if (!ok) break;
+        if (lane == 0) ptx::mbar_arrive_expect_tx(&bars[C::b_k_full + at], C::tile);
+        __syncwarp();
+        const int pieces = kKeys / p.box;
+        for (int i = lane; i < NC * pieces; i += 32) {
+          const int c = i / pieces, n = s.n0 + (i - c * pieces) * p.box;
+          const TilePlace x = place_of(a, s.b, n, s.len.keys);
+          ptx::tma_load_4d(sm + at * C::tile + c * kChunk + (n - s.n0) * 128, &map_k, c * 64, x.row, s.h, x.outer, &bars[C::b_k_full + at]);
+        }
+        __syncwarp();
+        ++n_k;
+      }
+      if (s.new_q) {
+        const uint32_t at = n_q % p.q_stages;
+        if (n_q >= (uint32_t)p.q_stages) ok = __all_sync(0xffffffffu, wait(C::b_q_empty + at, (n_q / p.q_stages - 1) & 1));
+        if (!ok) break;
+        if (lane == 0) {
+          ptx::mbar_arrive_expect_tx(&bars[C::b_q_full + at], NC * p.t.Gt * p.t.Tt * 128);
+          for (int c = 0; c < NC; ++c)
+            ptx::tma_load_4d(sm + q0 + at * C::tile + c * kChunk, &map_q, c * 64, s.gc * p.t.Gt, s.t0, s.b * a.Hkv + s.h, &bars[C::b_q_full + at]);
+        }
+        __syncwarp();
+        ++n_q;
+      }
+    }
+  } else if (warp == 1) {
+    // --------------------------------- log-sum-exp ----------------------------------
+    float* z = reinterpret_cast<float*>(sm + C::z);
+    uint32_t n = 0;
+    bool ok = true;
+    while (ok && st.next()) {
+      const uint32_t buf = n % kBuffers;
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = lane * 4 + i, g = s.gc * p.t.Gt + r % p.t.Gt, t = s.t0 + r / p.t.Gt;
+        v[i] = -INFINITY;                                     // rows not in use, and rows that see nothing, add nothing
+        if (r < p.t.Gt * p.t.Tt && g < p.t.G && t < s.len.rows) {
+          const float x = a.lse[((long long)s.b * a.Hq + s.h * p.t.G + g) * a.T + t];
+          if (x > -INFINITY) v[i] = -x * kLog2e;
+        }
+      }
+      if (n >= kBuffers) ok = __all_sync(0xffffffffu, wait(C::b_s_free + buf, (n / kBuffers - 1) & 1));
+      *reinterpret_cast<float4*>(z + buf * 128 + lane * 4) = make_float4(v[0], v[1], v[2], v[3]);
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&bars[C::b_z_full + buf]);
+      ++n;
+    }
+  } else if (warp == 2) {
+    // ---------------------------------- S^T = K Q^T ----------------------------------
+    constexpr uint32_t kI = idesc<T>(kKeys, kRows, false);
+    uint32_t n = 0, n_k = 0, n_q = 0;
+    bool ok = true;
+    while (ok && st.next()) {
+      // the tiles that are not needed any more are free once the products so far are done
+      if (s.new_k && n_k > 0 && ptx::elect_one()) ptx::umma_commit(&bars[C::b_k_empty + (n_k - 1) % p.k_stages]);
+      if (s.new_q && n_q > 0 && ptx::elect_one()) ptx::umma_commit(&bars[C::b_q_empty + (n_q - 1) % p.q_stages]);
+      __syncwarp();
+      n_k += s.new_k;
+      n_q += s.new_q;
+      const uint32_t ka = (n_k - 1) % p.k_stages, qa = (n_q - 1) % p.q_stages, buf = n % kBuffers;
+      if (s.new_k) ok = wait(C::b_k_full + ka, ((n_k - 1) / p.k_stages) & 1);
+      if (s.new_q) ok = ok && wait(C::b_q_full + qa, ((n_q - 1) / p.q_stages) & 1);
+      if (n >= kBuffers) ok = ok && wait(C::b_s_free + buf, (n / kBuffers - 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      ptx::tc_fence_after();
+      if (ptx::elect_one()) {
+        const uint32_t d = tmem + buf * 128, k_addr = ptx::smem_u32(sm + ka * C::tile), q_addr = ptx::smem_u32(sm + q0 + qa * C::tile);
+#pragma unroll 1
+        for (int c = 0; c < NC; ++c) {
+          const uint64_t da = make_desc(k_addr + c * kChunk, 16, 1024), db = make_desc(q_addr + c * kChunk, 16, 1024);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) ptx::umma_ss(d, da + 2 * k, db + 2 * k, kI, c + k > 0);
+        }
+        ptx::umma_commit(&bars[C::b_s_full + buf]);
+      }
+      __syncwarp();
+      ++n;
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------- sums --------------------------------------
+    const int wq = warp & 3, quarter = (warp - 4) >> 2;       // tensor-memory lane quarter; which 32 rows of a query tile
+    const int key = wq * 32 + lane, col0 = quarter * 32;
+    const float* z = reinterpret_cast<const float*>(sm + C::z);
+    float* sums = reinterpret_cast<float*>(sm + C::sums);
+    uint32_t n = 0, units = 0;
+    float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    float before = 0.f;
+    while (st.next()) {
+      float* out = a.mass + ((long long)s.b * a.Hkv + s.h) * a.mass_stride + s.n0 + key;
+      const bool mine = quarter == 0 && s.n0 + key < s.len.keys;
+      if (s.new_k) {
+        acc[0] = acc[1] = make_float2(0.f, 0.f);
+        if (mine && s.slot < 0) before = *out;                // wanted at the unit's end
+      }
+      const uint32_t buf = n % kBuffers, par = (n / kBuffers) & 1;
+      wait(C::b_s_full + buf, par);
+      wait(C::b_z_full + buf, par);
+      __syncwarp();
+      ptx::tc_fence_after();
+      uint32_t x[32];
+      ptx::tmem_ld32(tmem + ((uint32_t)(wq * 32) << 16) + buf * 128 + col0, x);
+      ptx::tmem_ld_wait();
+      const int p0 = s.len.keys - s.len.rows + s.t0, p1 = p0 + p.t.Tt - 1;      // positions of the tile's tokens
+      const bool whole = s.n0 + kKeys - 1 <= p0 && (a.window == 0 || s.n0 > p1 - a.window || s.n0 + kKeys <= a.sinks) && s.t0 + p.t.Tt <= s.len.rows;
+      if (!whole) {
+        // rows [lo, hi) of the tile see this key: the tokens from it on, up to a window behind it, that are in use
+        const int nn = s.n0 + key;
+        int lo = nn - p0, hi = p.t.Tt < s.len.rows - s.t0 ? p.t.Tt : s.len.rows - s.t0;
+        if (a.window > 0 && nn >= a.sinks && nn + a.window - p0 < hi) hi = nn + a.window - p0;
+        lo = lo < 0 ? 0 : (lo > kRows ? kRows : lo);
+        hi = hi < 0 ? 0 : hi;
+        const uint32_t seen = bits_below(hi * p.t.Gt - col0) & ~bits_below(lo * p.t.Gt - col0);
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (!((seen >> i) & 1u)) x[i] = 0xff800000u;        // -infinity
+      }
+      const float4* zp = reinterpret_cast<const float4*>(z + buf * 128 + col0);
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        const float4 zi = zp[i / 4];
+        float2 u = fma2v(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), p.scale_log2, zi.x, zi.y);
+        float2 w = fma2v(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]), p.scale_log2, zi.z, zi.w);
+        u.x = mma::exp2_approx(u.x); u.y = mma::exp2_approx(u.y);
+        w.x = mma::exp2_approx(w.x); w.y = mma::exp2_approx(w.y);
+        acc[0] = add2(acc[0], u);
+        acc[1] = add2(acc[1], w);
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&bars[C::b_s_free + buf]);
+      ++n;
+      if (s.last) {
+        // the four threads of a key, in order; the slot of two units ago has been read before the last unit's meeting
+        float* slot = sums + (units++ & 1) * 512;
+        slot[quarter * 128 + key] = (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+        asm volatile("bar.sync 1, %0;" ::"n"(kSumWarps * 32) : "memory");
+        if (quarter == 0) {
+          const float total = (slot[key] + slot[128 + key]) + (slot[256 + key] + slot[384 + key]);
+          if (s.slot >= 0) p.part[(long long)s.slot * 128 + key] = total;
+          else if (mine) *out = before + total;
+        }
+      }
+    }
+  }
+  __syncwarp();
+  __syncthreads();
+  if (*abort_flag) __nanosleep(100000);        // copies that were still in flight land before the memory is given back
+  if (warp == 2) ptx::tmem_dealloc(tmem, 512);
+}
+
+// adds up the pieces of a cut key tile, in order
+__global__ void __launch_bounds__(128) mass_join_kernel(const MassParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Cut cut = p.ranges.cuts[blockIdx.x];
+  if (cut.count == 0) return;
+  const Cursor c(p.ranges, p.a, cut.unit);
+  const int n = c.u * kKeys + threadIdx.x;
+  if (n >= c.len.keys) return;
+  float total = 0.f;
+  for (int i = 0; i < cut.count; ++i) total += p.part[(long long)piece_slot(cut, i) * 128 + threadIdx.x];
+  p.a.mass[((long long)c.b * p.a.Hkv + c.hg) * p.a.mass_stride + n] += total;
+}
+
+struct Plan { Tiling t; int per_row, grid; size_t total; };
+Plan plan_of(int B, int Hq, int Hkv, int T, int N) {
+  Plan x;
+  x.t = tiling_of(Hq, Hkv);
+  x.per_row = (N + kKeys - 1) / kKeys;
+  const long long tiles = (long long)B * Hkv * x.per_row * x.t.GC * ((T + x.t.Tt - 1) / x.t.Tt);
+  const int n_sm = sm_count(), most = n_sm < kMaxGrid ? n_sm : kMaxGrid;
+  x.grid = (int)(tiles < most ? tiles : most);
+  x.total = ranges_bytes(B, x.per_row, x.grid) + (size_t)2 * x.grid * 128 * 4;
+  return x;
+}
+
+template <typename T, int D>
+int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
+  using C = Cfg<D>;
+  const Plan x = plan_of(a.B, a.Hq, a.Hkv, a.T, a.N);
+  MassParams p{};
+  p.a = a;
+  p.t = x.t;
+  p.ranges = Ranges{a.B, a.Hkv, x.per_row, x.grid, nullptr, nullptr, nullptr};
+  p.box = box_rows(a);
+  // one query tile in all: it stays, keys stream; else queries stream past a key tile
+  const bool one = x.t.GC == 1 && a.T <= x.t.Tt;
+  p.q_stages = one ? 1 : C::tiles - (D == 256 ? 1 : 2);
+  p.k_stages = C::tiles - p.q_stages;
+  p.scale_log2 = a.scale * kLog2e;
+  p.part = reinterpret_cast<float*>(ranges_at(p.ranges, reinterpret_cast<uint8_t*>(a.workspace)));
+  CUtensorMap mq, mk;
+  CUresult r = encode_q(&mq, a, x.t);
+  if (r == CUDA_SUCCESS) r = encode_kv(&mk, a.k, a, p.box);
+  if (r != CUDA_SUCCESS) { set_error("attention_mass: cuTensorMapEncodeTiled failed with CUresult %d", (int)r); return DFLASH_ERR_CUDA; }
+  auto kernel = mass_kernel<T, D>;
+  DFLASH_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::total));
+  mass_plan_kernel<<<1, 1024, 0, stream>>>(p);
+  DFLASH_LAUNCH_CHECK();
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.stream = stream;
+  cfg.gridDim = dim3(x.grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::total;
+  DFLASH_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, mq, mk, p));
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = 0;
+  DFLASH_CUDA_CHECK(cudaLaunchKernelEx(&cfg, mass_join_kernel, p));
+  count_launch(3);
+  return DFLASH_OK;
+}
+
+template <typename T>
+int32_t launch_dims(const CacheArgs& a, cudaStream_t s) {
+  if (a.D == 64) return launch_typed<T, 64>(a, s);
+  if (a.D == 128) return launch_typed<T, 128>(a, s);
+  return launch_typed<T, 256>(a, s);
+}
+
+}  // namespace
+
+size_t mass_workspace_bytes(int B, int Hq, int Hkv, int T, int, int N) { return plan_of(B, Hq, Hkv, T, N).total; }
+
+int32_t launch_mass(const CacheArgs& a, cudaStream_t stream) {
+  return a.dtype == DFLASH_BF16 ? launch_dims<__nv_bfloat16>(a, stream) : launch_dims<__half>(a, stream);
+}
+
+}  // namespace dflash

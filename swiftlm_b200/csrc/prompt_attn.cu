@@ -18,10 +18,10 @@
 //   the row's 128 exponentials were a chain of 4000 clocks.
 // * Only the key tiles that some row of the unit sees are visited; only those that some row does not see whole are masked.
 //   Value rows behind the sequence's length are zeroed in shared memory before the product, whatever the cache holds there.
-// * Persistent CTAs, one per SM.  plan_kernel lays the key tiles of all units in a row and cuts them into equal ranges, so
-//   that unequal lengths, causal triangles and few query rows over a long cache all fill the GPU; a cut closer than kMinCut
-//   tiles to a unit's edge moves to the edge.  A unit cut in pieces leaves (O, m, l) per piece in the workspace and
+// * Persistent CTAs, one per SM.  plan_kernel cuts the key tiles of all units into equal ranges (ranges.cuh), so that unequal
+//   lengths, causal triangles and few query rows over a long cache all fill the GPU.  A unit cut in pieces leaves (O, m, l) per piece in the workspace and
 //   join_kernel adds them up in order.
+#include "ranges.cuh"
 #include "tc_common.cuh"
 
 namespace dflash {
@@ -31,28 +31,18 @@ using namespace tc;
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kRescale = 8.f;              // in log2 units
-constexpr int kMinCut = 4;                   // key tiles of the smallest piece of a cut unit
 constexpr int kUnitCost = 3;                 // what a unit costs besides its key tiles (loading queries, storing rows), in tiles
-
-struct Boundary { long long unit; int off, pad; };   // in front of key tile `off` of a unit
-struct Cut { long long unit; int first, count; };
 
 struct PromptParams {
   CacheArgs a;
   Tiling t;
-  int NTT;                     // units (of two query tiles) per (sequence, KV head, head group)
+  Ranges ranges;               // rows of units of two query tiles
   int box;
-  int grid;
   float scale_log2;
   int out32;                   // `out` is 32-byte aligned
-  long long* cost;             // [B * NTT + 1] cost of what is in front of every (sequence, unit)
-  Boundary* bounds;            // [grid + 1]
-  Cut* cuts;                   // [grid]
   float4* part_o;              // [2 * grid][D / 4][256]
   float2* part_ml;             // [2 * grid][256]
 };
-
-constexpr int kMaxGrid = 1023;                // workers at most: a boundary for each thread of plan_kernel
 
 template <int D> struct Cfg {
   static constexpr bool PAIR = D == 256;                    // two CTAs on one unit, a query tile each
@@ -86,104 +76,14 @@ template <int D> struct Cfg {
 static_assert(Cfg<256>::total <= 232448 && Cfg<128>::total <= 232448 && Cfg<64>::total <= 232448, "shared memory");
 
 // ---- the plan ----
-__device__ __forceinline__ int unit_cost(const PromptParams& p, RowLens len, int tt, int tokens) {
-  const int t0 = tt * tokens;
+__device__ __forceinline__ int unit_steps(const CacheArgs& a, RowLens len, int u, int tokens) {
+  const int t0 = u * tokens;
   if (t0 >= len.rows) return 0;
-  const int t1 = t0 + tokens < len.rows ? t0 + tokens : len.rows;
-  return kUnitCost + key_tiles(p.a, len, t0, t1).count;
+  return key_tiles(a, len, t0, t0 + tokens < len.rows ? t0 + tokens : len.rows).count;
 }
-
-__global__ void __launch_bounds__(1024) plan_kernel(const PromptParams p, int tokens) {
-  __shared__ long long warp_sums[32];
+__global__ void __launch_bounds__(1024) plan_kernel(const PromptParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long E = (long long)p.a.B * p.NTT, HG = (long long)p.a.Hkv * p.t.GC;
-  const long long per_thread = (E + 1023) / 1024, e0 = tid * per_thread, e1 = e0 + per_thread < E ? e0 + per_thread : E;
-  long long mine = 0;
-  int b = -1;
-  RowLens len{0, 0};
-  for (long long e = e0; e < e1; ++e) {
-    const int eb = (int)(e / p.NTT);
-    if (eb != b) { b = eb; len = lens_of(p.a, b, true); }
-    mine += unit_cost(p, len, (int)(e - (long long)b * p.NTT), tokens);
-  }
-  long long x = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  if (lane == 31) warp_sums[warp] = x;
-  __syncthreads();
-  long long at = x - mine;
-  for (int w = 0; w < warp; ++w) at += warp_sums[w];
-  b = -1;
-  for (long long e = e0; e < e1; ++e) {
-    const int eb = (int)(e / p.NTT);
-    if (eb != b) { b = eb; len = lens_of(p.a, b); }
-    p.cost[e] = at;
-    at += unit_cost(p, len, (int)(e - (long long)b * p.NTT), tokens);
-  }
-  long long all = 0;
-  for (int w = 0; w < 32; ++w) all += warp_sums[w];
-  if (tid == 0) p.cost[E] = all;
-  __syncthreads();               // the table is read by other threads of this block below
-  const long long total = all * HG;
-  const long long per = total > p.grid ? (total + p.grid - 1) / p.grid : 1;
-  __shared__ Boundary raw[kMaxGrid + 1];
-  if (tid <= p.grid) {
-    const int c = tid;
-    const long long pos = c * per;
-    Boundary r{E * HG, 0, 0};
-    if (pos < total) {
-      int lo = 0, hi = p.a.B - 1;             // the last sequence that starts at or before pos
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (p.cost[(long long)mid * p.NTT] * HG <= pos) lo = mid; else hi = mid - 1;
-      }
-      const long long base = p.cost[(long long)lo * p.NTT], len_b = p.cost[(long long)(lo + 1) * p.NTT] - base;
-      const long long hg = (pos - base * HG) / len_b, rem = pos - base * HG - hg * len_b;
-      int ta = 0, tb = p.NTT - 1;             // the last unit that starts at or before rem
-      while (ta < tb) {
-        const int mid = (ta + tb + 1) >> 1;
-        if (p.cost[(long long)lo * p.NTT + mid] - base <= rem) ta = mid; else tb = mid - 1;
-      }
-      const long long s = p.cost[(long long)lo * p.NTT + ta] - base, e = p.cost[(long long)lo * p.NTT + ta + 1] - base;
-      const long long unit = ((long long)lo * HG + hg) * p.NTT + ta;
-      const int size = (int)(e - s) - kUnitCost;
-      int off = (int)(rem - s) - kUnitCost;
-      off = off < 0 ? 0 : off / kMinCut * kMinCut;
-      const bool back = size < kMinCut ? 2 * (rem - s) >= e - s : size - off < kMinCut;    // the unit's end is nearer
-      r = back ? Boundary{unit + 1, 0, 0} : Boundary{unit, off, 0};
-    }
-    raw[c] = r;
-  }
-  __syncthreads();
-  // equal boundaries become one, so that the pieces of a cut unit belong to workers in a row
-  {
-    const bool fresh = tid <= p.grid && (tid == 0 || raw[tid].unit != raw[tid - 1].unit || raw[tid].off != raw[tid - 1].off);
-    const uint32_t in_warp = __ballot_sync(0xffffffffu, fresh);
-    if (lane == 0) warp_sums[warp] = __popc(in_warp);
-    __syncthreads();
-    int before = 0, all_fresh = 0;
-    for (int w = 0; w < 32; ++w) {
-      before += w < warp ? (int)warp_sums[w] : 0;
-      all_fresh += (int)warp_sums[w];
-    }
-    if (fresh) p.bounds[before + __popc(in_warp & ((1u << lane) - 1u))] = raw[tid];
-    if (tid >= all_fresh && tid <= p.grid) p.bounds[tid] = Boundary{E * HG, 0, 0};
-  }
-  __syncthreads();
-  if (tid < p.grid) {
-    const int c = tid;
-    Cut cut{0, 0, 0};
-    if (c >= 1 && p.bounds[c].off > 0 && !(p.bounds[c - 1].off > 0 && p.bounds[c - 1].unit == p.bounds[c].unit)) {
-      int n = 1;
-      while (c + n <= p.grid && p.bounds[c + n].off > 0 && p.bounds[c + n].unit == p.bounds[c].unit) ++n;
-      cut = Cut{p.bounds[c].unit, c - 1, n + 1};
-    }
-    p.cuts[c] = cut;
-  }
+  plan_ranges<kUnitCost>(p.ranges, p.a, [&](RowLens len, int u) { return unit_steps(p.a, len, u, 2 * p.t.Tt); });
 }
 
 struct Unit {
@@ -198,65 +98,28 @@ struct Segment {
   int nq;                      // query tiles with rows in use
   int slot;                    // -1: the whole unit
 };
-// The units from number `unit` on, one after another; sequences' lengths are read once each.
-struct Cursor {
-  const PromptParams& p;
-  int b, hg, tt;
-  RowLens len;
-  __device__ Cursor(const PromptParams& p_, long long unit) : p(p_) {
-    const int HG = p.a.Hkv * p.t.GC;
-    const long long bhg = unit / p.NTT;
-    tt = (int)(unit - bhg * p.NTT);
-    b = (int)(bhg / HG);
-    hg = (int)(bhg - (long long)b * HG);
-    len = b < p.a.B ? lens_of(p.a, b) : RowLens{0, 0};
-  }
-  __device__ long long number() const { return ((long long)b * (p.a.Hkv * p.t.GC) + hg) * p.NTT + tt; }
-  __device__ bool live() const { return tt * (2 * p.t.Tt) < len.rows; }
-  __device__ void next_row() {                 // the next head: the rest of this one's units, if any, have no rows
-    tt = 0;
-    if (++hg == p.a.Hkv * p.t.GC) {
-      hg = 0;
-      ++b;
-      len = b < p.a.B ? lens_of(p.a, b) : RowLens{0, 0};
-    }
-  }
-  __device__ void next() { if (++tt == p.NTT) next_row(); }
-  __device__ Unit unit() const {
-    Unit u;
-    u.b = b;
-    u.h = p.t.GC == 1 ? hg : hg / p.t.GC;
-    u.gc = hg - u.h * p.t.GC;
-    u.t0 = tt * 2 * p.t.Tt;
-    u.len = len;
-    const int t1 = u.t0 + 2 * p.t.Tt;
-    u.k = key_tiles(p.a, len, u.t0, t1 < len.rows ? t1 : len.rows);
-    return u;
-  }
-};
-// the segments of one worker (a CTA or a pair of CTAs), in order; every role walks them for itself
+__device__ __forceinline__ Unit unit_at(const PromptParams& p, const Cursor& c) {
+  Unit u;
+  u.b = c.b;
+  u.h = p.t.GC == 1 ? c.hg : c.hg / p.t.GC;
+  u.gc = c.hg - u.h * p.t.GC;
+  u.t0 = c.u * 2 * p.t.Tt;
+  u.len = c.len;
+  const int t1 = u.t0 + 2 * p.t.Tt;
+  u.k = key_tiles(p.a, c.len, u.t0, t1 < c.len.rows ? t1 : c.len.rows);
+  return u;
+}
 struct Walker {
-  Cursor c;
-  long long last;              // unit in which the range ends, in front of key tile last_off
-  int off, last_off, worker;
-  __device__ Walker(const PromptParams& p, int worker_)
-      : c(p, p.bounds[worker_].unit), last(p.bounds[worker_ + 1].unit), off(p.bounds[worker_].off), last_off(p.bounds[worker_ + 1].off), worker(worker_) {}
+  const PromptParams& p;
+  RangeWalker w;
+  __device__ Walker(const PromptParams& p_, int worker) : p(p_), w(p_.ranges, p_.a, worker) {}
   __device__ bool next(Segment& s) {
-    for (;;) {
-      const long long at = c.number();
-      if (at > last || (at == last && off >= last_off)) return false;
-      if (c.live()) {
-        s.u = c.unit();
-        s.lo = off;
-        s.hi = at == last ? last_off : s.u.k.count;
-        s.nq = s.u.t0 + c.p.t.Tt < c.len.rows ? 2 : 1;
-        s.slot = (s.lo == 0 && s.hi == s.u.k.count) ? -1 : 2 * worker + (s.lo > 0 ? 0 : 1);
-        off = 0;
-        c.next();
-        return true;
-      }
-      c.next_row();
-    }
+    const int tokens = 2 * p.t.Tt;
+    if (!w.find([&](RowLens len, int u) { return u * tokens < len.rows ? u : p.ranges.per_row; }, s.lo)) return false;
+    s.u = unit_at(p, w.c);
+    s.nq = s.u.t0 + p.t.Tt < s.u.len.rows ? 2 : 1;
+    s.hi = w.take(s.lo, s.u.k.count, s.slot);
+    return true;
   }
 };
 
@@ -276,20 +139,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// (x, y) * s + t in one instruction; (x, y) + (u, v) in one
-__device__ __forceinline__ float2 fma2(float x, float y, float s, float t) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, c, e;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\tfma.rn.f32x2 e, a, b, c;\n\tmov.b64 {%0, %1}, e;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(x), "f"(y), "f"(s), "f"(t));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n\t.reg .b64 a, b, e;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 e, a, b;\n\tmov.b64 {%0, %1}, e;\n\t}"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(Cfg<D>::threads, 1)
 prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -645,7 +494,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
           const uint32_t(&x)[32] = xs[half % kAt];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            float2 w = fma2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), p.scale_log2, neg);
+            float2 w = fma2v(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), p.scale_log2, neg, neg);
             w.x = mma::exp2_approx(w.x);
             w.y = mma::exp2_approx(w.y);
             add[(i >> 1) & 1] = add2(add[(i >> 1) & 1], w);
@@ -724,16 +573,16 @@ template <typename T, int D>
 __global__ void __launch_bounds__(128) join_kernel(const PromptParams p) {
   constexpr int R = 256;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Cut cut = p.cuts[blockIdx.x];
+  const Cut cut = p.ranges.cuts[blockIdx.x];
   if (cut.count == 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Unit u = Cursor(p, cut.unit).unit();
+  const Unit u = unit_at(p, Cursor(p.ranges, p.a, cut.unit));
   const int rr = blockIdx.y * 32 + lane, qi = rr / 128, r = rr % 128;
   const int col = blockIdx.z * 64 + warp * 16;
   int t;
   long long row;
   if (!row_of(p, u, qi, r, t, row)) return;
-  auto slot = [&](int i) { return (long long)(2 * (cut.first + i) + (i == 0 ? 1 : 0)); };
+  auto slot = [&](int i) { return (long long)piece_slot(cut, i); };
   float top = -INFINITY;
   for (int i = 0; i < cut.count; ++i) top = fmaxf(top, p.part_ml[slot(i) * R + rr].x);
   const float z = top == -INFINITY ? 0.f : top;
@@ -769,23 +618,20 @@ size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 struct Plan {
   Tiling t;
-  int NTT, grid;               // grid: workers, a CTA each (D <= 128) or a pair of CTAs
-  size_t steps, bounds, cuts, part_ml, part_o, total;
+  int per_row, grid;           // grid: workers, a CTA each (D <= 128) or a pair of CTAs
+  size_t part_ml, part_o, total;
 };
 Plan plan_of(int B, int Hq, int Hkv, int T, int D, int N) {
   Plan x;
   x.t = tiling_of(Hq, Hkv);
-  x.NTT = (T + 2 * x.t.Tt - 1) / (2 * x.t.Tt);
-  const long long tiles = (long long)B * Hkv * x.t.GC * x.NTT * ((N + kKeys - 1) / kKeys);
-  const int most = D == 256 ? sm_count() / 2 : sm_count();
+  x.per_row = (T + 2 * x.t.Tt - 1) / (2 * x.t.Tt);
+  const long long tiles = (long long)B * Hkv * x.t.GC * x.per_row * ((N + kKeys - 1) / kKeys);
+  int most = D == 256 ? sm_count() / 2 : sm_count();
+  if (most > kMaxGrid) most = kMaxGrid;
   x.grid = (int)(tiles < most ? tiles : most);
-  if (x.grid > kMaxGrid) x.grid = kMaxGrid;
-  x.steps = up256(((size_t)B * x.NTT + 1) * 8);
-  x.bounds = up256((size_t)(x.grid + 1) * sizeof(Boundary));
-  x.cuts = up256((size_t)x.grid * sizeof(Cut));
   x.part_ml = up256((size_t)2 * x.grid * 256 * sizeof(float2));
   x.part_o = up256((size_t)2 * x.grid * 256 * D * 4);
-  x.total = x.steps + x.bounds + x.cuts + x.part_ml + x.part_o;
+  x.total = ranges_bytes(B, x.per_row, x.grid) + x.part_ml + x.part_o;
   return x;
 }
 
@@ -796,17 +642,13 @@ int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
   PromptParams p{};
   p.a = a;
   p.t = x.t;
-  p.NTT = x.NTT;
+  p.ranges = Ranges{a.B, a.Hkv * x.t.GC, x.per_row, x.grid, nullptr, nullptr, nullptr};
   p.box = box_rows(a);
-  p.grid = x.grid;
   p.scale_log2 = a.scale * kLog2e;
   p.out32 = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
-  uint8_t* ws = reinterpret_cast<uint8_t*>(a.workspace);
-  p.cost = reinterpret_cast<long long*>(ws);
-  p.bounds = reinterpret_cast<Boundary*>(ws += x.steps);
-  p.cuts = reinterpret_cast<Cut*>(ws += x.bounds);
-  p.part_ml = reinterpret_cast<float2*>(ws += x.cuts);
-  p.part_o = reinterpret_cast<float4*>(ws += x.part_ml);
+  uint8_t* ws = ranges_at(p.ranges, reinterpret_cast<uint8_t*>(a.workspace));
+  p.part_ml = reinterpret_cast<float2*>(ws);
+  p.part_o = reinterpret_cast<float4*>(ws + x.part_ml);
   CUtensorMap mq, mk, mv;
   CUresult r = encode_q(&mq, a, x.t);
   if (r == CUDA_SUCCESS) r = encode_kv(&mk, a.k, a, p.box < C::k_rows ? p.box : C::k_rows);
@@ -817,7 +659,7 @@ int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
   // the register hand-over waits for good if the launch gives the CTA fewer than it takes
   static const int regs = [&] { cudaFuncAttributes f; return cudaFuncGetAttributes(&f, kernel) == cudaSuccess ? f.numRegs : 0; }();
   if (regs != C::regs_launch) { set_error("prompt_sdpa: the kernel is launched with %d registers a thread, %d expected", regs, C::regs_launch); return DFLASH_ERR_CUDA; }
-  plan_kernel<<<1, 1024, 0, stream>>>(p, 2 * x.t.Tt);
+  plan_kernel<<<1, 1024, 0, stream>>>(p);
   DFLASH_LAUNCH_CHECK();
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];

@@ -27,6 +27,12 @@ __host__ __device__ constexpr uint32_t idesc(int m, int n, bool b_mn) {
   return (1u << 4) | (f << 7) | (f << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
+// packed fp32: (x, y) * s + (u, v) and (x, y) + (u, v), one instruction each
+__device__ __forceinline__ float2 fma2v(float x, float y, float s, float u, float v) {
+  return __ffma2_rn(make_float2(x, y), make_float2(s, s), make_float2(u, v));
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+
 // Rows of a query tile: the Gt query heads of one KV head for consecutive tokens, head fastest, so that a tile spans as
 // few positions as possible and a group of heads fills it even when there are few tokens.
 struct Tiling {
