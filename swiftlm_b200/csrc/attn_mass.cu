@@ -2,13 +2,13 @@
 //     mass[b, h, n] += sum over the rows r of h's query heads that see n of 2^(scale log2(e) q_r . k_n - log2(e) lse_r)
 //
 // Computed as S^T = K Q^T on the tensor cores (tcgen05): 128 keys are the lanes of tensor memory and 128 query rows its
-// columns, so that the sum over rows stays inside a thread and nothing is reduced across lanes; four threads share a key.
+// columns, so that the sum over rows stays inside a thread and nothing is reduced across lanes; two or four threads share a key.
 // A unit of work is one key tile, its steps are the query tiles that see it.  Few rows (a verify block, the last rows of a
 // prompt: one query tile): every key is read once and used by 128 rows, bound by HBM; the query tile stays in shared
 // memory.  Many rows: 2 D operations and one exponential a pair of row and key, bound by the 16 exponentials a clock of
 // an SM (1024 clocks a tile against 512 of products at D = 128), the key tile stays and query tiles stream.
 //
-// Warps: 0 loads key and query tiles (whichever changed), 1 the rows' -log2(e) lse, 2 issues the products, 4-19 sum.  Four
+// Warps: 0 loads key and query tiles (whichever changed), 1 and 3 the rows' -log2(e) lse, 2 issues the products, 4-19 sum.  Four
 // score buffers in tensor memory let the products run ahead.  Units are cut into equal ranges per CTA (ranges.cuh);
 // pieces of a cut unit leave 128 sums in the workspace, added in order by join_kernel: the order of every sum is fixed.
 #include "ranges.cuh"
@@ -41,8 +41,8 @@ template <int D> struct Cfg {
                        b_s_free = b_s_full + kBuffers, b_z_full = b_s_free + kBuffers, n_bars = b_z_full + kBuffers;
   static constexpr int misc = bars + (8 * n_bars + 15) / 16 * 16;
   static constexpr int z = misc + 16;                       // [kBuffers][128] -log2(e) lse of the rows
-  static constexpr int sums = z + kBuffers * 128 * 4;       // [2][4][128] of the four threads of a key
-  static constexpr int total = sums + 2 * 4 * 128 * 4;
+  static constexpr int sums = z + kBuffers * 128 * 4;       // [2][4][128] of a key's four threads, [2 groups][2][2][128] of two
+  static constexpr int total = sums + 2 * (2 * 4 * 128 * 4);
 };
 static_assert(Cfg<256>::total <= 232448 && Cfg<128>::total <= 232448 && Cfg<64>::total <= 232448, "shared memory");
 
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(1024) mass_plan_kernel(const MassParams p) {
 struct Step {
   int b, h, n0, gc, t0;        // t0: first token of the query tile
   RowLens len;
-  bool new_k, new_q, last;     // the first step of a unit; another query tile than the step before; the last step of a unit
+  bool new_k, new_q, last, single;   // the first step of a unit; another query tile than before; the last step; the only one
   int slot;                    // of the unit (see RangeWalker::take)
 };
 struct Steps {
@@ -107,6 +107,7 @@ struct Steps {
       tt0 = x.first / p.t.Tt;
       per_gc = x.last / p.t.Tt - tt0 + 1;
       hi = w.take(i, p.t.GC * per_gc, s.slot);
+      s.single = hi - i == 1;
     }
     s.gc = p.t.GC == 1 ? 0 : i / per_gc;
     s.t0 = (tt0 + i - s.gc * per_gc) * p.t.Tt;
@@ -136,7 +137,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
   if (threadIdx.x == 0) {
     ptx::prefetch_tensormap(&map_q);
     ptx::prefetch_tensormap(&map_k);
-    for (int i = 0; i < C::n_bars; ++i) ptx::mbar_init(&bars[i], i >= C::b_s_free && i < C::b_z_full ? kSumWarps : 1);
+    for (int i = 0; i < C::n_bars; ++i) ptx::mbar_init(&bars[i], i >= C::b_s_free && i < C::b_z_full ? kSumWarps / 2 : 1);
     *abort_flag = (ptx::smem_u32(sm) & 1023u) != 0u;      // swizzled tiles need 1024-byte alignment; never seen violated
     if (*abort_flag) atomicExch(a.status, kStatusSmemAlign);
     ptx::fence_mbar_init();
@@ -195,28 +196,51 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         ++n_q;
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || warp == 3) {
     // --------------------------------- log-sum-exp ----------------------------------
+    // The two warps take the steps in turn, each loading its next one's values before it hands over this one's.
     float* z = reinterpret_cast<float*>(sm + C::z);
-    uint32_t n = 0;
-    bool ok = true;
-    while (ok && st.next()) {
-      const uint32_t buf = n % kBuffers;
-      float v[4];
+    long long off[4];                                         // lane i has the rows 4 i ... 4 i + 3 of a query tile
+    int tok[4], head[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = lane * 4 + i, g = s.gc * p.t.Gt + r % p.t.Gt, t = s.t0 + r / p.t.Gt;
-        v[i] = -INFINITY;                                     // rows not in use, and rows that see nothing, add nothing
-        if (r < p.t.Gt * p.t.Tt && g < p.t.G && t < s.len.rows) {
-          const float x = a.lse[((long long)s.b * a.Hq + s.h * p.t.G + g) * a.T + t];
-          if (x > -INFINITY) v[i] = -x * kLog2e;
-        }
-      }
-      if (n >= kBuffers) ok = __all_sync(0xffffffffu, wait(C::b_s_free + buf, (n / kBuffers - 1) & 1));
-      *reinterpret_cast<float4*>(z + buf * 128 + lane * 4) = make_float4(v[0], v[1], v[2], v[3]);
+    for (int i = 0; i < 4; ++i) {
+      const int r = lane * 4 + i;
+      head[i] = r < p.t.Gt * p.t.Tt ? r % p.t.Gt : p.t.G;     // G: no such head
+      tok[i] = r / p.t.Gt;
+      off[i] = (long long)head[i] * a.T + tok[i];
+    }
+    auto fetch = [&](float (&v)[4]) {
+      const float* base = a.lse + ((long long)s.b * a.Hq + s.h * p.t.G + s.gc * p.t.Gt) * a.T + s.t0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)                             // rows not in use add nothing
+        v[i] = s.gc * p.t.Gt + head[i] < p.t.G && s.t0 + tok[i] < s.len.rows ? base[off[i]] : -INFINITY;
+    };
+    uint32_t n = 0;
+    auto advance = [&]() {                                    // to this warp's next step
+      bool more = st.next();
+      if (more && (n++ & 1u) != (uint32_t)(warp >> 1)) { more = st.next(); ++n; }
+      return more;
+    };
+    float v[4], next[4];
+    bool more = advance(), ok = true;
+    uint32_t step = n - 1;
+    if (more) fetch(v);
+    while (ok && more) {
+      const uint32_t buf = step % kBuffers, round = step / kBuffers;
+      more = advance();
+      step = n - 1;
+      if (more) fetch(next);
+      if (round > 0) ok = __all_sync(0xffffffffu, wait(C::b_s_free + buf, (round - 1) & 1));
+      float4 x;                                               // neither do rows that see nothing: their lse is -infinity
+      x.x = v[0] > -INFINITY ? -v[0] * kLog2e : -INFINITY;
+      x.y = v[1] > -INFINITY ? -v[1] * kLog2e : -INFINITY;
+      x.z = v[2] > -INFINITY ? -v[2] * kLog2e : -INFINITY;
+      x.w = v[3] > -INFINITY ? -v[3] * kLog2e : -INFINITY;
+      *reinterpret_cast<float4*>(z + buf * 128 + lane * 4) = x;
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&bars[C::b_z_full + buf]);
-      ++n;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = next[i];
     }
   } else if (warp == 2) {
     // ---------------------------------- S^T = K Q^T ----------------------------------
@@ -252,67 +276,84 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     }
   } else if (warp >= 4) {
     // ------------------------------------- sums --------------------------------------
-    const int wq = warp & 3, quarter = (warp - 4) >> 2;       // tensor-memory lane quarter; which 32 rows of a query tile
-    const int key = wq * 32 + lane, col0 = quarter * 32;
+    // Two groups of eight warps take the steps in turn; in a group two threads share a key, 64 rows each.
+    const int wq = warp & 3, group = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;   // wq: tensor-memory lane quarter
+    const int key = wq * 32 + lane;
     const float* z = reinterpret_cast<const float*>(sm + C::z);
     float* sums = reinterpret_cast<float*>(sm + C::sums);
-    uint32_t n = 0, units = 0;
+    uint32_t n = 0, n_all = 0, n_single = 0;
     float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     float before = 0.f;
-    while (st.next()) {
+    for (; st.next(); ++n) {
+      const bool mine = (n & 1u) == (uint32_t)group;          // this step is this group's
+      const bool writer = half == 0 && (s.single ? mine : group == 0) && s.n0 + key < s.len.keys;
       float* out = a.mass + ((long long)s.b * a.Hkv + s.h) * a.mass_stride + s.n0 + key;
-      const bool mine = quarter == 0 && s.n0 + key < s.len.keys;
       if (s.new_k) {
         acc[0] = acc[1] = make_float2(0.f, 0.f);
-        if (mine && s.slot < 0) before = *out;                // wanted at the unit's end
+        if (writer && s.slot < 0) before = *out;              // wanted at the unit's end
       }
-      const uint32_t buf = n % kBuffers, par = (n / kBuffers) & 1;
-      wait(C::b_s_full + buf, par);
-      wait(C::b_z_full + buf, par);
-      __syncwarp();
-      ptx::tc_fence_after();
-      uint32_t x[32];
-      ptx::tmem_ld32(tmem + ((uint32_t)(wq * 32) << 16) + buf * 128 + col0, x);
-      ptx::tmem_ld_wait();
-      const int p0 = s.len.keys - s.len.rows + s.t0, p1 = p0 + p.t.Tt - 1;      // positions of the tile's tokens
-      const bool whole = s.n0 + kKeys - 1 <= p0 && (a.window == 0 || s.n0 > p1 - a.window || s.n0 + kKeys <= a.sinks) && s.t0 + p.t.Tt <= s.len.rows;
-      if (!whole) {
-        // rows [lo, hi) of the tile see this key: the tokens from it on, up to a window behind it, that are in use
+      if (mine) {
+        const uint32_t buf = n % kBuffers, par = (n / kBuffers) & 1;
+        wait(C::b_s_full + buf, par);
+        wait(C::b_z_full + buf, par);
+        __syncwarp();
+        ptx::tc_fence_after();
+        const int p0 = s.len.keys - s.len.rows + s.t0, p1 = p0 + p.t.Tt - 1;      // positions of the tile's tokens
+        const bool whole = s.n0 + kKeys - 1 <= p0 && (a.window == 0 || s.n0 > p1 - a.window || s.n0 + kKeys <= a.sinks) && s.t0 + p.t.Tt <= s.len.rows;
+        // otherwise rows [lo, hi) of the tile see this key: the tokens from it on, up to a window behind it, that are in use
         const int nn = s.n0 + key;
         int lo = nn - p0, hi = p.t.Tt < s.len.rows - s.t0 ? p.t.Tt : s.len.rows - s.t0;
         if (a.window > 0 && nn >= a.sinks && nn + a.window - p0 < hi) hi = nn + a.window - p0;
         lo = lo < 0 ? 0 : (lo > kRows ? kRows : lo);
         hi = hi < 0 ? 0 : hi;
-        const uint32_t seen = bits_below(hi * p.t.Gt - col0) & ~bits_below(lo * p.t.Gt - col0);
+#pragma unroll 1
+        for (int col = half * 64; col < half * 64 + 64; col += 32) {
+          uint32_t x[32];
+          ptx::tmem_ld32(tmem + ((uint32_t)(wq * 32) << 16) + buf * 128 + col, x);
+          ptx::tmem_ld_wait();
+          if (!whole) {
+            const uint32_t seen = bits_below(hi * p.t.Gt - col) & ~bits_below(lo * p.t.Gt - col);
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (!((seen >> i) & 1u)) x[i] = 0xff800000u;        // -infinity
-      }
-      const float4* zp = reinterpret_cast<const float4*>(z + buf * 128 + col0);
+            for (int i = 0; i < 32; ++i)
+              if (!((seen >> i) & 1u)) x[i] = 0xff800000u;    // -infinity
+          }
+          const float4* zp = reinterpret_cast<const float4*>(z + buf * 128 + col);
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) {
-        const float4 zi = zp[i / 4];
-        float2 u = fma2v(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), p.scale_log2, zi.x, zi.y);
-        float2 w = fma2v(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]), p.scale_log2, zi.z, zi.w);
-        u.x = mma::exp2_approx(u.x); u.y = mma::exp2_approx(u.y);
-        w.x = mma::exp2_approx(w.x); w.y = mma::exp2_approx(w.y);
-        acc[0] = add2(acc[0], u);
-        acc[1] = add2(acc[1], w);
-      }
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&bars[C::b_s_free + buf]);
-      ++n;
-      if (s.last) {
-        // the four threads of a key, in order; the slot of two units ago has been read before the last unit's meeting
-        float* slot = sums + (units++ & 1) * 512;
-        slot[quarter * 128 + key] = (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
-        asm volatile("bar.sync 1, %0;" ::"n"(kSumWarps * 32) : "memory");
-        if (quarter == 0) {
-          const float total = (slot[key] + slot[128 + key]) + (slot[256 + key] + slot[384 + key]);
-          if (s.slot >= 0) p.part[(long long)s.slot * 128 + key] = total;
-          else if (mine) *out = before + total;
+          for (int i = 0; i < 32; i += 4) {
+            const float4 zi = zp[i / 4];
+            float2 u = fma2v(__uint_as_float(x[i]), __uint_as_float(x[i + 1]), p.scale_log2, zi.x, zi.y);
+            float2 w = fma2v(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]), p.scale_log2, zi.z, zi.w);
+            u.x = mma::exp2_approx(u.x); u.y = mma::exp2_approx(u.y);
+            w.x = mma::exp2_approx(w.x); w.y = mma::exp2_approx(w.y);
+            acc[0] = add2(acc[0], u);
+            acc[1] = add2(acc[1], w);
+          }
         }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&bars[C::b_s_free + buf]);
+      }
+      if (!s.last) continue;
+      // A key's threads, in order.  Each kind of slot is used every other time: the one of two times ago was read before
+      // the last meeting.
+      const float sum = (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+      float total;
+      if (s.single) {                                         // one step: one group's matter, the other goes on
+        if (!mine) continue;
+        float* slot = sums + 1024 + group * 512 + (n_single++ & 1) * 256;
+        slot[half * 128 + key] = sum;
+        asm volatile("bar.sync %0, %1;" ::"r"(2 + group), "n"(kSumWarps * 16) : "memory");
+        total = slot[key] + slot[128 + key];
+      } else {
+        float* slot = sums + (n_all++ & 1) * 512;
+        slot[(group * 2 + half) * 128 + key] = sum;
+        asm volatile("bar.sync 1, %0;" ::"n"(kSumWarps * 32) : "memory");
+        total = (slot[key] + slot[128 + key]) + (slot[256 + key] + slot[384 + key]);
+      }
+      if (s.slot >= 0) {
+        if (half == 0 && (s.single || group == 0)) p.part[(long long)s.slot * 128 + key] = total;
+      } else if (writer) {
+        *out = before + total;
       }
     }
   }

@@ -3,16 +3,19 @@
 // For every (sequence, KV head) with n > budget tokens: keep the first S, the last R and the need = budget - S - R
 // heaviest of the m = n - S - R between, move the kept rows to the front in the order they are in.
 //
-// select_kernel, one CTA per (sequence, KV head): the need-th largest mass by radix selection on the masses' bits
-// (32-bit keys whose unsigned order is the floats' order; 11 + 11 + 10 bits, one histogram in shared memory per digit),
-// then one pass that writes the kept places in ascending order by a block-wide count: a token stays when its key is above
-// the threshold, or equal to it and among the first (need - above) equals.  No atomic decides an order, so ties
-// go to the lowest index on every run.
-// move_kernel: a kept row only moves towards the front (its new place j <= its old place idx[j]) and the places
-// ascend, so a CTA that owns one column slice of one (sequence, KV head) may go through the rows in chunks in place:
-// it loads a whole chunk, meets at a barrier, and stores it.  What later chunks still have to read lies at or behind their
-// own places, in front of which the stores of this chunk end.
+// select_kernel, one cluster of 1 to 8 CTAs per (sequence, KV head), a CTA for every 4096 tokens: the need-th largest mass by
+// radix selection on the masses' bits (32-bit keys whose unsigned order is the floats' order; 11 + 11 + 10 bits, a
+// histogram in each CTA's shared memory per digit, added up through distributed shared memory), then one pass that writes
+// the kept places in ascending order by counts in front: a token stays when its key is above the threshold, or equal to it and
+// among the first (need - above) equals.  No atomic decides an order, so ties go to the lowest index on every run.
+// Masses are read four times, from L2; one CTA for 32768 tokens took 38 us.
+// move_kernel: a kept row only moves towards the front (its new place j <= its old place) and the places ascend,
+// so a CTA that owns one column slice of one (sequence, KV head) may go through the rows in chunks in place: it loads a whole
+// chunk, meets at a barrier, and stores it.  What later chunks still have to read lies at or behind their own places,
+// in front of which the stores of this chunk end: the next chunk's loads are in flight while this one is stored, and one
+// barrier a chunk is enough.  Bound by HBM: every row that moves is read once and written once.
 #include "common.cuh"
+#include "ptx.cuh"
 
 namespace dflash {
 namespace {
@@ -24,12 +27,14 @@ struct EvictParams {
   int32_t* kv_len_out;
   float* mass_out;
   int32_t* kept;          // [B*Hkv, kept_stride]
+  int2* moves;            // [B*Hkv] rows that stay, first of them that moves
   int B, Hkv, N, page_tokens, max_pages, num_pages, mass_stride, budget, recent, sinks, kept_stride;
   int row_bytes;
   int* status;
 };
 
-constexpr int kSelThreads = 1024;
+constexpr int kMaxCluster = 8;
+constexpr int kSelThreads = 1024, kPer = 4, kChunk = kSelThreads * kPer;   // tokens of one CTA at a time
 
 // unsigned order of the key = order of the float; -0 and +0 are equal, every NaN is above +inf
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -61,52 +66,81 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t mine, uint32_t& total,
   return x - mine + (warp ? base : 0u);
 }
 
-__global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p) {
+__device__ __forceinline__ uint32_t peer_load(const uint32_t* mine, uint32_t rank) {   // the same word in CTA `rank` of the cluster
+  uint32_t x;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(ptx::cluster_addr(mine, rank)) : "memory");
+  return x;
+}
+
+__global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p, int C) {
   __shared__ uint32_t hist[2048];
   __shared__ uint32_t warp_sums[32];
-  __shared__ uint32_t s_digit, s_left;
-  const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
-  const long long unit = (long long)b * p.Hkv + h;
+  __shared__ uint32_t s_digit, s_left, s_counts[2], s_first;
+  const int unit = blockIdx.x / C, b = unit / p.Hkv, tid = threadIdx.x;
+  const uint32_t rank = blockIdx.x - unit * C;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  auto meet = [&]() {
+    __syncwarp();
+    if (C > 1) ptx::cluster_sync();
+    else __syncthreads();
+  };
   int n = p.kv_len[b];
   if (n < 0 || n > p.N) {
-    if (tid == 0 && h == 0) atomicExch(p.status, kStatusCacheLen);
+    if (tid == 0 && unit == b * p.Hkv && rank == 0) atomicExch(p.status, kStatusCacheLen);
     n = n < 0 ? 0 : p.N;
   }
-  const float* mass = p.mass + unit * p.mass_stride;
-  float* mass_out = p.mass_out + unit * p.mass_stride;
-  int32_t* kept = p.kept + unit * p.kept_stride;
+  const float* mass = p.mass + (long long)unit * p.mass_stride;
+  float* mass_out = p.mass_out + (long long)unit * p.mass_stride;
+  int32_t* kept = p.kept + (long long)unit * p.kept_stride;
   const int left = n < p.budget ? n : p.budget;
-  for (int i = left + tid; i < p.kept_stride; i += kSelThreads) kept[i] = -1;
-  if (n <= p.budget) {
-    for (int i = tid; i < n; i += kSelThreads) {
+  const int all = tid + (int)rank * kSelThreads, stride = C * kSelThreads;
+  for (int i = left + all; i < p.kept_stride; i += stride) kept[i] = -1;
+  if (n <= p.budget) {                                      // the same in every CTA of the cluster
+    for (int i = all; i < n; i += stride) {
       kept[i] = i;
       mass_out[i] = mass[i];
     }
+    if (all == 0) p.moves[unit] = make_int2(left, left);
     return;
   }
   const int lo = p.sinks, hi = n - p.recent;
   uint32_t need = (uint32_t)(p.budget - p.sinks - p.recent);
+  if (tid == 0) s_first = (uint32_t)left;
   // ---- the need-th largest key of [lo, hi), digit by digit ----
   uint32_t threshold = 0, mask = 0;
   if (need > 0) {
-#pragma unroll
+#pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
       for (int i = tid; i < bins; i += kSelThreads) hist[i] = 0;
       __syncthreads();
-      for (int i = lo + tid; i < hi; i += kSelThreads) {
+#pragma unroll 4
+      for (int i = lo + all; i < hi; i += stride) {
         const uint32_t key = order_key(mass[i]);
         if ((key & mask) == threshold) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
       }
-      __syncthreads();
+      meet();
       // from the top: the digit in which the running count reaches `need`
       const int per = bins / kSelThreads;                 // 2 or 1 bins a thread, thread 0 has the highest
-      uint32_t c[2] = {hist[bins - 1 - tid * per], per == 2 ? hist[bins - 2 - tid * per] : 0u};
+      uint32_t c[2] = {0, 0};
+      if (C == 1) {
+        c[0] = hist[bins - 1 - tid * per];
+        if (per == 2) c[1] = hist[bins - 2 - tid * per];
+      } else {                                            // all loads in flight together
+        uint32_t x[2][kMaxCluster] = {};
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) {
+          if (r < C) x[0][r] = peer_load(&hist[bins - 1 - tid * per], r);
+          if (r < C && per == 2) x[1][r] = peer_load(&hist[bins - 2 - tid * per], r);
+        }
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) { c[0] += x[0][r]; c[1] += x[1][r]; }
+      }
       uint32_t total;
       const uint32_t before = block_prefix(c[0] + c[1], total, warp_sums);
       if (before < need && need <= before + c[0]) { s_digit = bins - 1 - tid * per; s_left = need - before; }
       else if (before + c[0] < need && need <= before + c[0] + c[1]) { s_digit = bins - 2 - tid * per; s_left = need - before - c[0]; }
-      __syncthreads();
+      meet();                                             // also: every CTA has read the histograms
       threshold |= s_digit << shift;
       mask |= (uint32_t)(bins - 1) << shift;
       need = s_left;
@@ -115,43 +149,69 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p
   }
   const uint32_t equals = need;                          // how many tokens equal to the threshold stay
   const bool any = p.budget > p.sinks + p.recent;
-  // ---- kept places, ascending ----
+  // ---- kept places, ascending: CTA r of the cluster takes chunk r of every round, a thread kPer tokens in a row ----
   uint32_t done = 0, eq_done = 0;
-  for (int base = 0; base < n; base += kSelThreads) {
-    const int i = base + tid;
-    float w = 0.f;
-    bool sure = false, eq = false;
-    if (i < n) {
-      w = mass[i];
-      if (i < lo || i >= hi) sure = true;
+  for (int base = 0; base < n; base += C * kChunk) {
+    const int i0 = base + (int)rank * kChunk + tid * kPer;
+    float w[kPer];
+    uint32_t sure = 0, eq = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) w[j] = i0 + j < n ? mass[i0 + j] : 0.f;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int i = i0 + j;
+      if (i >= n) continue;
+      if (i < lo || i >= hi) sure |= 1u << j;
       else if (any) {
-        const uint32_t key = order_key(w);
-        sure = key > threshold;
-        eq = key == threshold;
+        const uint32_t key = order_key(w[j]);
+        sure |= key > threshold ? 1u << j : 0u;
+        eq |= key == threshold ? 1u << j : 0u;
       }
     }
-    uint32_t total;
-    const uint32_t at = block_prefix((sure ? 1u : 0u) | (eq ? 0x10000u : 0u), total, warp_sums);
-    const uint32_t eq_at = eq_done + (at >> 16);
-    const uint32_t eq_before = eq_at < equals ? eq_at : equals;          // equals in front of this one that stay
-    const uint32_t slot = done + (at & 0xffffu) + eq_before;              // done counts the sure ones only
-    if (sure || (eq && eq_at < equals)) {
-      kept[slot] = i;
-      mass_out[slot] = w;                                               // slot <= i, and this chunk has been read
+    uint32_t total;                                       // both counts of a chunk are at most 4096
+    const uint32_t at = block_prefix(__popc(sure) | (__popc(eq) << 16), total, warp_sums);
+    if (tid == 0) s_counts[0] = total;
+    meet();                                               // every CTA has read its chunk and counted
+    uint32_t sure_at = done + (at & 0xffffu), eq_at = eq_done + (at >> 16);
+    uint32_t counts[kMaxCluster];
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) counts[r] = C == 1 ? total : (r < C ? peer_load(&s_counts[0], r) : 0u);
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      if (r >= C) break;
+      const uint32_t c = counts[r];
+      if (r < (int)rank) { sure_at += c & 0xffffu; eq_at += c >> 16; }
+      done += c & 0xffffu;
+      eq_done += c >> 16;
     }
-    done += total & 0xffffu;
-    eq_done += total >> 16;
-    __syncthreads();
+    uint32_t first = 0xffffffffu;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const bool e = (eq >> j) & 1u, on = ((sure >> j) & 1u) || (e && eq_at < equals);
+      if (on) {
+        const uint32_t slot = sure_at + (eq_at < equals ? eq_at : equals);
+        kept[slot] = i0 + j;
+        mass_out[slot] = w[j];                            // slot <= token, and this round has been read
+        if (slot != (uint32_t)(i0 + j) && slot < first) first = slot;
+      }
+      sure_at += (sure >> j) & 1u;
+      eq_at += e;
+    }
+    first = __reduce_min_sync(0xffffffffu, first);
+    if ((tid & 31) == 0 && first < s_first) atomicMin(&s_first, first);
+    meet();                                               // s_counts is used again
   }
-  for (int i = left + tid; i < n; i += kSelThreads) mass_out[i] = 0.f;
-}
-
-__global__ void lens_kernel(const EvictParams p) {
-  const int b = blockIdx.x * blockDim.x + threadIdx.x;
-  if (b >= p.B) return;
-  int n = p.kv_len[b];
-  n = n < 0 ? 0 : (n > p.N ? p.N : n);
-  p.kv_len_out[b] = n < p.budget ? n : p.budget;
+  for (int i = left + all; i < n; i += stride) mass_out[i] = 0.f;
+  // the first row that moves
+  if (tid == 0 && rank == 0) {
+    uint32_t first = s_first;
+    for (int r = 1; r < C; ++r) {
+      const uint32_t x = peer_load(&s_first, r);
+      first = x < first ? x : first;
+    }
+    p.moves[unit] = make_int2(left, (int)first);
+  }
+  meet();                                                 // no CTA leaves while another reads its shared memory
 }
 
 // byte address of token n's row of (b, h), or -1
@@ -165,46 +225,73 @@ __device__ __forceinline__ long long row_at(const EvictParams& p, int b, int h, 
   return (((long long)page * p.Hkv + h) * p.page_tokens + n % p.page_tokens) * p.row_bytes;
 }
 
-constexpr int kMoveThreads = 256, kMoveVecs = 4;
-// One CTA: columns [16 * vecs * blockIdx.x, ...) of K (z = 0) or V (z = 1) of one (b, h).
+constexpr int kMoveThreads = 256, kMoveRows = 4;           // rows a thread has in flight in one chunk
+// One CTA: `vecs` 16-byte columns from vecs * blockIdx.x on, of K (z = 0) or V (z = 1) of one (b, h).
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const EvictParams p, int vecs) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int unit = blockIdx.y, b = unit / p.Hkv, h = unit % p.Hkv;
+  const int2 range = p.moves[unit];
+  if (blockIdx.x == 0 && blockIdx.z == 0 && h == 0 && threadIdx.x == 0) p.kv_len_out[b] = range.x;   // kv_len may be the same array
   const int32_t* kept = p.kept + (long long)unit * p.kept_stride;
-  uint8_t* x = blockIdx.z ? p.v : p.k;
-  const int rows_per = kMoveThreads / vecs, col = (blockIdx.x * vecs + threadIdx.x % vecs) * 16;
-  const int limit = p.kept_stride < p.budget ? p.kept_stride : p.budget;
-  if (threadIdx.x / vecs >= rows_per) return;   // never: vecs is a power of two
+  const int per = kMoveThreads / vecs, col = (blockIdx.x * vecs + threadIdx.x % vecs) * 16, row = threadIdx.x / vecs;
+  uint8_t* x = (blockIdx.z ? p.v : p.k) + col;
   const bool live = col < p.row_bytes;
-  for (int j0 = 0; j0 < limit; j0 += rows_per * kMoveVecs) {
-    uint4 val[kMoveVecs];
-    long long dst[kMoveVecs];
+  const int chunk = per * kMoveRows;
+  if (range.y >= range.x) return;                // nothing moves
+  // Three chunks are under way: the places of one are looked up, the rows of the next are loaded, those of the last stored.
+  long long from[2][kMoveRows];
+  uint4 val[2][kMoveRows];
+  uint32_t moves[2];
+  auto place = [&](int j0, long long (&f)[kMoveRows]) {
+    int src[kMoveRows];
 #pragma unroll
-    for (int u = 0; u < kMoveVecs; ++u) {
-      const int j = j0 + u * rows_per + threadIdx.x / vecs;
-      dst[u] = -1;
-      const int src = j < limit ? kept[j] : -1;
-      if (live && src > j) {                     // src == j: the row is where it belongs
-        const long long from = row_at(p, b, h, src), to = row_at(p, b, h, j);
-        if (from >= 0 && to >= 0) {
-          val[u] = *reinterpret_cast<const uint4*>(x + from + col);
-          dst[u] = to + col;
-        }
-      }
+    for (int u = 0; u < kMoveRows; ++u) {
+      const int j = j0 + u * per + row;
+      src[u] = live && j < range.x ? kept[j] : -1;
     }
-    __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kMoveVecs; ++u)
-      if (dst[u] >= 0) *reinterpret_cast<uint4*>(x + dst[u]) = val[u];
+    for (int u = 0; u < kMoveRows; ++u) f[u] = src[u] > j0 + u * per + row ? row_at(p, b, h, src[u]) : -1;   // equal: it is where it belongs
+  };
+  auto load = [&](const long long (&f)[kMoveRows], uint4 (&v)[kMoveRows], uint32_t& m) {
+    m = 0;
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u)
+      if (f[u] >= 0) {
+        v[u] = *reinterpret_cast<const uint4*>(x + f[u]);
+        m |= 1u << u;
+      }
+  };
+  auto store = [&](int j0, const uint4 (&v)[kMoveRows], uint32_t m) {
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u)
+      if ((m >> u) & 1u) {
+        const long long to = row_at(p, b, h, j0 + u * per + row);
+        if (to >= 0) *reinterpret_cast<uint4*>(x + to) = v[u];
+      }
+  };
+  place(range.y, from[0]);
+  load(from[0], val[0], moves[0]);
+  place(range.y + chunk, from[1]);
+  for (int j0 = range.y; j0 < range.x; j0 += 2 * chunk) {
     __syncthreads();
+    load(from[1], val[1], moves[1]);
+    place(j0 + 2 * chunk, from[0]);
+    store(j0, val[0], moves[0]);
+    __syncthreads();
+    load(from[0], val[0], moves[0]);
+    place(j0 + 3 * chunk, from[1]);
+    store(j0 + chunk, val[1], moves[1]);
   }
 }
 
 }  // namespace
 }  // namespace dflash
 
+static size_t moves_bytes(int B, int Hkv) { return ((size_t)B * Hkv * sizeof(int2) + 255) / 256 * 256; }
+
 extern "C" size_t dflash_kv_evict_workspace_bytes(int32_t B, int32_t Hkv, int32_t N, int32_t budget) {
   if (B <= 0 || Hkv <= 0 || N <= 0 || budget <= 0) return 0;
-  return ((size_t)B * Hkv * (size_t)(budget < N ? budget : N) * 4 + 255) / 256 * 256;
+  return moves_bytes(B, Hkv) + ((size_t)B * Hkv * (size_t)(budget < N ? budget : N) * 4 + 255) / 256 * 256;
 }
 
 extern "C" int32_t dflash_kv_evict(void* k_cache, void* v_cache, const int32_t* page_table, const int32_t* kv_len, const float* mass,
@@ -225,33 +312,41 @@ extern "C" int32_t dflash_kv_evict(void* k_cache, void* v_cache, const int32_t* 
   auto off = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; };
   if (row_bytes % 16 != 0 || row_bytes > (1 << 20) || off(k_cache, 16) || off(v_cache, 16))
     return invalid("rows must be multiples of 16 bytes (at most 1 MiB) and the caches 16-byte aligned");
-  if (off(page_table, 4) || off(kv_len, 4) || off(mass, 4) || off(kv_len_out, 4) || off(mass_out, 4) || off(kept, 4) || off(workspace, 4))
+  if (off(page_table, 4) || off(kv_len, 4) || off(mass, 4) || off(kv_len_out, 4) || off(mass_out, 4) || off(kept, 4) || off(workspace, 16))
     return invalid("misaligned pointer");
-  if ((long long)B * Hkv > 65535 || B > 65535) { set_error("kv_evict: more than 65535 (sequence, head) pairs"); return DFLASH_ERR_UNSUPPORTED; }
+  if ((long long)B * Hkv > 65535) { set_error("kv_evict: more than 65535 (sequence, head) pairs"); return DFLASH_ERR_UNSUPPORTED; }
   const int stride = kept ? budget : (budget < N ? budget : N);
-  if (!kept) {
-    const size_t need = dflash_kv_evict_workspace_bytes(B, Hkv, N, budget);
-    if (!workspace || workspace_bytes < need) {
-      set_error("kv_evict: workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
-      return DFLASH_ERR_WORKSPACE;
-    }
-    kept = reinterpret_cast<int32_t*>(workspace);
+  const size_t need = dflash_kv_evict_workspace_bytes(B, Hkv, N, budget);
+  if (!workspace || workspace_bytes < need) {
+    set_error("kv_evict: workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+    return DFLASH_ERR_WORKSPACE;
   }
+  if (!kept) kept = reinterpret_cast<int32_t*>(reinterpret_cast<uint8_t*>(workspace) + moves_bytes(B, Hkv));
   int* status = device_status_word();
   if (!status) { set_error("no CUDA device"); return DFLASH_ERR_CUDA; }
   EvictParams p{reinterpret_cast<uint8_t*>(k_cache), reinterpret_cast<uint8_t*>(v_cache), page_table, kv_len, mass, kv_len_out, mass_out,
-                kept, B, Hkv, N, page_tokens, max_pages, num_pages, mass_stride, budget, recent, sinks, stride, (int)row_bytes, status};
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  select_kernel<<<dim3(Hkv, B), kSelThreads, 0, s>>>(p);
-  DFLASH_LAUNCH_CHECK();
-  lens_kernel<<<(B + 127) / 128, 128, 0, s>>>(p);      // behind select_kernel, which reads kv_len: the two may be one array
-  DFLASH_LAUNCH_CHECK();
-  if (budget < N) {                                    // else no sequence can be longer than the budget
-    const int vecs = 4;
-    move_kernel<<<dim3((unsigned)((row_bytes / 16 + vecs - 1) / vecs), B * Hkv, 2), kMoveThreads, 0, s>>>(p, vecs);
-    DFLASH_LAUNCH_CHECK();
-    count_launch();
-  }
+                kept, reinterpret_cast<int2*>(workspace), B, Hkv, N, page_tokens, max_pages, num_pages, mass_stride, budget, recent, sinks,
+                stride, (int)row_bytes, status};
+  int C = 1;
+  while (C < kMaxCluster && N > C * kChunk) C *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+  cfg.gridDim = dim3(B * Hkv * C);
+  cfg.blockDim = dim3(kSelThreads);
+  DFLASH_CUDA_CHECK(cudaLaunchKernelEx(&cfg, select_kernel, p, C));
+  // 64 bytes of a row a CTA: 32 would halve the bytes of a memory access, 128 halve the CTAs of a small batch
+  const int vecs = 4;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)((row_bytes / 16 + vecs - 1) / vecs), B * Hkv, 2);
+  cfg.blockDim = dim3(kMoveThreads);
+  DFLASH_CUDA_CHECK(cudaLaunchKernelEx(&cfg, move_kernel, p, vecs));
   count_launch(2);
   return DFLASH_OK;
 }

@@ -475,7 +475,7 @@ def kv_evict(k_cache, v_cache, mass, kv_len, budget: int, recent: int, sinks: in
         raise _bad("kept must be a contiguous int32 tensor [B, Hkv, budget]")
     with _on_device_of(k_cache):
         L = _lib.lib()
-        ws = _scratch(0 if kept is not None else L.dflash_kv_evict_workspace_bytes(B, Hkv, N, budget), k_cache.device)
+        ws = _scratch(L.dflash_kv_evict_workspace_bytes(B, Hkv, N, budget), k_cache.device)
         _lib.check(L.dflash_kv_evict(
             _ptr(k_cache), _ptr(v_cache), _ptr(page_table), _ptr(kv_len), _ptr(mass), _ptr(kv_len_out), _ptr(mass_out), _ptr(kept),
             _ptr(ws), 0 if ws is None else ws.numel(), B, Hkv, D, N, page_tokens, max_pages, num_pages, mass.shape[2], budget,
