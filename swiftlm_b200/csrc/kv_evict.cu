@@ -66,6 +66,9 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t mine, uint32_t& total,
   return x - mine + (warp ? base : 0u);
 }
 
+__device__ __forceinline__ void peer_add(const uint32_t* mine, uint32_t rank, uint32_t x) {
+  asm volatile("red.shared::cluster.add.u32 [%0], %1;" ::"r"(ptx::cluster_addr(mine, rank)), "r"(x) : "memory");
+}
 __device__ __forceinline__ uint32_t peer_load(const uint32_t* mine, uint32_t rank) {   // the same word in CTA `rank` of the cluster
   uint32_t x;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(ptx::cluster_addr(mine, rank)) : "memory");
@@ -73,9 +76,9 @@ __device__ __forceinline__ uint32_t peer_load(const uint32_t* mine, uint32_t ran
 }
 
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p, int C) {
-  __shared__ uint32_t hist[2048];
+  __shared__ uint32_t hist[2048], hist_all[2048];          // this CTA's counts, the cluster's
   __shared__ uint32_t warp_sums[32];
-  __shared__ uint32_t s_digit, s_left, s_counts[2], s_first;
+  __shared__ uint32_t s_digit, s_left, s_count, s_counts[kMaxCluster], s_first;
   const int unit = blockIdx.x / C, b = unit / p.Hkv, tid = threadIdx.x;
   const uint32_t rank = blockIdx.x - unit * C;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -109,38 +112,37 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p
   // ---- the need-th largest key of [lo, hi), digit by digit ----
   uint32_t threshold = 0, mask = 0;
   if (need > 0) {
+    for (int i = tid; i < 2048; i += kSelThreads) hist[i] = hist_all[i] = 0;
+    meet();
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
-      for (int i = tid; i < bins; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
+      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048, per = bins / kSelThreads;
 #pragma unroll 4
       for (int i = lo + all; i < hi; i += stride) {
         const uint32_t key = order_key(mass[i]);
         if ((key & mask) == threshold) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
       }
-      meet();
-      // from the top: the digit in which the running count reaches `need`
-      const int per = bins / kSelThreads;                 // 2 or 1 bins a thread, thread 0 has the highest
-      uint32_t c[2] = {0, 0};
-      if (C == 1) {
-        c[0] = hist[bins - 1 - tid * per];
-        if (per == 2) c[1] = hist[bins - 2 - tid * per];
-      } else {                                            // all loads in flight together
-        uint32_t x[2][kMaxCluster] = {};
-#pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r) {
-          if (r < C) x[0][r] = peer_load(&hist[bins - 1 - tid * per], r);
-          if (r < C && per == 2) x[1][r] = peer_load(&hist[bins - 2 - tid * per], r);
+      if (C > 1) {
+        // Masses have few leading digits: a CTA adds its few counts to every CTA's sums.  (Each thread reading its bins
+        // from eight CTAs took 14000 clocks a digit.)
+        __syncthreads();
+        for (int i = tid; i < bins; i += kSelThreads) {
+          const uint32_t c = hist[i];
+          if (c)
+            for (int r = 0; r < C; ++r) peer_add(&hist_all[i], r, c);
         }
-#pragma unroll
-        for (int r = 0; r < kMaxCluster; ++r) { c[0] += x[0][r]; c[1] += x[1][r]; }
       }
+      meet();
+      // from the top: the digit in which the running count reaches `need`; thread 0 has the highest of 2 or 1 bins a thread
+      uint32_t* sums = C > 1 ? hist_all : hist;
+      const int top = bins - 1 - tid * per;
+      const uint32_t c0 = sums[top], c1 = per == 2 ? sums[top - 1] : 0u;
       uint32_t total;
-      const uint32_t before = block_prefix(c[0] + c[1], total, warp_sums);
-      if (before < need && need <= before + c[0]) { s_digit = bins - 1 - tid * per; s_left = need - before; }
-      else if (before + c[0] < need && need <= before + c[0] + c[1]) { s_digit = bins - 2 - tid * per; s_left = need - before - c[0]; }
-      meet();                                             // also: every CTA has read the histograms
+      const uint32_t before = block_prefix(c0 + c1, total, warp_sums);
+      if (before < need && need <= before + c0) { s_digit = top; s_left = need - before; }
+      else if (before + c0 < need && need <= before + c0 + c1) { s_digit = top - 1; s_left = need - before - c0; }
+      for (int i = tid; i < 2048; i += kSelThreads) hist[i] = hist_all[i] = 0;     // all threads have read theirs
+      meet();
       threshold |= s_digit << shift;
       mask |= (uint32_t)(bins - 1) << shift;
       need = s_left;
@@ -170,16 +172,13 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p
     }
     uint32_t total;                                       // both counts of a chunk are at most 4096
     const uint32_t at = block_prefix(__popc(sure) | (__popc(eq) << 16), total, warp_sums);
-    if (tid == 0) s_counts[0] = total;
+    if (tid == 0) s_count = total;
     meet();                                               // every CTA has read its chunk and counted
+    if (tid < C) s_counts[tid] = C == 1 ? total : peer_load(&s_count, tid);
+    __syncthreads();
     uint32_t sure_at = done + (at & 0xffffu), eq_at = eq_done + (at >> 16);
-    uint32_t counts[kMaxCluster];
-#pragma unroll
-    for (int r = 0; r < kMaxCluster; ++r) counts[r] = C == 1 ? total : (r < C ? peer_load(&s_counts[0], r) : 0u);
-#pragma unroll
-    for (int r = 0; r < kMaxCluster; ++r) {
-      if (r >= C) break;
-      const uint32_t c = counts[r];
+    for (int r = 0; r < C; ++r) {
+      const uint32_t c = s_counts[r];
       if (r < (int)rank) { sure_at += c & 0xffffu; eq_at += c >> 16; }
       done += c & 0xffffu;
       eq_done += c >> 16;
@@ -199,7 +198,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p
     }
     first = __reduce_min_sync(0xffffffffu, first);
     if ((tid & 31) == 0 && first < s_first) atomicMin(&s_first, first);
-    meet();                                               // s_counts is used again
+    meet();                                               // the counts are used again
   }
   for (int i = left + all; i < n; i += stride) mass_out[i] = 0.f;
   // the first row that moves
@@ -214,20 +213,11 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p
   meet();                                                 // no CTA leaves while another reads its shared memory
 }
 
-// byte address of token n's row of (b, h), or -1
-__device__ __forceinline__ long long row_at(const EvictParams& p, int b, int h, int n) {
-  if (!p.page_table) return (((long long)b * p.Hkv + h) * p.N + n) * p.row_bytes;
-  const int page = p.page_table[(long long)b * p.max_pages + n / p.page_tokens];
-  if ((unsigned)page >= (unsigned)p.num_pages) {
-    atomicExch(p.status, kStatusKvRange);
-    return -1;
-  }
-  return (((long long)page * p.Hkv + h) * p.page_tokens + n % p.page_tokens) * p.row_bytes;
-}
-
-constexpr int kMoveThreads = 256, kMoveRows = 4;           // rows a thread has in flight in one chunk
+constexpr int kMoveThreads = 256, kMoveRows = 8;           // rows a thread has in flight in one chunk
+constexpr int kMovePages = 4096;                          // entries of the page table that fit in shared memory
 // One CTA: `vecs` 16-byte columns from vecs * blockIdx.x on, of K (z = 0) or V (z = 1) of one (b, h).
-__global__ void __launch_bounds__(kMoveThreads) move_kernel(const EvictParams p, int vecs) {
+__global__ void __launch_bounds__(kMoveThreads, 2) move_kernel(const EvictParams p, int vecs) {
+  __shared__ int32_t pages[kMovePages];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int unit = blockIdx.y, b = unit / p.Hkv, h = unit % p.Hkv;
   const int2 range = p.moves[unit];
@@ -238,6 +228,25 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const EvictParams p,
   const bool live = col < p.row_bytes;
   const int chunk = per * kMoveRows;
   if (range.y >= range.x) return;                // nothing moves
+  // the part of the page table that holds kept rows, where it fits: two dependent look-ups less in front of a row's load
+  const int32_t* table = p.page_table ? p.page_table + (long long)b * p.max_pages : nullptr;
+  if (table) {
+    const int used = kept[range.x - 1] / p.page_tokens + 1;
+    if (used <= kMovePages) {
+      for (int i = threadIdx.x; i < used; i += kMoveThreads) pages[i] = table[i];
+      table = pages;
+      __syncthreads();
+    }
+  }
+  auto row_at = [&](int n) -> long long {        // byte offset of token n's row, -1: its page is outside the pool
+    if (!table) return (((long long)b * p.Hkv + h) * p.N + n) * p.row_bytes;
+    const int index = n / p.page_tokens, page = table[index];
+    if ((unsigned)page >= (unsigned)p.num_pages) {
+      atomicExch(p.status, kStatusKvRange);
+      return -1;
+    }
+    return (((long long)page * p.Hkv + h) * p.page_tokens + n - index * p.page_tokens) * p.row_bytes;
+  };
   // Three chunks are under way: the places of one are looked up, the rows of the next are loaded, those of the last stored.
   long long from[2][kMoveRows];
   uint4 val[2][kMoveRows];
@@ -250,7 +259,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const EvictParams p,
       src[u] = live && j < range.x ? kept[j] : -1;
     }
 #pragma unroll
-    for (int u = 0; u < kMoveRows; ++u) f[u] = src[u] > j0 + u * per + row ? row_at(p, b, h, src[u]) : -1;   // equal: it is where it belongs
+    for (int u = 0; u < kMoveRows; ++u) f[u] = src[u] > j0 + u * per + row ? row_at(src[u]) : -1;   // equal: it is where it belongs
   };
   auto load = [&](const long long (&f)[kMoveRows], uint4 (&v)[kMoveRows], uint32_t& m) {
     m = 0;
@@ -265,7 +274,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const EvictParams p,
 #pragma unroll
     for (int u = 0; u < kMoveRows; ++u)
       if ((m >> u) & 1u) {
-        const long long to = row_at(p, b, h, j0 + u * per + row);
+        const long long to = row_at(j0 + u * per + row);
         if (to >= 0) *reinterpret_cast<uint4*>(x + to) = v[u];
       }
   };
