@@ -8,7 +8,8 @@
 // memory.  Many rows: 2 D operations and one exponential a pair of row and key, bound by the 16 exponentials a clock of
 // an SM (1024 clocks a tile against 512 of products at D = 128), the key tile stays and query tiles stream.
 //
-// Warps: 0 loads key and query tiles (whichever changed), 1 and 3 the rows' -log2(e) lse, 2 issues the products, 4-19 sum.  Four
+// Warps: 0 loads key and query tiles (whichever changed), 1 the rows' -log2(e) lse, 2 issues the products, 3 walks the
+// steps, 4-19 sum.  Four
 // score buffers in tensor memory let the products run ahead.  Units are cut into equal ranges per CTA (ranges.cuh);
 // pieces of a cut unit leave 128 sums in the workspace, added in order by join_kernel: the order of every sum is fixed.
 #include "ranges.cuh"
@@ -23,6 +24,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kUnitCost = 1;                 // what a unit costs besides its query tiles
 constexpr int kSumWarps = 16, kThreads = 128 + kSumWarps * 32;
 constexpr int kBuffers = 4;
+constexpr int kRing = 16;                    // steps that are described ahead
 
 struct MassParams {
   CacheArgs a;
@@ -33,16 +35,25 @@ struct MassParams {
   float* part;                 // [2 * grid][128]
 };
 
+// One step: a key tile against a query tile.
+enum : int { kNewKeys = 1, kNewQueries = 2, kLast = 4, kSingle = 8, kEnd = 16 };   // the first step of a unit; another query tile than
+struct __align__(16) Step {                                                        // before; the last step; the only one; no step
+  int b, h, n0, gc;
+  int t0, keys, rows, flags;   // t0: first token of the query tile; the sequence's lengths
+  int slot, pad[3];            // of the unit (see RangeWalker::take)
+};
+
 template <int D> struct Cfg {
   static constexpr int NC = D / 64, tile = NC * kChunk;
   static constexpr int tiles = D == 256 ? 3 : 6;            // tiles of keys and queries together
   static constexpr int bars = tiles * tile;
   static constexpr int b_k_full = 0, b_k_empty = tiles, b_q_full = 2 * tiles, b_q_empty = 3 * tiles, b_s_full = 4 * tiles,
-                       b_s_free = b_s_full + kBuffers, b_z_full = b_s_free + kBuffers, n_bars = b_z_full + kBuffers;
+                       b_s_free = b_s_full + kBuffers, b_z_full = b_s_free + kBuffers, b_step = b_z_full + kBuffers, n_bars = b_step + kRing;
   static constexpr int misc = bars + (8 * n_bars + 15) / 16 * 16;
   static constexpr int z = misc + 16;                       // [kBuffers][128] -log2(e) lse of the rows
   static constexpr int sums = z + kBuffers * 128 * 4;       // [2][4][128] of a key's four threads, [2 groups][2][2][128] of two
-  static constexpr int total = sums + 2 * (2 * 4 * 128 * 4);
+  static constexpr int steps = sums + 2 * (2 * 4 * 128 * 4);   // [kRing] Step
+  static constexpr int total = steps + kRing * (int)sizeof(Step);
 };
 static_assert(Cfg<256>::total <= 232448 && Cfg<128>::total <= 232448 && Cfg<64>::total <= 232448, "shared memory");
 
@@ -76,13 +87,6 @@ __global__ void __launch_bounds__(1024) mass_plan_kernel(const MassParams p) {
   plan_ranges<kUnitCost>(p.ranges, p.a, [&](RowLens len, int u) { return tile_steps(p.a, p.t, len, u); });
 }
 
-// One step: a key tile against a query tile.
-struct Step {
-  int b, h, n0, gc, t0;        // t0: first token of the query tile
-  RowLens len;
-  bool new_k, new_q, last, single;   // the first step of a unit; another query tile than before; the last step; the only one
-  int slot;                    // of the unit (see RangeWalker::take)
-};
 struct Steps {
   const MassParams& p;
   RangeWalker w;
@@ -92,8 +96,8 @@ struct Steps {
   __device__ Steps(const MassParams& p_, int worker) : p(p_), w(p_.ranges, p_.a, worker), i(0), hi(0), any(false) {}
   __device__ bool next() {
     const int b = s.b, h = s.h, gc = s.gc, t0 = s.t0;
-    s.new_k = ++i >= hi || !any;
-    if (s.new_k) {
+    int flags = ++i >= hi || !any ? kNewKeys : 0;
+    if (flags) {
       if (!w.find([&](RowLens len, int u) {
             u = next_tile(p.a, len, u, p.ranges.per_row);
             while (u < p.ranges.per_row && tile_steps(p.a, p.t, len, u) == 0) u = next_tile(p.a, len, u + 1, p.ranges.per_row);
@@ -101,18 +105,20 @@ struct Steps {
           }, i)) return false;
       s.b = w.c.b;
       s.h = w.c.hg;
-      s.len = w.c.len;
+      s.keys = w.c.len.keys;
+      s.rows = w.c.len.rows;
       s.n0 = w.c.u * kKeys;
-      const Seeing x = seeing(p.a, s.len, s.n0);
+      const Seeing x = seeing(p.a, w.c.len, s.n0);
       tt0 = x.first / p.t.Tt;
       per_gc = x.last / p.t.Tt - tt0 + 1;
       hi = w.take(i, p.t.GC * per_gc, s.slot);
-      s.single = hi - i == 1;
+      if (hi - i == 1) flags |= kSingle;
     }
     s.gc = p.t.GC == 1 ? 0 : i / per_gc;
     s.t0 = (tt0 + i - s.gc * per_gc) * p.t.Tt;
-    s.new_q = !any || b != s.b || h != s.h || gc != s.gc || t0 != s.t0;
-    s.last = i == hi - 1;
+    if (!any || b != s.b || h != s.h || gc != s.gc || t0 != s.t0) flags |= kNewQueries;
+    if (i == hi - 1) flags |= kLast;
+    s.flags = flags;
     any = true;
     return true;
   }
@@ -160,15 +166,28 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
   // A wait that gives up raises the abort flag, after which every wait returns at once: the roles run through their loops
   // without results, meet at the end and leave.
   auto wait = [&](int bar, uint32_t parity) { return ptx::mbar_wait_or_abort(&bars[bar], parity, abort_flag, a.status, kStatusMbarWait); };
-  Steps st(p, blockIdx.x);
-  const Step& s = st.s;
+  // Warp 3 walks the CTA's steps and describes them in a ring; the others read.  (Every role walking for itself was five
+  // copies of that code: an eighth of the instruction fetches missed and each step took 2350 clocks.)
+  Step* ring = reinterpret_cast<Step*>(sm + C::steps);
+  auto step_at = [&](uint32_t n) {                            // step n; flags = kEnd behind the last
+    Step x;
+    if (!wait(C::b_step + n % kRing, (n / kRing) & 1)) { x.flags = kEnd; return x; }
+    const int4* src = reinterpret_cast<const int4*>(&ring[n % kRing]);
+    int4* dst = reinterpret_cast<int4*>(&x);
+    dst[0] = src[0];
+    dst[1] = src[1];
+    dst[2] = src[2];
+    return x;
+  };
 
   if (warp == 0) {
     // ------------------------------- keys and queries -------------------------------
     uint32_t n_k = 0, n_q = 0;
     bool ok = !*abort_flag;
-    while (ok && st.next()) {
-      if (s.new_k) {
+    for (uint32_t n = 0; ok; ++n) {
+      const Step s = step_at(n);
+      if (s.flags & kEnd) break;
+      if (s.flags & kNewKeys) {
         const uint32_t at = n_k % p.k_stages;
         if (n_k >= (uint32_t)p.k_stages) ok = __all_sync(0xffffffffu, wait(C::b_k_empty + at, (n_k / p.k_stages - 1) & 1));
         if (!ok) break;
@@ -176,14 +195,14 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         __syncwarp();
         const int pieces = kKeys / p.box;
         for (int i = lane; i < NC * pieces; i += 32) {
-          const int c = i / pieces, n = s.n0 + (i - c * pieces) * p.box;
-          const TilePlace x = place_of(a, s.b, n, s.len.keys);
-          ptx::tma_load_4d(sm + at * C::tile + c * kChunk + (n - s.n0) * 128, &map_k, c * 64, x.row, s.h, x.outer, &bars[C::b_k_full + at]);
+          const int c = i / pieces, key = s.n0 + (i - c * pieces) * p.box;
+          const TilePlace x = place_of(a, s.b, key, s.keys);
+          ptx::tma_load_4d(sm + at * C::tile + c * kChunk + (key - s.n0) * 128, &map_k, c * 64, x.row, s.h, x.outer, &bars[C::b_k_full + at]);
         }
         __syncwarp();
         ++n_k;
       }
-      if (s.new_q) {
+      if (s.flags & kNewQueries) {
         const uint32_t at = n_q % p.q_stages;
         if (n_q >= (uint32_t)p.q_stages) ok = __all_sync(0xffffffffu, wait(C::b_q_empty + at, (n_q / p.q_stages - 1) & 1));
         if (!ok) break;
@@ -196,9 +215,26 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         ++n_q;
       }
     }
-  } else if (warp == 1 || warp == 3) {
+  } else if (warp == 3) {
+    // ------------------------------------- steps -------------------------------------
+    // A slot is written again when the sums of sixteen steps ago are done; those of four ago are waited for, in order.
+    Steps st(p, blockIdx.x);
+    bool more = true, ok = true;
+    for (uint32_t n = 0; ok && more; ++n) {
+      more = st.next();
+      if (!more) st.s.flags = kEnd;
+      if (n >= kRing - kBuffers) {
+        const uint32_t done = n - (kRing - kBuffers);
+        ok = __all_sync(0xffffffffu, wait(C::b_s_free + done % kBuffers, (done / kBuffers) & 1));
+      }
+      if (lane == 0) {
+        ring[n % kRing] = st.s;
+        ptx::mbar_arrive(&bars[C::b_step + n % kRing]);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 1) {
     // --------------------------------- log-sum-exp ----------------------------------
-    // The two warps take the steps in turn, each loading its next one's values before it hands over this one's.
     float* z = reinterpret_cast<float*>(sm + C::z);
     long long off[4];                                         // lane i has the rows 4 i ... 4 i + 3 of a query tile
     int tok[4], head[4];
@@ -209,54 +245,59 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
       tok[i] = r / p.t.Gt;
       off[i] = (long long)head[i] * a.T + tok[i];
     }
-    auto fetch = [&](float (&v)[4]) {
+    auto fetch = [&](uint32_t n, float (&v)[4]) {             // false: there is no step n
+      const Step s = step_at(n);
+      if (s.flags & kEnd) return false;
       const float* base = a.lse + ((long long)s.b * a.Hq + s.h * p.t.G + s.gc * p.t.Gt) * a.T + s.t0;
 #pragma unroll
       for (int i = 0; i < 4; ++i)                             // rows not in use add nothing
-        v[i] = s.gc * p.t.Gt + head[i] < p.t.G && s.t0 + tok[i] < s.len.rows ? base[off[i]] : -INFINITY;
+        v[i] = s.gc * p.t.Gt + head[i] < p.t.G && s.t0 + tok[i] < s.rows ? base[off[i]] : -INFINITY;
+      return true;
     };
-    uint32_t n = 0;
-    auto advance = [&]() {                                    // to this warp's next step
-      bool more = st.next();
-      if (more && (n++ & 1u) != (uint32_t)(warp >> 1)) { more = st.next(); ++n; }
-      return more;
-    };
-    float v[4], next[4];
-    bool more = advance(), ok = true;
-    uint32_t step = n - 1;
-    if (more) fetch(v);
-    while (ok && more) {
-      const uint32_t buf = step % kBuffers, round = step / kBuffers;
-      more = advance();
-      step = n - 1;
-      if (more) fetch(next);
-      if (round > 0) ok = __all_sync(0xffffffffu, wait(C::b_s_free + buf, (round - 1) & 1));
-      float4 x;                                               // neither do rows that see nothing: their lse is -infinity
-      x.x = v[0] > -INFINITY ? -v[0] * kLog2e : -INFINITY;
-      x.y = v[1] > -INFINITY ? -v[1] * kLog2e : -INFINITY;
-      x.z = v[2] > -INFINITY ? -v[2] * kLog2e : -INFINITY;
-      x.w = v[3] > -INFINITY ? -v[3] * kLog2e : -INFINITY;
-      *reinterpret_cast<float4*>(z + buf * 128 + lane * 4) = x;
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&bars[C::b_z_full + buf]);
+    float v[kBuffers][4];                                     // values on their way
+    uint32_t have = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = next[i];
+    for (int i = 0; i < kBuffers - 1; ++i)
+      if (have == (uint32_t)i && fetch(i, v[i])) ++have;
+    bool ok = true, more = have == kBuffers - 1;
+    for (uint32_t n0 = 0; ok && n0 < have; n0 += kBuffers) {
+#pragma unroll
+      for (int k = 0; k < kBuffers; ++k) {
+        const uint32_t n = n0 + k;
+        if (!ok || n >= have) break;
+        if (more) {
+          more = fetch(n + kBuffers - 1, v[(k + kBuffers - 1) % kBuffers]);
+          have += more;
+        }
+        if (n >= kBuffers) ok = __all_sync(0xffffffffu, wait(C::b_s_free + k, (n / kBuffers - 1) & 1));
+        float4 x;                                             // neither do rows that see nothing: their lse is -infinity
+        x.x = v[k][0] > -INFINITY ? -v[k][0] * kLog2e : -INFINITY;
+        x.y = v[k][1] > -INFINITY ? -v[k][1] * kLog2e : -INFINITY;
+        x.z = v[k][2] > -INFINITY ? -v[k][2] * kLog2e : -INFINITY;
+        x.w = v[k][3] > -INFINITY ? -v[k][3] * kLog2e : -INFINITY;
+        *reinterpret_cast<float4*>(z + k * 128 + lane * 4) = x;
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&bars[C::b_z_full + k]);
+      }
     }
   } else if (warp == 2) {
     // ---------------------------------- S^T = K Q^T ----------------------------------
     constexpr uint32_t kI = idesc<T>(kKeys, kRows, false);
-    uint32_t n = 0, n_k = 0, n_q = 0;
+    uint32_t n_k = 0, n_q = 0;
     bool ok = true;
-    while (ok && st.next()) {
+    for (uint32_t n = 0; ok; ++n) {
+      const int flags = step_at(n).flags;
+      if (flags & kEnd) break;
       // the tiles that are not needed any more are free once the products so far are done
-      if (s.new_k && n_k > 0 && ptx::elect_one()) ptx::umma_commit(&bars[C::b_k_empty + (n_k - 1) % p.k_stages]);
-      if (s.new_q && n_q > 0 && ptx::elect_one()) ptx::umma_commit(&bars[C::b_q_empty + (n_q - 1) % p.q_stages]);
+      if ((flags & kNewKeys) && n_k > 0 && ptx::elect_one()) ptx::umma_commit(&bars[C::b_k_empty + (n_k - 1) % p.k_stages]);
       __syncwarp();
-      n_k += s.new_k;
-      n_q += s.new_q;
+      if ((flags & kNewQueries) && n_q > 0 && ptx::elect_one()) ptx::umma_commit(&bars[C::b_q_empty + (n_q - 1) % p.q_stages]);
+      __syncwarp();
+      n_k += (flags & kNewKeys) != 0;
+      n_q += (flags & kNewQueries) != 0;
       const uint32_t ka = (n_k - 1) % p.k_stages, qa = (n_q - 1) % p.q_stages, buf = n % kBuffers;
-      if (s.new_k) ok = wait(C::b_k_full + ka, ((n_k - 1) / p.k_stages) & 1);
-      if (s.new_q) ok = ok && wait(C::b_q_full + qa, ((n_q - 1) / p.q_stages) & 1);
+      if (flags & kNewKeys) ok = wait(C::b_k_full + ka, ((n_k - 1) / p.k_stages) & 1);
+      if (flags & kNewQueries) ok = ok && wait(C::b_q_full + qa, ((n_q - 1) / p.q_stages) & 1);
       if (n >= kBuffers) ok = ok && wait(C::b_s_free + buf, (n / kBuffers - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -272,7 +313,6 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         ptx::umma_commit(&bars[C::b_s_full + buf]);
       }
       __syncwarp();
-      ++n;
     }
   } else if (warp >= 4) {
     // ------------------------------------- sums --------------------------------------
@@ -281,14 +321,16 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     const int key = wq * 32 + lane;
     const float* z = reinterpret_cast<const float*>(sm + C::z);
     float* sums = reinterpret_cast<float*>(sm + C::sums);
-    uint32_t n = 0, n_all = 0, n_single = 0;
+    uint32_t n_all = 0, n_single = 0;
     float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     float before = 0.f;
-    for (; st.next(); ++n) {
-      const bool mine = (n & 1u) == (uint32_t)group;          // this step is this group's
-      const bool writer = half == 0 && (s.single ? mine : group == 0) && s.n0 + key < s.len.keys;
+    for (uint32_t n = 0;; ++n) {
+      const Step s = step_at(n);
+      if (s.flags & kEnd) break;
+      const bool mine = (n & 1u) == (uint32_t)group, single = s.flags & kSingle;   // mine: this step is this group's
+      const bool writer = half == 0 && (single ? mine : group == 0) && s.n0 + key < s.keys;
       float* out = a.mass + ((long long)s.b * a.Hkv + s.h) * a.mass_stride + s.n0 + key;
-      if (s.new_k) {
+      if (s.flags & kNewKeys) {
         acc[0] = acc[1] = make_float2(0.f, 0.f);
         if (writer && s.slot < 0) before = *out;              // wanted at the unit's end
       }
@@ -298,11 +340,11 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         wait(C::b_z_full + buf, par);
         __syncwarp();
         ptx::tc_fence_after();
-        const int p0 = s.len.keys - s.len.rows + s.t0, p1 = p0 + p.t.Tt - 1;      // positions of the tile's tokens
-        const bool whole = s.n0 + kKeys - 1 <= p0 && (a.window == 0 || s.n0 > p1 - a.window || s.n0 + kKeys <= a.sinks) && s.t0 + p.t.Tt <= s.len.rows;
+        const int p0 = s.keys - s.rows + s.t0, p1 = p0 + p.t.Tt - 1;      // positions of the tile's tokens
+        const bool whole = s.n0 + kKeys - 1 <= p0 && (a.window == 0 || s.n0 > p1 - a.window || s.n0 + kKeys <= a.sinks) && s.t0 + p.t.Tt <= s.rows;
         // otherwise rows [lo, hi) of the tile see this key: the tokens from it on, up to a window behind it, that are in use
         const int nn = s.n0 + key;
-        int lo = nn - p0, hi = p.t.Tt < s.len.rows - s.t0 ? p.t.Tt : s.len.rows - s.t0;
+        int lo = nn - p0, hi = p.t.Tt < s.rows - s.t0 ? p.t.Tt : s.rows - s.t0;
         if (a.window > 0 && nn >= a.sinks && nn + a.window - p0 < hi) hi = nn + a.window - p0;
         lo = lo < 0 ? 0 : (lo > kRows ? kRows : lo);
         hi = hi < 0 ? 0 : hi;
@@ -333,12 +375,12 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&bars[C::b_s_free + buf]);
       }
-      if (!s.last) continue;
+      if (!(s.flags & kLast)) continue;
       // A key's threads, in order.  Each kind of slot is used every other time: the one of two times ago was read before
       // the last meeting.
       const float sum = (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
       float total;
-      if (s.single) {                                         // one step: one group's matter, the other goes on
+      if (single) {                                           // one step: one group's matter, the other goes on
         if (!mine) continue;
         float* slot = sums + 1024 + group * 512 + (n_single++ & 1) * 256;
         slot[half * 128 + key] = sum;
@@ -351,7 +393,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         total = (slot[key] + slot[128 + key]) + (slot[256 + key] + slot[384 + key]);
       }
       if (s.slot >= 0) {
-        if (half == 0 && (s.single || group == 0)) p.part[(long long)s.slot * 128 + key] = total;
+        if (half == 0 && (single || group == 0)) p.part[(long long)s.slot * 128 + key] = total;
       } else if (writer) {
         *out = before + total;
       }

@@ -26,9 +26,10 @@ struct EvictParams {
   const float* mass;
   int32_t* kv_len_out;
   float* mass_out;
-  int32_t* kept;          // [B*Hkv, kept_stride]
+  int32_t* kept;          // [B*Hkv, budget] or null
   int2* moves;            // [B*Hkv] rows that stay, first of them that moves
-  int B, Hkv, N, page_tokens, max_pages, num_pages, mass_stride, budget, recent, sinks, kept_stride;
+  longlong2* places;      // [B*Hkv, stride] byte offsets of a row that stays: where it is, where it goes; .x < 0: nothing to do
+  int B, Hkv, N, page_tokens, max_pages, num_pages, mass_stride, budget, recent, sinks, stride;
   int row_bytes;
   int* status;
 };
@@ -75,6 +76,17 @@ __device__ __forceinline__ uint32_t peer_load(const uint32_t* mine, uint32_t ran
   return x;
 }
 
+// byte offset of token n's row of (b, h); -1: its page is outside the pool
+__device__ __forceinline__ long long row_at(const EvictParams& p, int b, int h, int n) {
+  if (!p.page_table) return (((long long)b * p.Hkv + h) * p.N + n) * p.row_bytes;
+  const int page = p.page_table[(long long)b * p.max_pages + n / p.page_tokens];
+  if ((unsigned)page >= (unsigned)p.num_pages) {
+    atomicExch(p.status, kStatusKvRange);
+    return -1;
+  }
+  return (((long long)page * p.Hkv + h) * p.page_tokens + n % p.page_tokens) * p.row_bytes;
+}
+
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p, int C) {
   __shared__ uint32_t hist[2048], hist_all[2048];          // this CTA's counts, the cluster's
   __shared__ uint32_t warp_sums[32];
@@ -94,13 +106,15 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p
   }
   const float* mass = p.mass + (long long)unit * p.mass_stride;
   float* mass_out = p.mass_out + (long long)unit * p.mass_stride;
-  int32_t* kept = p.kept + (long long)unit * p.kept_stride;
+  int32_t* kept = p.kept ? p.kept + (long long)unit * p.budget : nullptr;
+  longlong2* places = p.places + (long long)unit * p.stride;
   const int left = n < p.budget ? n : p.budget;
   const int all = tid + (int)rank * kSelThreads, stride = C * kSelThreads;
-  for (int i = left + all; i < p.kept_stride; i += stride) kept[i] = -1;
+  if (kept)
+    for (int i = left + all; i < p.budget; i += stride) kept[i] = -1;
   if (n <= p.budget) {                                      // the same in every CTA of the cluster
     for (int i = all; i < n; i += stride) {
-      kept[i] = i;
+      if (kept) kept[i] = i;
       mass_out[i] = mass[i];
     }
     if (all == 0) p.moves[unit] = make_int2(left, left);
@@ -189,8 +203,14 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p
       const bool e = (eq >> j) & 1u, on = ((sure >> j) & 1u) || (e && eq_at < equals);
       if (on) {
         const uint32_t slot = sure_at + (eq_at < equals ? eq_at : equals);
-        kept[slot] = i0 + j;
+        if (kept) kept[slot] = i0 + j;
         mass_out[slot] = w[j];                            // slot <= token, and this round has been read
+        longlong2 at2 = make_longlong2(-1, -1);           // looked up here once a row, not by every thread that moves a part of it
+        if (slot != (uint32_t)(i0 + j)) {
+          at2 = make_longlong2(row_at(p, b, unit - b * p.Hkv, i0 + j), row_at(p, b, unit - b * p.Hkv, (int)slot));
+          if (at2.y < 0) at2.x = -1;
+        }
+        places[slot] = at2;
         if (slot != (uint32_t)(i0 + j) && slot < first) first = slot;
       }
       sure_at += (sure >> j) & 1u;
@@ -213,83 +233,52 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p
   meet();                                                 // no CTA leaves while another reads its shared memory
 }
 
-constexpr int kMoveThreads = 256, kMoveRows = 8;           // rows a thread has in flight in one chunk
-constexpr int kMovePages = 4096;                          // entries of the page table that fit in shared memory
+// Rows a thread has in flight in one chunk, with 64 bytes of a row a CTA.  Measured at 32 x 1104 tokens and 8 x 32768 (whole
+// call): 2 rows 35 and 73 us, 4 rows 34 and 61, 8 rows 39 and 75; 32 bytes a CTA 41 and 67, 128 bytes 34 and 70.
+constexpr int kMoveThreads = 256, kMoveRows = 4;
 // One CTA: `vecs` 16-byte columns from vecs * blockIdx.x on, of K (z = 0) or V (z = 1) of one (b, h).
-__global__ void __launch_bounds__(kMoveThreads, 2) move_kernel(const EvictParams p, int vecs) {
-  __shared__ int32_t pages[kMovePages];
+__global__ void __launch_bounds__(kMoveThreads) move_kernel(const EvictParams p, int vecs) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int unit = blockIdx.y, b = unit / p.Hkv, h = unit % p.Hkv;
+  const int unit = blockIdx.y, b = unit / p.Hkv, h = unit - b * p.Hkv;
   const int2 range = p.moves[unit];
   if (blockIdx.x == 0 && blockIdx.z == 0 && h == 0 && threadIdx.x == 0) p.kv_len_out[b] = range.x;   // kv_len may be the same array
-  const int32_t* kept = p.kept + (long long)unit * p.kept_stride;
-  const int per = kMoveThreads / vecs, col = (blockIdx.x * vecs + threadIdx.x % vecs) * 16, row = threadIdx.x / vecs;
+  const int per = kMoveThreads / vecs, row = threadIdx.x / vecs, col = (blockIdx.x * vecs + threadIdx.x - row * vecs) * 16;
+  const longlong2* places = p.places + (long long)unit * p.stride + row;
   uint8_t* x = (blockIdx.z ? p.v : p.k) + col;
-  const bool live = col < p.row_bytes;
-  const int chunk = per * kMoveRows;
+  const int end = col < p.row_bytes ? range.x - row : 0, chunk = per * kMoveRows;
   if (range.y >= range.x) return;                // nothing moves
-  // the part of the page table that holds kept rows, where it fits: two dependent look-ups less in front of a row's load
-  const int32_t* table = p.page_table ? p.page_table + (long long)b * p.max_pages : nullptr;
-  if (table) {
-    const int used = kept[range.x - 1] / p.page_tokens + 1;
-    if (used <= kMovePages) {
-      for (int i = threadIdx.x; i < used; i += kMoveThreads) pages[i] = table[i];
-      table = pages;
-      __syncthreads();
-    }
-  }
-  auto row_at = [&](int n) -> long long {        // byte offset of token n's row, -1: its page is outside the pool
-    if (!table) return (((long long)b * p.Hkv + h) * p.N + n) * p.row_bytes;
-    const int index = n / p.page_tokens, page = table[index];
-    if ((unsigned)page >= (unsigned)p.num_pages) {
-      atomicExch(p.status, kStatusKvRange);
-      return -1;
-    }
-    return (((long long)page * p.Hkv + h) * p.page_tokens + n - index * p.page_tokens) * p.row_bytes;
-  };
-  // Three chunks are under way: the places of one are looked up, the rows of the next are loaded, those of the last stored.
-  long long from[2][kMoveRows];
+  // Three chunks are under way: the places of one are read, the rows of the next are loaded, those of the last stored.
+  longlong2 at[kMoveRows];
   uint4 val[2][kMoveRows];
-  uint32_t moves[2];
-  auto place = [&](int j0, long long (&f)[kMoveRows]) {
-    int src[kMoveRows];
+  long long to[2][kMoveRows];
+  auto read = [&](int j0) {
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u) at[u] = j0 + u * per < end ? places[j0 + u * per] : make_longlong2(-1, -1);
+  };
+  auto load = [&](uint4 (&v)[kMoveRows], long long (&t)[kMoveRows]) {
 #pragma unroll
     for (int u = 0; u < kMoveRows; ++u) {
-      const int j = j0 + u * per + row;
-      src[u] = live && j < range.x ? kept[j] : -1;
+      t[u] = at[u].x >= 0 ? at[u].y : -1;
+      if (at[u].x >= 0) v[u] = *reinterpret_cast<const uint4*>(x + at[u].x);
     }
-#pragma unroll
-    for (int u = 0; u < kMoveRows; ++u) f[u] = src[u] > j0 + u * per + row ? row_at(src[u]) : -1;   // equal: it is where it belongs
   };
-  auto load = [&](const long long (&f)[kMoveRows], uint4 (&v)[kMoveRows], uint32_t& m) {
-    m = 0;
+  auto store = [&](const uint4 (&v)[kMoveRows], const long long (&t)[kMoveRows]) {
 #pragma unroll
     for (int u = 0; u < kMoveRows; ++u)
-      if (f[u] >= 0) {
-        v[u] = *reinterpret_cast<const uint4*>(x + f[u]);
-        m |= 1u << u;
-      }
+      if (t[u] >= 0) *reinterpret_cast<uint4*>(x + t[u]) = v[u];
   };
-  auto store = [&](int j0, const uint4 (&v)[kMoveRows], uint32_t m) {
-#pragma unroll
-    for (int u = 0; u < kMoveRows; ++u)
-      if ((m >> u) & 1u) {
-        const long long to = row_at(j0 + u * per + row);
-        if (to >= 0) *reinterpret_cast<uint4*>(x + to) = v[u];
-      }
-  };
-  place(range.y, from[0]);
-  load(from[0], val[0], moves[0]);
-  place(range.y + chunk, from[1]);
+  read(range.y);
+  load(val[0], to[0]);
+  read(range.y + chunk);
   for (int j0 = range.y; j0 < range.x; j0 += 2 * chunk) {
     __syncthreads();
-    load(from[1], val[1], moves[1]);
-    place(j0 + 2 * chunk, from[0]);
-    store(j0, val[0], moves[0]);
+    load(val[1], to[1]);
+    read(j0 + 2 * chunk);
+    store(val[0], to[0]);
     __syncthreads();
-    load(from[0], val[0], moves[0]);
-    place(j0 + 3 * chunk, from[1]);
-    store(j0 + chunk, val[1], moves[1]);
+    load(val[0], to[0]);
+    read(j0 + 3 * chunk);
+    store(val[1], to[1]);
   }
 }
 
@@ -300,7 +289,7 @@ static size_t moves_bytes(int B, int Hkv) { return ((size_t)B * Hkv * sizeof(int
 
 extern "C" size_t dflash_kv_evict_workspace_bytes(int32_t B, int32_t Hkv, int32_t N, int32_t budget) {
   if (B <= 0 || Hkv <= 0 || N <= 0 || budget <= 0) return 0;
-  return moves_bytes(B, Hkv) + ((size_t)B * Hkv * (size_t)(budget < N ? budget : N) * 4 + 255) / 256 * 256;
+  return moves_bytes(B, Hkv) + (size_t)B * Hkv * (size_t)(budget < N ? budget : N) * sizeof(longlong2);
 }
 
 extern "C" int32_t dflash_kv_evict(void* k_cache, void* v_cache, const int32_t* page_table, const int32_t* kv_len, const float* mass,
@@ -324,18 +313,17 @@ extern "C" int32_t dflash_kv_evict(void* k_cache, void* v_cache, const int32_t* 
   if (off(page_table, 4) || off(kv_len, 4) || off(mass, 4) || off(kv_len_out, 4) || off(mass_out, 4) || off(kept, 4) || off(workspace, 16))
     return invalid("misaligned pointer");
   if ((long long)B * Hkv > 65535) { set_error("kv_evict: more than 65535 (sequence, head) pairs"); return DFLASH_ERR_UNSUPPORTED; }
-  const int stride = kept ? budget : (budget < N ? budget : N);
   const size_t need = dflash_kv_evict_workspace_bytes(B, Hkv, N, budget);
   if (!workspace || workspace_bytes < need) {
     set_error("kv_evict: workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
     return DFLASH_ERR_WORKSPACE;
   }
-  if (!kept) kept = reinterpret_cast<int32_t*>(reinterpret_cast<uint8_t*>(workspace) + moves_bytes(B, Hkv));
   int* status = device_status_word();
   if (!status) { set_error("no CUDA device"); return DFLASH_ERR_CUDA; }
   EvictParams p{reinterpret_cast<uint8_t*>(k_cache), reinterpret_cast<uint8_t*>(v_cache), page_table, kv_len, mass, kv_len_out, mass_out,
-                kept, reinterpret_cast<int2*>(workspace), B, Hkv, N, page_tokens, max_pages, num_pages, mass_stride, budget, recent, sinks,
-                stride, (int)row_bytes, status};
+                kept, reinterpret_cast<int2*>(workspace),
+                reinterpret_cast<longlong2*>(reinterpret_cast<uint8_t*>(workspace) + moves_bytes(B, Hkv)), B, Hkv, N, page_tokens, max_pages, num_pages, mass_stride, budget, recent, sinks,
+                budget < N ? budget : N, (int)row_bytes, status};
   int C = 1;
   while (C < kMaxCluster && N > C * kChunk) C *= 2;
   cudaLaunchConfig_t cfg = {};
@@ -349,7 +337,6 @@ extern "C" int32_t dflash_kv_evict(void* k_cache, void* v_cache, const int32_t* 
   cfg.gridDim = dim3(B * Hkv * C);
   cfg.blockDim = dim3(kSelThreads);
   DFLASH_CUDA_CHECK(cudaLaunchKernelEx(&cfg, select_kernel, p, C));
-  // 64 bytes of a row a CTA: 32 would halve the bytes of a memory access, 128 halve the CTAs of a small batch
   const int vecs = 4;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
