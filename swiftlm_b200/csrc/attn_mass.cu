@@ -57,6 +57,15 @@ template <int D> struct Cfg {
 };
 static_assert(Cfg<256>::total <= 232448 && Cfg<128>::total <= 232448 && Cfg<64>::total <= 232448, "shared memory");
 
+// Place in a ring of a length known at run time: stage and phase by counting, not by division.
+struct RingAt {
+  int stage = 0;
+  uint32_t round = 0;
+  __device__ void next(int stages) {
+    if (++stage == stages) { stage = 0; ++round; }
+  }
+};
+
 // query tokens of sequence (len) that see some key of [n0, n0 + 128): first and last; last < first: none
 struct Seeing { int first, last; };
 __device__ __forceinline__ Seeing seeing(const CacheArgs& a, RowLens len, int n0) {
@@ -182,37 +191,34 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
 
   if (warp == 0) {
     // ------------------------------- keys and queries -------------------------------
-    uint32_t n_k = 0, n_q = 0;
+    RingAt k, q;
+    const int pieces = kKeys / p.box, q_bytes = NC * p.t.Gt * p.t.Tt * 128;
     bool ok = !*abort_flag;
     for (uint32_t n = 0; ok; ++n) {
       const Step s = step_at(n);
       if (s.flags & kEnd) break;
       if (s.flags & kNewKeys) {
-        const uint32_t at = n_k % p.k_stages;
-        if (n_k >= (uint32_t)p.k_stages) ok = __all_sync(0xffffffffu, wait(C::b_k_empty + at, (n_k / p.k_stages - 1) & 1));
+        if (k.round > 0) ok = __all_sync(0xffffffffu, wait(C::b_k_empty + k.stage, (k.round - 1) & 1));
         if (!ok) break;
-        if (lane == 0) ptx::mbar_arrive_expect_tx(&bars[C::b_k_full + at], C::tile);
+        if (lane == 0) ptx::mbar_arrive_expect_tx(&bars[C::b_k_full + k.stage], C::tile);
         __syncwarp();
-        const int pieces = kKeys / p.box;
         for (int i = lane; i < NC * pieces; i += 32) {
           const int c = i / pieces, key = s.n0 + (i - c * pieces) * p.box;
           const TilePlace x = place_of(a, s.b, key, s.keys);
-          ptx::tma_load_4d(sm + at * C::tile + c * kChunk + (key - s.n0) * 128, &map_k, c * 64, x.row, s.h, x.outer, &bars[C::b_k_full + at]);
+          ptx::tma_load_4d(sm + k.stage * C::tile + c * kChunk + (key - s.n0) * 128, &map_k, c * 64, x.row, s.h, x.outer, &bars[C::b_k_full + k.stage]);
         }
         __syncwarp();
-        ++n_k;
+        k.next(p.k_stages);
       }
       if (s.flags & kNewQueries) {
-        const uint32_t at = n_q % p.q_stages;
-        if (n_q >= (uint32_t)p.q_stages) ok = __all_sync(0xffffffffu, wait(C::b_q_empty + at, (n_q / p.q_stages - 1) & 1));
+        if (q.round > 0) ok = __all_sync(0xffffffffu, wait(C::b_q_empty + q.stage, (q.round - 1) & 1));
         if (!ok) break;
-        if (lane == 0) {
-          ptx::mbar_arrive_expect_tx(&bars[C::b_q_full + at], NC * p.t.Gt * p.t.Tt * 128);
-          for (int c = 0; c < NC; ++c)
-            ptx::tma_load_4d(sm + q0 + at * C::tile + c * kChunk, &map_q, c * 64, s.gc * p.t.Gt, s.t0, s.b * a.Hkv + s.h, &bars[C::b_q_full + at]);
-        }
+        if (lane == 0) ptx::mbar_arrive_expect_tx(&bars[C::b_q_full + q.stage], q_bytes);
         __syncwarp();
-        ++n_q;
+        if (lane < NC)
+          ptx::tma_load_4d(sm + q0 + q.stage * C::tile + lane * kChunk, &map_q, lane * 64, s.gc * p.t.Gt, s.t0, s.b * a.Hkv + s.h, &bars[C::b_q_full + q.stage]);
+        __syncwarp();
+        q.next(p.q_stages);
       }
     }
   } else if (warp == 3) {
@@ -283,28 +289,36 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
   } else if (warp == 2) {
     // ---------------------------------- S^T = K Q^T ----------------------------------
     constexpr uint32_t kI = idesc<T>(kKeys, kRows, false);
-    uint32_t n_k = 0, n_q = 0;
+    RingAt k, q;                                              // the tiles to come
+    int ka = -1, qa = -1;                                     // the tiles in use
     bool ok = true;
     for (uint32_t n = 0; ok; ++n) {
-      const int flags = step_at(n).flags;
+      ok = wait(C::b_step + n % kRing, (n / kRing) & 1);
+      const int flags = ok ? ring[n % kRing].flags : kEnd;
       if (flags & kEnd) break;
-      // the tiles that are not needed any more are free once the products so far are done
-      if ((flags & kNewKeys) && n_k > 0 && ptx::elect_one()) ptx::umma_commit(&bars[C::b_k_empty + (n_k - 1) % p.k_stages]);
-      __syncwarp();
-      if ((flags & kNewQueries) && n_q > 0 && ptx::elect_one()) ptx::umma_commit(&bars[C::b_q_empty + (n_q - 1) % p.q_stages]);
-      __syncwarp();
-      n_k += (flags & kNewKeys) != 0;
-      n_q += (flags & kNewQueries) != 0;
-      const uint32_t ka = (n_k - 1) % p.k_stages, qa = (n_q - 1) % p.q_stages, buf = n % kBuffers;
-      if (flags & kNewKeys) ok = wait(C::b_k_full + ka, ((n_k - 1) / p.k_stages) & 1);
-      if (flags & kNewQueries) ok = ok && wait(C::b_q_full + qa, ((n_q - 1) / p.q_stages) & 1);
+      const uint32_t buf = n % kBuffers;
+      if (flags & kNewKeys) {
+        // the last one is free once the products so far are done
+        if (ka >= 0 && ptx::elect_one()) ptx::umma_commit(&bars[C::b_k_empty + ka]);
+        __syncwarp();
+        ka = k.stage;
+        ok = wait(C::b_k_full + ka, k.round & 1);
+        k.next(p.k_stages);
+      }
+      if (flags & kNewQueries) {
+        if (qa >= 0 && ptx::elect_one()) ptx::umma_commit(&bars[C::b_q_empty + qa]);
+        __syncwarp();
+        qa = q.stage;
+        ok = ok && wait(C::b_q_full + qa, q.round & 1);
+        q.next(p.q_stages);
+      }
       if (n >= kBuffers) ok = ok && wait(C::b_s_free + buf, (n / kBuffers - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       ptx::tc_fence_after();
       if (ptx::elect_one()) {
         const uint32_t d = tmem + buf * 128, k_addr = ptx::smem_u32(sm + ka * C::tile), q_addr = ptx::smem_u32(sm + q0 + qa * C::tile);
-#pragma unroll 1
+#pragma unroll
         for (int c = 0; c < NC; ++c) {
           const uint64_t da = make_desc(k_addr + c * kChunk, 16, 1024), db = make_desc(q_addr + c * kChunk, 16, 1024);
 #pragma unroll
