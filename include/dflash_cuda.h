@@ -236,8 +236,8 @@ int32_t dflash_kv_commit(int32_t* kv_len, const int32_t* commit, int32_t B, int3
  *              of the lengths (<= max_pages * page_tokens).  A page id outside the pool reads as zeros and
  *              is reported through dflash_device_status.
  *   kv_len     int32[B] or NULL (N each): cached tokens of sequence b, the queries' own tokens among them.
- *   q_len      int32[B] or NULL (T each): query rows of sequence b that are in use.  Rows behind them are neither
- *              read nor written (out, lse).
+ *   q_len      int32[B] or NULL (T each): query rows of sequence b that are in use.  Rows behind them are not used,
+ *              their rows of `out` keep what they hold, an lse that is written is -infinity there.
  *              Entries outside [0,N] and [0,T] are clamped to that range and reported (DFLASH_ERR_DEVICE_DATA).
  *   visibility query row r of sequence b stands at position p = kv_len[b] - q_len[b] + r and sees token n iff
  *              n <= p and (window == 0 or n > p - window or n < sinks).  window counts the query's own

@@ -464,7 +464,8 @@ int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
   if (r == CUDA_SUCCESS) r = encode_kv(&mk, a.k, a, p.box);
   if (r != CUDA_SUCCESS) { set_error("attention_mass: cuTensorMapEncodeTiled failed with CUresult %d", (int)r); return DFLASH_ERR_CUDA; }
   auto kernel = mass_kernel<T, D>;
-  DFLASH_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::total));
+  static std::atomic<uint64_t> ready{0};
+  DFLASH_CUDA_CHECK(allow_shared(ready, kernel, C::total));
   mass_plan_kernel<<<1, 1024, 0, stream>>>(p);
   DFLASH_LAUNCH_CHECK();
   cudaLaunchConfig_t cfg = {};

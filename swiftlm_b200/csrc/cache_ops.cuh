@@ -2,6 +2,8 @@
 // arguments, lengths and visibility.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace dflash {
@@ -47,6 +49,17 @@ __device__ __forceinline__ long long kv_row(const CacheArgs& a, int b, int h, in
 
 __device__ __forceinline__ bool sees(const CacheArgs& a, int p, int n) {
   return n <= p && (a.window == 0 || n > p - a.window || n < a.sinks);
+}
+
+// Dynamic shared memory of a kernel, set once per device (a driver call of a microsecond); `ready` belongs to the kernel.
+template <typename F>
+inline cudaError_t allow_shared(std::atomic<uint64_t>& ready, F kernel, int bytes) {
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  if (dev < 64 && (ready.load(std::memory_order_acquire) >> dev & 1)) return cudaSuccess;
+  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_release);
+  return cudaSuccess;
 }
 
 size_t decode_workspace_bytes(int B, int Hq, int Hkv, int D, int N, int window, int sinks, bool with_mass);

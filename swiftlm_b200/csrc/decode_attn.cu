@@ -593,7 +593,8 @@ int32_t launch_typed(const CacheArgs& a, const Plan& t, cudaStream_t stream) {
   p.scores = a.mass ? reinterpret_cast<float*>(ws + t.part + t.info) : nullptr;
   p.lse2 = a.mass ? reinterpret_cast<float*>(ws + t.part + t.info + t.scores) : nullptr;
   auto kernel = decode_kernel<T, D, NT>;
-  DFLASH_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::fixed + kMaxBatch * 8));
+  static std::atomic<uint64_t> ready{0};
+  DFLASH_CUDA_CHECK(allow_shared(ready, kernel, L::fixed + kMaxBatch * 8));
   for (int b0 = 0; b0 < a.B; b0 += kMaxBatch) {
     p.b0 = b0;
     p.nb = a.B - b0 < kMaxBatch ? a.B - b0 : kMaxBatch;

@@ -573,6 +573,14 @@ template <typename T, int D>
 __global__ void __launch_bounds__(128) join_kernel(const PromptParams p) {
   constexpr int R = 256;
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (p.a.lse && p.a.q_len) {                  // rows behind a sequence's last query
+    const long long rows = (long long)p.a.B * p.a.Hq * p.a.T, threads = (long long)gridDim.x * gridDim.y * gridDim.z * 128;
+    const long long block = ((long long)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+    for (long long i = block * 128 + threadIdx.x; i < rows; i += threads) {
+      const long long bh = i / p.a.T;
+      if ((int)(i - bh * p.a.T) >= lens_of(p.a, (int)(bh / p.a.Hq)).rows) p.a.lse[i] = -INFINITY;
+    }
+  }
   const Cut cut = p.ranges.cuts[blockIdx.x];
   if (cut.count == 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -655,7 +663,8 @@ int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
   if (r == CUDA_SUCCESS) r = encode_kv(&mv, a.v, a, p.box);
   if (r != CUDA_SUCCESS) { set_error("prompt_sdpa: cuTensorMapEncodeTiled failed with CUresult %d", (int)r); return DFLASH_ERR_CUDA; }
   auto kernel = prompt_kernel<T, D>;
-  DFLASH_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::total));
+  static std::atomic<uint64_t> ready{0};
+  DFLASH_CUDA_CHECK(allow_shared(ready, kernel, C::total));
   // the register hand-over waits for good if the launch gives the CTA fewer than it takes
   static const int regs = [&] { cudaFuncAttributes f; return cudaFuncGetAttributes(&f, kernel) == cudaSuccess ? f.numRegs : 0; }();
   if (regs != C::regs_launch) { set_error("prompt_sdpa: the kernel is launched with %d registers a thread, %d expected", regs, C::regs_launch); return DFLASH_ERR_CUDA; }

@@ -11,8 +11,8 @@ from __future__ import annotations
 
 from typing import Optional, Tuple
 
-import contextlib
 import ctypes as C
+import functools
 
 import torch
 
@@ -275,17 +275,33 @@ def _bad(what: str):
     return _lib.DFlashError(_lib.ERR_INVALID_ARG, what)
 
 
-def _on_device_of(t: torch.Tensor):
-    """The tensor's device made current for a call (allocation, stream and launch all go to it)."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+# The calls below are made once a token: what they check and allocate is kept to a few microseconds.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
-def _same_device(first: torch.Tensor, *others):
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(name: str, device_index: int, *sizes) -> int:
+    with torch.cuda.device(device_index):
+        return getattr(_lib.lib(), name)(*sizes)
+
+
+def _on_its_device(fn):
+    """Runs fn(t, ...) with t's device current: allocation, stream and launch all go to it."""
+    @functools.wraps(fn)
+    def call(t, *args, **kwargs):
+        if not t.is_cuda:
+            _need_cuda(t)
+        if t.device.index == torch.cuda.current_device():
+            return fn(t, *args, **kwargs)
+        with torch.cuda.device(t.device):
+            return fn(t, *args, **kwargs)
+    return call
+
+
+def _same_device(device, *others):
     for t in others:
-        if t is not None and t.device != first.device:
-            raise _bad(f"tensors on different devices: {first.device} and {t.device}")
+        if t is not None and t.device != device:
+            raise _bad(f"tensors on different devices: {device} and {t.device}")
 
 
 def _int_vector(x, n: int, device, name: str):
@@ -293,7 +309,7 @@ def _int_vector(x, n: int, device, name: str):
         return None
     if not (isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.device == device and x.is_contiguous()):
         x = torch.as_tensor(x, device=device).to(torch.int32).contiguous()
-    if x.shape != (n,):
+    if x.dim() != 1 or x.shape[0] != n:
         raise _bad(f"{name} must have one entry per sequence")
     return x
 
@@ -309,21 +325,26 @@ def _cache_shape(keys, page_table, n_max, B: int):
         raise _bad("page_table must be [B, max_pages]")
     if page_table.dtype != torch.int32 or not page_table.is_contiguous():
         page_table = page_table.to(torch.int32).contiguous()
-    capacity = page_table.shape[1] * keys.shape[2]
-    return page_table, (capacity if n_max is None else min(int(n_max), capacity)), keys.shape[2], page_table.shape[1], keys.shape[0]
+    num_pages, _, page_tokens, _ = keys.shape
+    max_pages = page_table.shape[1]
+    capacity = max_pages * page_tokens
+    return page_table, (capacity if n_max is None else min(int(n_max), capacity)), page_tokens, max_pages, num_pages
 
 
-def _cache_tensors(queries, keys, values):
-    _need_cuda(queries, keys, values)
-    _same_device(queries, keys, values)
-    if keys.dim() != 4 or (values is not None and values.shape != keys.shape):
-        raise _bad("keys and values must be two 4-dimensional tensors of one shape")
-    if queries.shape[-1] != keys.shape[3]:
-        raise _bad("queries and keys have different head dimensions")
-    if keys.dtype != queries.dtype or (values is not None and values.dtype != queries.dtype):
+def _cache_tensors(queries, dims: int, keys, values, *others):
+    """What the three attention calls refuse alike."""
+    if queries.dim() != dims:
+        raise _bad("queries must be " + ("[B, Hq, D]" if dims == 3 else "[B, Hq, T, D]"))
+    if keys.dim() != 4 or queries.shape[-1] != keys.shape[3]:
+        raise _bad("keys must be 4-dimensional, with the queries' head dimension")
+    dt = queries.dtype
+    if dt is not torch.bfloat16 and dt is not torch.float16:
+        raise _lib.DFlashUnsupported(_lib.ERR_UNSUPPORTED, f"dtype {dt} (bf16 or f16)")
+    if keys.dtype is not dt or (values is not None and values.dtype is not dt):
         raise _lib.DFlashUnsupported(_lib.ERR_UNSUPPORTED, "queries, keys and values must have one dtype")
-    if queries.dtype not in (torch.bfloat16, torch.float16):
-        raise _lib.DFlashUnsupported(_lib.ERR_UNSUPPORTED, f"dtype {queries.dtype} (bf16 or f16)")
+    if values is not None and values.shape != keys.shape:
+        raise _bad("keys and values must have one shape")
+    _same_device(queries.device, keys, values, *others)
 
 
 def _mass_arg(mass, B: int, Hkv: int, N: int, name: str = "mass"):
@@ -346,6 +367,7 @@ def _scratch(nbytes: int, device) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
+@_on_its_device
 def decode_sdpa(queries, keys, values, scale: float, kv_len=None, page_table=None, window: int = 0, sinks: int = 0,
                 mass: Optional[torch.Tensor] = None, return_lse: bool = False, out=None, n_max=None):
     """Attention of one new token per sequence over its cache, the new token being the last cached one.
@@ -357,29 +379,26 @@ def decode_sdpa(queries, keys, values, scale: float, kv_len=None, page_table=Non
     it.  n_max: an upper bound of kv_len for a page pool, when less than the table's reach is in use.
     Returns [B,Hq,D], or (that, lse fp32 [B,Hq]) with return_lse.
     """
-    _cache_tensors(queries, keys, values)
-    if queries.dim() != 3:
-        raise _bad("queries must be [B, Hq, D]")
+    _cache_tensors(queries, 3, keys, values, page_table, mass, out)
     B, Hq, D = queries.shape
-    Hkv = keys.shape[1]
-    _same_device(queries, page_table, mass, out)
+    Hkv, device = keys.shape[1], queries.device
     page_table, N, page_tokens, max_pages, num_pages = _cache_shape(keys, page_table, n_max, B)
+    stride = 0
     if mass is not None:
-        _mass_arg(mass, B, Hkv, N)
-    with _on_device_of(queries):
-        q, k, v = queries.contiguous(), keys.contiguous(), values.contiguous()
-        kv_len = _int_vector(kv_len, B, q.device, "kv_len")
-        out = _out_arg(out, q)
-        lse = torch.empty((B, Hq), dtype=torch.float32, device=q.device) if return_lse else None
-        L = _lib.lib()
-        ws = _scratch(L.dflash_decode_sdpa_workspace_bytes(B, Hq, Hkv, D, N, int(window), int(sinks), int(mass is not None)), q.device)
-        _lib.check(L.dflash_decode_sdpa(
-            _ptr(q), _ptr(k), _ptr(v), _ptr(page_table), _ptr(kv_len), _ptr(out), _ptr(lse), _ptr(mass), _ptr(ws),
-            0 if ws is None else ws.numel(), B, Hq, Hkv, D, N, page_tokens, max_pages, num_pages,
-            0 if mass is None else mass.shape[2], int(window), int(sinks), float(scale), _DT[q.dtype], _stream()))
+        stride = _mass_arg(mass, B, Hkv, N).shape[2]
+    q, k, v = queries.contiguous(), keys.contiguous(), values.contiguous()
+    kv_len = _int_vector(kv_len, B, device, "kv_len")
+    out = _out_arg(out, q)
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=device) if return_lse else None
+    need = _workspace_bytes("dflash_decode_sdpa_workspace_bytes", device.index, B, Hq, Hkv, D, N, window, sinks, int(mass is not None))
+    ws = _scratch(need, device)
+    _lib.check(_lib.lib().dflash_decode_sdpa(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(page_table), _ptr(kv_len), out.data_ptr(), _ptr(lse), _ptr(mass), _ptr(ws), need,
+        B, Hq, Hkv, D, N, page_tokens, max_pages, num_pages, stride, window, sinks, scale, _DT[q.dtype], _raw_stream(device.index)))
     return (out, lse) if return_lse else out
 
 
+@_on_its_device
 def prompt_sdpa(queries, keys, values, scale: float, q_len=None, kv_len=None, page_table=None, window: int = 0, sinks: int = 0,
                 return_lse: bool = False, out=None, n_max=None):
     """Attention of a prompt, or of a chunk of one behind what the cache holds already, with the chunk's own rows in the
@@ -390,56 +409,46 @@ def prompt_sdpa(queries, keys, values, scale: float, q_len=None, kv_len=None, pa
     own, within the window or among the sinks.  Rows at and behind q_len[b] are left as they are in `out`.
     Returns [B,Hq,T,D], or (that, lse fp32 [B,Hq,T]) with return_lse (-inf on rows that see nothing or are not in use).
     """
-    _cache_tensors(queries, keys, values)
-    if queries.dim() != 4:
-        raise _bad("queries must be [B, Hq, T, D]")
+    _cache_tensors(queries, 4, keys, values, page_table, out)
     B, Hq, T, D = queries.shape
-    Hkv = keys.shape[1]
-    _same_device(queries, page_table, out)
+    Hkv, device = keys.shape[1], queries.device
     page_table, N, page_tokens, max_pages, num_pages = _cache_shape(keys, page_table, n_max, B)
-    with _on_device_of(queries):
-        q, k, v = queries.contiguous(), keys.contiguous(), values.contiguous()
-        kv_len, q_len = _int_vector(kv_len, B, q.device, "kv_len"), _int_vector(q_len, B, q.device, "q_len")
-        out = _out_arg(out, q)
-        lse = None
-        if return_lse:
-            lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device) if q_len is None else \
-                torch.full((B, Hq, T), float("-inf"), dtype=torch.float32, device=q.device)
-        L = _lib.lib()
-        ws = _scratch(L.dflash_prompt_sdpa_workspace_bytes(B, Hq, Hkv, T, D, N), q.device)
-        _lib.check(L.dflash_prompt_sdpa(
-            _ptr(q), _ptr(k), _ptr(v), _ptr(page_table), _ptr(q_len), _ptr(kv_len), _ptr(out), _ptr(lse), _ptr(ws),
-            0 if ws is None else ws.numel(), B, Hq, Hkv, T, D, N, page_tokens, max_pages, num_pages, int(window), int(sinks),
-            float(scale), _DT[q.dtype], _stream()))
+    q, k, v = queries.contiguous(), keys.contiguous(), values.contiguous()
+    kv_len, q_len = _int_vector(kv_len, B, device, "kv_len"), _int_vector(q_len, B, device, "q_len")
+    out = _out_arg(out, q)
+    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=device) if return_lse else None
+    need = _workspace_bytes("dflash_prompt_sdpa_workspace_bytes", device.index, B, Hq, Hkv, T, D, N)
+    ws = _scratch(need, device)
+    _lib.check(_lib.lib().dflash_prompt_sdpa(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(page_table), _ptr(q_len), _ptr(kv_len), out.data_ptr(), _ptr(lse), _ptr(ws), need,
+        B, Hq, Hkv, T, D, N, page_tokens, max_pages, num_pages, window, sinks, scale, _DT[q.dtype], _raw_stream(device.index)))
     return (out, lse) if return_lse else out
 
 
+@_on_its_device
 def attention_mass(queries, keys, lse, scale: float, mass, q_len=None, kv_len=None, page_table=None, window: int = 0,
                    sinks: int = 0, n_max=None) -> None:
     """Adds to mass fp32 [B,Hkv,>= capacity] the weight that the queries [B,Hq,T,D] give to every cached token, summed over
     rows and the query heads of a KV head: exp(scale * q.k - lse) with the lse [B,Hq,T] of prompt_sdpa over the same cache
     (all of a chunk's rows, or its last ones: the rows given are the last T, or q_len, tokens of the cache)."""
-    _cache_tensors(queries, keys, None)
-    if queries.dim() != 4:
-        raise _bad("queries must be [B, Hq, T, D]")
+    _cache_tensors(queries, 4, keys, None, page_table, lse, mass)
     B, Hq, T, D = queries.shape
-    Hkv = keys.shape[1]
+    Hkv, device = keys.shape[1], queries.device
     if lse.dtype != torch.float32 or lse.shape != (B, Hq, T):
         raise _bad("lse must be fp32 [B, Hq, T]")
-    _same_device(queries, page_table, lse, mass)
     page_table, N, page_tokens, max_pages, num_pages = _cache_shape(keys, page_table, n_max, B)
     _mass_arg(mass, B, Hkv, N)
-    with _on_device_of(queries):
-        q, k, lse = queries.contiguous(), keys.contiguous(), lse.contiguous()
-        kv_len, q_len = _int_vector(kv_len, B, q.device, "kv_len"), _int_vector(q_len, B, q.device, "q_len")
-        L = _lib.lib()
-        ws = _scratch(L.dflash_attention_mass_workspace_bytes(B, Hq, Hkv, T, D, N), q.device)
-        _lib.check(L.dflash_attention_mass(
-            _ptr(q), _ptr(k), _ptr(page_table), _ptr(q_len), _ptr(kv_len), _ptr(lse), _ptr(mass), _ptr(ws),
-            0 if ws is None else ws.numel(), B, Hq, Hkv, T, D, N, page_tokens, max_pages, num_pages, mass.shape[2], int(window),
-            int(sinks), float(scale), _DT[q.dtype], _stream()))
+    q, k, lse = queries.contiguous(), keys.contiguous(), lse.contiguous()
+    kv_len, q_len = _int_vector(kv_len, B, device, "kv_len"), _int_vector(q_len, B, device, "q_len")
+    need = _workspace_bytes("dflash_attention_mass_workspace_bytes", device.index, B, Hq, Hkv, T, D, N)
+    ws = _scratch(need, device)
+    _lib.check(_lib.lib().dflash_attention_mass(
+        q.data_ptr(), k.data_ptr(), _ptr(page_table), _ptr(q_len), _ptr(kv_len), lse.data_ptr(), mass.data_ptr(), _ptr(ws), need,
+        B, Hq, Hkv, T, D, N, page_tokens, max_pages, num_pages, mass.shape[2], window, sinks, scale, _DT[q.dtype],
+        _raw_stream(device.index)))
 
 
+@_on_its_device
 def kv_evict(k_cache, v_cache, mass, kv_len, budget: int, recent: int, sinks: int = 0, page_table=None, kv_len_out=None,
              mass_out=None, kept=None, n_max=None) -> torch.Tensor:
     """Cuts every sequence longer than `budget` tokens down to it, per KV head and in place: the first `sinks` tokens, the
@@ -451,8 +460,9 @@ def kv_evict(k_cache, v_cache, mass, kv_len, budget: int, recent: int, sinks: in
     old length; kept int32 [B,Hkv,budget], if given, their old places (-1 behind the last).  Returns kv_len_out
     (default: kv_len itself, updated): min(kv_len, budget).
     """
-    _need_cuda(k_cache, v_cache, mass, kv_len)
-    _same_device(k_cache, v_cache, mass, kv_len, page_table, kv_len_out, mass_out, kept)
+    _need_cuda(mass, kv_len)
+    device = k_cache.device
+    _same_device(device, v_cache, mass, kv_len, page_table, kv_len_out, mass_out, kept)
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
         raise _bad("k_cache and v_cache must be two 4-dimensional tensors of one shape and dtype")
     if k_cache.dtype not in (torch.bfloat16, torch.float16, torch.float32):
@@ -473,13 +483,12 @@ def kv_evict(k_cache, v_cache, mass, kv_len, budget: int, recent: int, sinks: in
         raise _bad("mass_out must have the shape of mass")
     if kept is not None and (kept.dtype != torch.int32 or kept.shape != (B, Hkv, budget) or not kept.is_contiguous()):
         raise _bad("kept must be a contiguous int32 tensor [B, Hkv, budget]")
-    with _on_device_of(k_cache):
-        L = _lib.lib()
-        ws = _scratch(L.dflash_kv_evict_workspace_bytes(B, Hkv, N, budget), k_cache.device)
-        _lib.check(L.dflash_kv_evict(
-            _ptr(k_cache), _ptr(v_cache), _ptr(page_table), _ptr(kv_len), _ptr(mass), _ptr(kv_len_out), _ptr(mass_out), _ptr(kept),
-            _ptr(ws), 0 if ws is None else ws.numel(), B, Hkv, D, N, page_tokens, max_pages, num_pages, mass.shape[2], budget,
-            int(recent), int(sinks), _DT[k_cache.dtype], _stream()))
+    need = _workspace_bytes("dflash_kv_evict_workspace_bytes", device.index, B, Hkv, N, budget)
+    ws = _scratch(need, device)
+    _lib.check(_lib.lib().dflash_kv_evict(
+        k_cache.data_ptr(), v_cache.data_ptr(), _ptr(page_table), kv_len.data_ptr(), mass.data_ptr(), kv_len_out.data_ptr(),
+        mass_out.data_ptr(), _ptr(kept), _ptr(ws), need, B, Hkv, D, N, page_tokens, max_pages, num_pages, mass.shape[2], budget,
+        int(recent), int(sinks), _DT[k_cache.dtype], _raw_stream(device.index)))
     return kv_len_out
 
 
