@@ -32,10 +32,13 @@ struct EvictParams {
   int B, Hkv, N, page_tokens, max_pages, num_pages, mass_stride, budget, recent, sinks, stride;
   int row_bytes;
   int* status;
+  uint32_t page_mul, page_shift;
+  // n / page_tokens for 0 <= n < 2^31: multiplication by a rounded-up 2^32+shift / page_tokens
+  __device__ int by_page(int n) const { return (int)((__umulhi((uint32_t)n, page_mul) + (uint32_t)n) >> page_shift); }
 };
 
 constexpr int kMaxCluster = 8;
-constexpr int kSelThreads = 1024, kPer = 4, kChunk = kSelThreads * kPer;   // tokens of one CTA at a time
+constexpr int kSelThreads = 512, kPer = 8, kChunk = kSelThreads * kPer;   // tokens of one CTA at a time
 
 // unsigned order of the key = order of the float; -0 and +0 are equal, every NaN is above +inf
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -55,7 +58,7 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t mine, uint32_t& total,
   }
   if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
-  uint32_t w = warp_sums[lane];
+  uint32_t w = lane < kSelThreads / 32 ? warp_sums[lane] : 0u;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const uint32_t y = __shfl_up_sync(0xffffffffu, w, o);
@@ -76,18 +79,7 @@ __device__ __forceinline__ uint32_t peer_load(const uint32_t* mine, uint32_t ran
   return x;
 }
 
-// byte offset of token n's row of (b, h); -1: its page is outside the pool
-__device__ __forceinline__ long long row_at(const EvictParams& p, int b, int h, int n) {
-  if (!p.page_table) return (((long long)b * p.Hkv + h) * p.N + n) * p.row_bytes;
-  const int page = p.page_table[(long long)b * p.max_pages + n / p.page_tokens];
-  if ((unsigned)page >= (unsigned)p.num_pages) {
-    atomicExch(p.status, kStatusKvRange);
-    return -1;
-  }
-  return (((long long)page * p.Hkv + h) * p.page_tokens + n % p.page_tokens) * p.row_bytes;
-}
-
-__global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p, int C) {
+__global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParams p, int C) {
   __shared__ uint32_t hist[2048], hist_all[2048];          // this CTA's counts, the cluster's
   __shared__ uint32_t warp_sums[32];
   __shared__ uint32_t s_digit, s_left, s_count, s_counts[kMaxCluster], s_first;
@@ -131,7 +123,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048, per = bins / kSelThreads;
-#pragma unroll 4
+#pragma unroll 8
       for (int i = lo + all; i < hi; i += stride) {
         const uint32_t key = order_key(mass[i]);
         if ((key & mask) == threshold) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
@@ -147,14 +139,18 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p
         }
       }
       meet();
-      // from the top: the digit in which the running count reaches `need`; thread 0 has the highest of 2 or 1 bins a thread
+      // from the top: the digit in which the running count reaches `need`; thread 0 has the highest of 4 or 2 bins a thread
       uint32_t* sums = C > 1 ? hist_all : hist;
       const int top = bins - 1 - tid * per;
-      const uint32_t c0 = sums[top], c1 = per == 2 ? sums[top - 1] : 0u;
-      uint32_t total;
-      const uint32_t before = block_prefix(c0 + c1, total, warp_sums);
-      if (before < need && need <= before + c0) { s_digit = top; s_left = need - before; }
-      else if (before + c0 < need && need <= before + c0 + c1) { s_digit = top - 1; s_left = need - before - c0; }
+      uint32_t c[4], total;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c[j] = j < per ? sums[top - j] : 0u;
+      uint32_t before = block_prefix(c[0] + c[1] + c[2] + c[3], total, warp_sums);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (before < need && need <= before + c[j]) { s_digit = top - j; s_left = need - before; }
+        before += c[j];
+      }
       for (int i = tid; i < 2048; i += kSelThreads) hist[i] = hist_all[i] = 0;     // all threads have read theirs
       meet();
       threshold |= s_digit << shift;
@@ -198,23 +194,46 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p
       eq_done += c >> 16;
     }
     uint32_t first = 0xffffffffu;
+    int slot[kPer];
+    int page_from[kPer], page_to[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const bool e = (eq >> j) & 1u, on = ((sure >> j) & 1u) || (e && eq_at < equals);
-      if (on) {
-        const uint32_t slot = sure_at + (eq_at < equals ? eq_at : equals);
-        if (kept) kept[slot] = i0 + j;
-        mass_out[slot] = w[j];                            // slot <= token, and this round has been read
-        longlong2 at2 = make_longlong2(-1, -1);           // looked up here once a row, not by every thread that moves a part of it
-        if (slot != (uint32_t)(i0 + j)) {
-          at2 = make_longlong2(row_at(p, b, unit - b * p.Hkv, i0 + j), row_at(p, b, unit - b * p.Hkv, (int)slot));
-          if (at2.y < 0) at2.x = -1;
-        }
-        places[slot] = at2;
-        if (slot != (uint32_t)(i0 + j) && slot < first) first = slot;
-      }
+      slot[j] = on ? (int)(sure_at + (eq_at < equals ? eq_at : equals)) : -1;
+      if (on && slot[j] != i0 + j && (uint32_t)slot[j] < first) first = (uint32_t)slot[j];
       sure_at += (sure >> j) & 1u;
       eq_at += e;
+    }
+    // Addresses are looked up here, once a row, and not by every thread that moves a part of it.
+    const int h = unit - b * p.Hkv;
+    if (p.page_table) {
+      const int32_t* table = p.page_table + (long long)b * p.max_pages;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j)
+        if (slot[j] >= 0) {
+          page_from[j] = table[p.by_page(i0 + j)];
+          page_to[j] = table[p.by_page(slot[j])];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      if (slot[j] < 0) continue;
+      if (kept) kept[slot[j]] = i0 + j;
+      mass_out[slot[j]] = w[j];                           // slot <= token, and this round has been read
+      longlong2 at2 = make_longlong2(-1, -1);
+      if (slot[j] != i0 + j) {
+        if (!p.page_table) {
+          const long long base = ((long long)b * p.Hkv + h) * p.N;
+          at2 = make_longlong2((base + i0 + j) * p.row_bytes, (base + slot[j]) * p.row_bytes);
+        } else if ((unsigned)page_from[j] >= (unsigned)p.num_pages || (unsigned)page_to[j] >= (unsigned)p.num_pages) {
+          atomicExch(p.status, kStatusKvRange);           // a page outside the pool: the row is skipped
+        } else {
+          const int rf = i0 + j - p.by_page(i0 + j) * p.page_tokens, rt = slot[j] - p.by_page(slot[j]) * p.page_tokens;
+          at2 = make_longlong2((((long long)page_from[j] * p.Hkv + h) * p.page_tokens + rf) * p.row_bytes,
+                               (((long long)page_to[j] * p.Hkv + h) * p.page_tokens + rt) * p.row_bytes);
+        }
+      }
+      places[slot[j]] = at2;
     }
     first = __reduce_min_sync(0xffffffffu, first);
     if ((tid & 31) == 0 && first < s_first) atomicMin(&s_first, first);
@@ -323,7 +342,11 @@ extern "C" int32_t dflash_kv_evict(void* k_cache, void* v_cache, const int32_t* 
   EvictParams p{reinterpret_cast<uint8_t*>(k_cache), reinterpret_cast<uint8_t*>(v_cache), page_table, kv_len, mass, kv_len_out, mass_out,
                 kept, reinterpret_cast<int2*>(workspace),
                 reinterpret_cast<longlong2*>(reinterpret_cast<uint8_t*>(workspace) + moves_bytes(B, Hkv)), B, Hkv, N, page_tokens, max_pages, num_pages, mass_stride, budget, recent, sinks,
-                budget < N ? budget : N, (int)row_bytes, status};
+                budget < N ? budget : N, (int)row_bytes, status, 0, 0};
+  if (page_table) {
+    while ((1ull << p.page_shift) < (uint64_t)page_tokens) ++p.page_shift;
+    p.page_mul = (uint32_t)(((1ull << 32) * ((1ull << p.page_shift) - (uint64_t)page_tokens)) / (uint64_t)page_tokens + 1);
+  }
   int C = 1;
   while (C < kMaxCluster && N > C * kChunk) C *= 2;
   cudaLaunchConfig_t cfg = {};
