@@ -2,16 +2,17 @@
 //     mass[b, h, n] += sum over the rows r of h's query heads that see n of 2^(scale log2(e) q_r . k_n - log2(e) lse_r)
 //
 // Computed as S^T = K Q^T on the tensor cores (tcgen05): 128 keys are the lanes of tensor memory and 128 query rows its
-// columns, so that the sum over rows stays inside a thread and nothing is reduced across lanes; two or four threads share a key.
-// A unit of work is one key tile, its steps are the query tiles that see it.  Few rows (a verify block, the last rows of a
-// prompt: one query tile): every key is read once and used by 128 rows, bound by HBM; the query tile stays in shared
-// memory.  Many rows: 2 D operations and one exponential a pair of row and key, bound by the 16 exponentials a clock of
-// an SM (1024 clocks a tile against 512 of products at D = 128), the key tile stays and query tiles stream.
+// columns, so that the sum over rows stays inside a thread and nothing is reduced across lanes; two threads share a key.
+// A unit of work is 256 keys (two key tiles), its steps are the query tiles that see some of them.  Few rows (a verify
+// block, the last rows of a prompt: one query tile): every key is read once and used by 128 rows, bound by HBM; the query
+// tile stays in shared memory and keys stream.  Many rows: 2 D operations and one exponential a pair of row and key, bound by
+// the 16 exponentials a clock of an SM (1024 clocks a tile against 512 of products at D = 128); the keys stay and query
+// tiles stream, each used for both key tiles: with one key tile they took 32 KiB from L2 every 1000 clocks, and L2 set the pace.
 //
-// Warps: 0 loads key and query tiles (whichever changed), 1 the rows' -log2(e) lse, 2 issues the products, 3 walks the
-// steps, 4-19 sum.  Four
-// score buffers in tensor memory let the products run ahead.  Units are cut into equal ranges per CTA (ranges.cuh);
-// pieces of a cut unit leave 128 sums in the workspace, added in order by join_kernel: the order of every sum is fixed.
+// Warps: 0 loads keys and queries, 1 the rows' -log2(e) lse, 2 issues the products, 3 walks the steps, 4-11
+// sum the first key tile, 12-19 the second.  Four score buffers in tensor memory let the products run a step ahead.  Units
+// are cut into equal ranges per CTA (ranges.cuh); pieces of a cut unit leave 256 sums in the workspace, added in order by
+// mass_join_kernel: the order of every sum is fixed.
 #include "ranges.cuh"
 #include "tc_common.cuh"
 
@@ -23,77 +24,82 @@ using namespace tc;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kUnitCost = 1;                 // what a unit costs besides its query tiles
 constexpr int kSumWarps = 16, kThreads = 128 + kSumWarps * 32;
-constexpr int kBuffers = 4;
+constexpr int kUnitKeys = 2 * kKeys;
+constexpr int kBuffers = 4;                  // steps whose log-sum-exps are in shared memory; score buffers of two steps
 constexpr int kRing = 16;                    // steps that are described ahead
 
 struct MassParams {
   CacheArgs a;
   Tiling t;
   Ranges ranges;               // rows of key tiles
-  int box, k_stages, q_stages; // tiles of keys and of queries in shared memory
+  int box, k_stages, q_stages; // stages of keys and of queries in shared memory
   float scale_log2;
-  float* part;                 // [2 * grid][128]
+  float* part;                 // [2 * grid][256]
 };
 
 // One step: a key tile against a query tile.
-enum : int { kNewKeys = 1, kNewQueries = 2, kLast = 4, kSingle = 8, kEnd = 16 };   // the first step of a unit; another query tile than
-struct __align__(16) Step {                                                        // before; the last step; the only one; no step
+// the first step of a unit; another query tile than before; the last step of the unit; of the query tile; one key tile; no step
+enum : int { kNewKeys = 1, kNewQueries = 2, kLast = 4, kQueriesLast = 8, kOneTile = 16, kEnd = 32 };
+struct __align__(16) Step {
   int b, h, n0, gc;
   int t0, keys, rows, flags;   // t0: first token of the query tile; the sequence's lengths
   int slot, pad[3];            // of the unit (see RangeWalker::take)
 };
 
 template <int D> struct Cfg {
-  static constexpr int NC = D / 64, tile = NC * kChunk;
-  static constexpr int tiles = D == 256 ? 3 : 6;            // tiles of keys and queries together
-  static constexpr int bars = tiles * tile;
-  static constexpr int b_k_full = 0, b_k_empty = tiles, b_q_full = 2 * tiles, b_q_empty = 3 * tiles, b_s_full = 4 * tiles,
-                       b_s_free = b_s_full + kBuffers, b_z_full = b_s_free + kBuffers, b_step = b_z_full + kBuffers, n_bars = b_step + kRing;
+  static constexpr int NC = D / 64;
+  // Stages of two chunks (one at D = 64), of keys and queries together: a wait and an issue for every 8 products.  (For
+  // every 4 the issuing warp was the slowest part: 470 us for 411.)
+  static constexpr int SC = NC < 2 ? NC : 2, NS = NC / SC, stages = 12 / SC, stage = SC * kChunk;
+  static constexpr int bars = stages * stage;
+  static constexpr int b_full = 0, b_empty = stages, b_s_full = 2 * stages, b_s_free = b_s_full + 4, b_z_full = b_s_free + 4,
+                       b_z_free = b_z_full + kBuffers, b_step = b_z_free + kBuffers, n_bars = b_step + kRing;
   static constexpr int misc = bars + (8 * n_bars + 15) / 16 * 16;
   static constexpr int z = misc + 16;                       // [kBuffers][128] -log2(e) lse of the rows
-  static constexpr int sums = z + kBuffers * 128 * 4;       // [2][4][128] of a key's four threads, [2 groups][2][2][128] of two
-  static constexpr int steps = sums + 2 * (2 * 4 * 128 * 4);   // [kRing] Step
+  static constexpr int sums = z + kBuffers * 128 * 4;       // [2 key tiles][2][2 halves][128]
+  static constexpr int steps = sums + 2 * 2 * 2 * 128 * 4;  // [kRing] Step
   static constexpr int total = steps + kRing * (int)sizeof(Step);
 };
 static_assert(Cfg<256>::total <= 232448 && Cfg<128>::total <= 232448 && Cfg<64>::total <= 232448, "shared memory");
 
-// Place in a ring of a length known at run time: stage and phase by counting, not by division.
+// Place in a ring of a length known at run time: stage and round by counting, not by division.
 struct RingAt {
   int stage = 0;
   uint32_t round = 0;
-  __device__ void next(int stages) {
-    if (++stage == stages) { stage = 0; ++round; }
+  __device__ void next(int stages, int by = 1) {
+    stage += by;
+    if (stage >= stages) { stage -= stages; ++round; }
   }
 };
 
-// query tokens of sequence (len) that see some key of [n0, n0 + 128): first and last; last < first: none
+// query tokens of sequence (len) that see some key of [n0, n0 + 256): first and last; last < first: none
 struct Seeing { int first, last; };
 __device__ __forceinline__ Seeing seeing(const CacheArgs& a, RowLens len, int n0) {
-  const int past = len.keys - len.rows, n1 = (n0 + kKeys < len.keys ? n0 + kKeys : len.keys) - 1;
+  const int past = len.keys - len.rows, n1 = (n0 + kUnitKeys < len.keys ? n0 + kUnitKeys : len.keys) - 1;
   Seeing s{n0 > past ? n0 - past : 0, len.rows - 1};
   if (a.window > 0 && n0 >= a.sinks && n1 + a.window - 1 - past < s.last) s.last = n1 + a.window - 1 - past;
   if (n1 < n0) s.last = -1;
   return s;
 }
-// query tiles (times head groups) of a key tile
-__device__ __forceinline__ int tile_steps(const CacheArgs& a, const Tiling& t, RowLens len, int u) {
-  const Seeing s = seeing(a, len, u * kKeys);
+// query tiles (times head groups) of a unit
+__device__ __forceinline__ int unit_steps(const CacheArgs& a, const Tiling& t, RowLens len, int u) {
+  const Seeing s = seeing(a, len, u * kUnitKeys);
   return s.last < s.first ? 0 : t.GC * (s.last / t.Tt - s.first / t.Tt + 1);
 }
-// first key tile at or behind u that is seen
-__device__ __forceinline__ int next_tile(const CacheArgs& a, RowLens len, int u, int per_row) {
-  const int tiles = (len.keys + kKeys - 1) / kKeys;
+// first unit at or behind u that is seen
+__device__ __forceinline__ int next_unit(const CacheArgs& a, RowLens len, int u, int per_row) {
+  const int tiles = (len.keys + kUnitKeys - 1) / kUnitKeys;
   if (len.rows == 0 || u >= tiles) return per_row;
   const int past = len.keys - len.rows;
-  const int lo = a.window > 0 && past - a.window + 1 > 0 ? (past - a.window + 1) / kKeys : 0;      // of the first row's window
-  const int sinks = a.window > 0 ? (a.sinks + kKeys - 1) / kKeys : 0;
+  const int lo = a.window > 0 && past - a.window + 1 > 0 ? (past - a.window + 1) / kUnitKeys : 0;   // of the first row's window
+  const int sinks = a.window > 0 ? (a.sinks + kUnitKeys - 1) / kUnitKeys : 0;
   if (u >= sinks && u < lo) u = lo;
   return u < tiles ? u : per_row;
 }
 
 __global__ void __launch_bounds__(1024) mass_plan_kernel(const MassParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  plan_ranges<kUnitCost>(p.ranges, p.a, [&](RowLens len, int u) { return tile_steps(p.a, p.t, len, u); });
+  plan_ranges<kUnitCost>(p.ranges, p.a, [&](RowLens len, int u) { return unit_steps(p.a, p.t, len, u); });
 }
 
 struct Steps {
@@ -108,25 +114,25 @@ struct Steps {
     int flags = ++i >= hi || !any ? kNewKeys : 0;
     if (flags) {
       if (!w.find([&](RowLens len, int u) {
-            u = next_tile(p.a, len, u, p.ranges.per_row);
-            while (u < p.ranges.per_row && tile_steps(p.a, p.t, len, u) == 0) u = next_tile(p.a, len, u + 1, p.ranges.per_row);
+            u = next_unit(p.a, len, u, p.ranges.per_row);
+            while (u < p.ranges.per_row && unit_steps(p.a, p.t, len, u) == 0) u = next_unit(p.a, len, u + 1, p.ranges.per_row);
             return u;
           }, i)) return false;
       s.b = w.c.b;
       s.h = w.c.hg;
       s.keys = w.c.len.keys;
       s.rows = w.c.len.rows;
-      s.n0 = w.c.u * kKeys;
+      s.n0 = w.c.u * kUnitKeys;
       const Seeing x = seeing(p.a, w.c.len, s.n0);
       tt0 = x.first / p.t.Tt;
       per_gc = x.last / p.t.Tt - tt0 + 1;
       hi = w.take(i, p.t.GC * per_gc, s.slot);
-      if (hi - i == 1) flags |= kSingle;
     }
     s.gc = p.t.GC == 1 ? 0 : i / per_gc;
     s.t0 = (tt0 + i - s.gc * per_gc) * p.t.Tt;
     if (!any || b != s.b || h != s.h || gc != s.gc || t0 != s.t0) flags |= kNewQueries;
     if (i == hi - 1) flags |= kLast;
+    if (s.n0 + kKeys >= s.keys) flags |= kOneTile;
     s.flags = flags;
     any = true;
     return true;
@@ -141,7 +147,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const MassParams p) {
   using C = Cfg<D>;
-  constexpr int NC = C::NC;
+  constexpr int NS = C::NS, SC = C::SC;
   extern __shared__ __align__(1024) uint8_t sm[];
   const CacheArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -152,15 +158,16 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
   if (threadIdx.x == 0) {
     ptx::prefetch_tensormap(&map_q);
     ptx::prefetch_tensormap(&map_k);
-    for (int i = 0; i < C::n_bars; ++i) ptx::mbar_init(&bars[i], i >= C::b_s_free && i < C::b_z_full ? kSumWarps / 2 : 1);
+    for (int i = 0; i < C::n_bars; ++i)
+      ptx::mbar_init(&bars[i], i >= C::b_s_free && i < C::b_z_full ? kSumWarps / 2 : (i >= C::b_z_free && i < C::b_step ? kSumWarps : 1));
     *abort_flag = (ptx::smem_u32(sm) & 1023u) != 0u;      // swizzled tiles need 1024-byte alignment; never seen violated
     if (*abort_flag) atomicExch(a.status, kStatusSmemAlign);
     ptx::fence_mbar_init();
   }
   // rows of a query tile behind Gt * Tt are never loaded: zeros, so that their scores are numbers
-  const int q0 = p.k_stages * C::tile;
+  const int q0 = p.k_stages;                   // first stage of the queries' ring
   if (p.t.Gt * p.t.Tt < kRows) {
-    for (int e = threadIdx.x; e < p.q_stages * C::tile / 16; e += kThreads) *reinterpret_cast<uint4*>(sm + q0 + e * 16) = make_uint4(0, 0, 0, 0);
+    for (int e = threadIdx.x; e < p.q_stages * C::stage / 16; e += kThreads) *reinterpret_cast<uint4*>(sm + q0 * C::stage + e * 16) = make_uint4(0, 0, 0, 0);
     ptx::fence_proxy_async();
   }
   if (warp == 2) {
@@ -192,52 +199,64 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
   if (warp == 0) {
     // ------------------------------- keys and queries -------------------------------
     RingAt k, q;
-    const int pieces = kKeys / p.box, q_bytes = NC * p.t.Gt * p.t.Tt * 128;
+    const int pieces = kKeys / p.box, q_bytes = SC * p.t.Gt * p.t.Tt * 128;
     bool ok = !*abort_flag;
     for (uint32_t n = 0; ok; ++n) {
       const Step s = step_at(n);
       if (s.flags & kEnd) break;
       if (s.flags & kNewKeys) {
-        if (k.round > 0) ok = __all_sync(0xffffffffu, wait(C::b_k_empty + k.stage, (k.round - 1) & 1));
-        if (!ok) break;
-        if (lane == 0) ptx::mbar_arrive_expect_tx(&bars[C::b_k_full + k.stage], C::tile);
-        __syncwarp();
-        for (int i = lane; i < NC * pieces; i += 32) {
-          const int c = i / pieces, key = s.n0 + (i - c * pieces) * p.box;
-          const TilePlace x = place_of(a, s.b, key, s.keys);
-          ptx::tma_load_4d(sm + k.stage * C::tile + c * kChunk + (key - s.n0) * 128, &map_k, c * 64, x.row, s.h, x.outer, &bars[C::b_k_full + k.stage]);
+        const int uses = (s.flags & kOneTile ? 1 : 2) * NS;
+        const TilePlace x0 = place_of(a, s.b, s.n0 + lane * p.box, lane < 2 * pieces ? s.keys : 0);   // lane i: box i of the unit
+        for (int i = 0; i < uses; ++i) {
+          const int tile = i / NS, c0 = i % NS * SC;
+          if (k.round > 0) ok = __all_sync(0xffffffffu, wait(C::b_empty + k.stage, (k.round - 1) & 1));
+          if (!ok) break;
+          if (lane == 0) ptx::mbar_arrive_expect_tx(&bars[C::b_full + k.stage], C::stage);
+          __syncwarp();
+          const int box = lane - tile * pieces;
+          if (box >= 0 && box < pieces)
+            for (int c = 0; c < SC; ++c)
+              ptx::tma_load_4d(sm + k.stage * C::stage + c * kChunk + box * p.box * 128, &map_k, (c0 + c) * 64, x0.row, s.h, x0.outer, &bars[C::b_full + k.stage]);
+          __syncwarp();
+          k.next(p.k_stages);
         }
-        __syncwarp();
-        k.next(p.k_stages);
+        if (!ok) break;
       }
       if (s.flags & kNewQueries) {
-        if (q.round > 0) ok = __all_sync(0xffffffffu, wait(C::b_q_empty + q.stage, (q.round - 1) & 1));
-        if (!ok) break;
-        if (lane == 0) ptx::mbar_arrive_expect_tx(&bars[C::b_q_full + q.stage], q_bytes);
-        __syncwarp();
-        if (lane < NC)
-          ptx::tma_load_4d(sm + q0 + q.stage * C::tile + lane * kChunk, &map_q, lane * 64, s.gc * p.t.Gt, s.t0, s.b * a.Hkv + s.h, &bars[C::b_q_full + q.stage]);
-        __syncwarp();
-        q.next(p.q_stages);
+        for (int i = 0; i < NS; ++i) {
+          if (q.round > 0) ok = __all_sync(0xffffffffu, wait(C::b_empty + q0 + q.stage, (q.round - 1) & 1));
+          if (!ok) break;
+          if (lane == 0) ptx::mbar_arrive_expect_tx(&bars[C::b_full + q0 + q.stage], q_bytes);
+          __syncwarp();
+          if (lane < SC)
+            ptx::tma_load_4d(sm + (q0 + q.stage) * C::stage + lane * kChunk, &map_q, (i * SC + lane) * 64, s.gc * p.t.Gt, s.t0, s.b * a.Hkv + s.h, &bars[C::b_full + q0 + q.stage]);
+          __syncwarp();
+          q.next(p.q_stages);
+        }
       }
     }
   } else if (warp == 3) {
     // ------------------------------------- steps -------------------------------------
-    // A slot is written again when the sums of sixteen steps ago are done; those of four ago are waited for, in order.
+    // A slot is written again when the sums of sixteen steps ago are done; those of twelve ago are waited for, in order.
     Steps st(p, blockIdx.x);
-    bool more = true, ok = true;
-    for (uint32_t n = 0; ok && more; ++n) {
-      more = st.next();
-      if (!more) st.s.flags = kEnd;
+    bool more = st.next(), ok = true;
+    for (uint32_t n = 0; ok; ++n) {
+      Step s = st.s;
+      if (!more) s.flags = kEnd;
+      else {
+        more = st.next();
+        if (!more || (st.s.flags & kNewQueries)) s.flags |= kQueriesLast;
+      }
       if (n >= kRing - kBuffers) {
         const uint32_t done = n - (kRing - kBuffers);
-        ok = __all_sync(0xffffffffu, wait(C::b_s_free + done % kBuffers, (done / kBuffers) & 1));
+        ok = __all_sync(0xffffffffu, wait(C::b_z_free + done % kBuffers, (done / kBuffers) & 1));
       }
       if (lane == 0) {
-        ring[n % kRing] = st.s;
+        ring[n % kRing] = s;
         ptx::mbar_arrive(&bars[C::b_step + n % kRing]);
       }
       __syncwarp();
+      if (s.flags & kEnd) break;
     }
   } else if (warp == 1) {
     // --------------------------------- log-sum-exp ----------------------------------
@@ -275,7 +294,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
           more = fetch(n + kBuffers - 1, v[(k + kBuffers - 1) % kBuffers]);
           have += more;
         }
-        if (n >= kBuffers) ok = __all_sync(0xffffffffu, wait(C::b_s_free + k, (n / kBuffers - 1) & 1));
+        if (n >= kBuffers) ok = __all_sync(0xffffffffu, wait(C::b_z_free + k, (n / kBuffers - 1) & 1));
         float4 x;                                             // neither do rows that see nothing: their lse is -infinity
         x.x = v[k][0] > -INFINITY ? -v[k][0] * kLog2e : -INFINITY;
         x.y = v[k][1] > -INFINITY ? -v[k][1] * kLog2e : -INFINITY;
@@ -289,75 +308,83 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
   } else if (warp == 2) {
     // ---------------------------------- S^T = K Q^T ----------------------------------
     constexpr uint32_t kI = idesc<T>(kKeys, kRows, false);
-    RingAt k, q;                                              // the tiles to come
-    int ka = -1, qa = -1;                                     // the tiles in use
+    RingAt k, q, k_unit, q_tile;                              // the chunks to come; those of the unit and query tile in use
+    uint32_t used = 0;                                        // second key tile's two score buffers: bits 0, 1 in use, bits 2, 3 the phase
+    const uint32_t base = ptx::smem_u32(sm);
     bool ok = true;
     for (uint32_t n = 0; ok; ++n) {
       ok = wait(C::b_step + n % kRing, (n / kRing) & 1);
       const int flags = ok ? ring[n % kRing].flags : kEnd;
       if (flags & kEnd) break;
-      const uint32_t buf = n % kBuffers;
-      if (flags & kNewKeys) {
-        // the last one is free once the products so far are done
-        if (ka >= 0 && ptx::elect_one()) ptx::umma_commit(&bars[C::b_k_empty + ka]);
-        __syncwarp();
-        ka = k.stage;
-        ok = wait(C::b_k_full + ka, k.round & 1);
-        k.next(p.k_stages);
-      }
-      if (flags & kNewQueries) {
-        if (qa >= 0 && ptx::elect_one()) ptx::umma_commit(&bars[C::b_q_empty + qa]);
-        __syncwarp();
-        qa = q.stage;
-        ok = ok && wait(C::b_q_full + qa, q.round & 1);
-        q.next(p.q_stages);
-      }
-      if (n >= kBuffers) ok = ok && wait(C::b_s_free + buf, (n / kBuffers - 1) & 1);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      ptx::tc_fence_after();
-      if (ptx::elect_one()) {
-        const uint32_t d = tmem + buf * 128, k_addr = ptx::smem_u32(sm + ka * C::tile), q_addr = ptx::smem_u32(sm + q0 + qa * C::tile);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const uint64_t da = make_desc(k_addr + c * kChunk, 16, 1024), db = make_desc(q_addr + c * kChunk, 16, 1024);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) ptx::umma_ss(d, da + 2 * k, db + 2 * k, kI, c + k > 0);
+      const int tiles = flags & kOneTile ? 1 : 2;
+      if (flags & kNewKeys) { k_unit = k; k.next(p.k_stages, tiles * NS); }
+      if (flags & kNewQueries) { q_tile = q; q.next(p.q_stages, NS); }
+      RingAt ka = k_unit;
+#pragma unroll 1
+      for (int tile = 0; ok && tile < tiles; ++tile) {
+        const uint32_t buf = (n & 1) * 2 + tile, par = n & 1;
+        if (tile == 0) {
+          if (n >= 2) ok = wait(C::b_s_free + buf, ((n >> 1) - 1) & 1);
+        } else {
+          if (used >> par & 1) ok = wait(C::b_s_free + buf, used >> (2 + par) & 1);
+          used = (used ^ (used >> par & 1) << (2 + par)) | 1u << par;
         }
-        ptx::umma_commit(&bars[C::b_s_full + buf]);
+        RingAt qa = q_tile;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          // a stage of new queries (keys) is used as soon as it is there
+          if ((flags & kNewQueries) && tile == 0) ok = ok && wait(C::b_full + q0 + qa.stage, qa.round & 1);
+          if (flags & kNewKeys) ok = ok && wait(C::b_full + ka.stage, ka.round & 1);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          ptx::tc_fence_after();
+          if (ptx::elect_one()) {
+            const uint32_t d = tmem + buf * 128, k_addr = base + ka.stage * C::stage, q_addr = base + (q0 + qa.stage) * C::stage;
+#pragma unroll
+            for (int c = 0; c < SC; ++c) {
+              const uint64_t da = make_desc(k_addr + c * kChunk, 16, 1024), db = make_desc(q_addr + c * kChunk, 16, 1024);
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk) ptx::umma_ss(d, da + 2 * kk, db + 2 * kk, kI, i + c + kk > 0);
+            }
+            if (i == NS - 1) ptx::umma_commit(&bars[C::b_s_full + buf]);
+            if (flags & kLast) ptx::umma_commit(&bars[C::b_empty + ka.stage]);
+            if ((flags & kQueriesLast) && tile == tiles - 1) ptx::umma_commit(&bars[C::b_empty + q0 + qa.stage]);
+          }
+          __syncwarp();
+          ka.next(p.k_stages);
+          qa.next(p.q_stages);
+        }
       }
-      __syncwarp();
     }
   } else if (warp >= 4) {
     // ------------------------------------- sums --------------------------------------
-    // Two groups of eight warps take the steps in turn; in a group two threads share a key, 64 rows each.
-    const int wq = warp & 3, group = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;   // wq: tensor-memory lane quarter
+    const int wq = warp & 3, tile = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;    // wq: tensor-memory lane quarter
     const int key = wq * 32 + lane;
     const float* z = reinterpret_cast<const float*>(sm + C::z);
-    float* sums = reinterpret_cast<float*>(sm + C::sums);
-    uint32_t n_all = 0, n_single = 0;
+    float* sums = reinterpret_cast<float*>(sm + C::sums) + tile * 512;
+    uint32_t phase = 0, units = 0;                            // phase bits of this tile's two score buffers
     float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     float before = 0.f;
     for (uint32_t n = 0;; ++n) {
       const Step s = step_at(n);
       if (s.flags & kEnd) break;
-      const bool mine = (n & 1u) == (uint32_t)group, single = s.flags & kSingle;   // mine: this step is this group's
-      const bool writer = half == 0 && (single ? mine : group == 0) && s.n0 + key < s.keys;
-      float* out = a.mass + ((long long)s.b * a.Hkv + s.h) * a.mass_stride + s.n0 + key;
-      if (s.flags & kNewKeys) {
-        acc[0] = acc[1] = make_float2(0.f, 0.f);
-        if (writer && s.slot < 0) before = *out;              // wanted at the unit's end
-      }
-      if (mine) {
-        const uint32_t buf = n % kBuffers, par = (n / kBuffers) & 1;
-        wait(C::b_s_full + buf, par);
-        wait(C::b_z_full + buf, par);
+      const uint32_t zb = n % kBuffers;
+      if (tile == 0 || !(s.flags & kOneTile)) {
+        const int n0 = s.n0 + tile * kKeys, nn = n0 + key;
+        float* out = a.mass + ((long long)s.b * a.Hkv + s.h) * a.mass_stride + nn;
+        const bool writer = half == 0 && nn < s.keys;
+        if (s.flags & kNewKeys) {
+          acc[0] = acc[1] = make_float2(0.f, 0.f);
+          if (writer && s.slot < 0) before = *out;            // wanted at the unit's end
+        }
+        const int buf = (n & 1) * 2 + tile;
+        wait(C::b_s_full + buf, phase >> (n & 1) & 1);
+        phase ^= 1u << (n & 1);
+        wait(C::b_z_full + zb, (n / kBuffers) & 1);
         __syncwarp();
         ptx::tc_fence_after();
-        const int p0 = s.keys - s.rows + s.t0, p1 = p0 + p.t.Tt - 1;      // positions of the tile's tokens
-        const bool whole = s.n0 + kKeys - 1 <= p0 && (a.window == 0 || s.n0 > p1 - a.window || s.n0 + kKeys <= a.sinks) && s.t0 + p.t.Tt <= s.rows;
+        const int p0 = s.keys - s.rows + s.t0, p1 = p0 + p.t.Tt - 1;              // positions of the tile's tokens
+        const bool whole = n0 + kKeys - 1 <= p0 && (a.window == 0 || n0 > p1 - a.window || n0 + kKeys <= a.sinks) && s.t0 + p.t.Tt <= s.rows;
         // otherwise rows [lo, hi) of the tile see this key: the tokens from it on, up to a window behind it, that are in use
-        const int nn = s.n0 + key;
         int lo = nn - p0, hi = p.t.Tt < s.rows - s.t0 ? p.t.Tt : s.rows - s.t0;
         if (a.window > 0 && nn >= a.sinks && nn + a.window - p0 < hi) hi = nn + a.window - p0;
         lo = lo < 0 ? 0 : (lo > kRows ? kRows : lo);
@@ -373,7 +400,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
             for (int i = 0; i < 32; ++i)
               if (!((seen >> i) & 1u)) x[i] = 0xff800000u;    // -infinity
           }
-          const float4* zp = reinterpret_cast<const float4*>(z + buf * 128 + col);
+          const float4* zp = reinterpret_cast<const float4*>(z + zb * 128 + col);
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
             const float4 zi = zp[i / 4];
@@ -388,29 +415,18 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&bars[C::b_s_free + buf]);
+        if (s.flags & kLast) {
+          // a key's two threads; the slot of two units ago was read before the last unit's meeting
+          float* slot = sums + (units++ & 1) * 256;
+          slot[half * 128 + key] = (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
+          asm volatile("bar.sync %0, %1;" ::"r"(1 + tile), "n"(kSumWarps * 16) : "memory");
+          const float total = slot[key] + slot[128 + key];
+          if (half == 0 && s.slot >= 0) p.part[(long long)s.slot * kUnitKeys + tile * kKeys + key] = total;
+          else if (writer) *out = before + total;
+        }
       }
-      if (!(s.flags & kLast)) continue;
-      // A key's threads, in order.  Each kind of slot is used every other time: the one of two times ago was read before
-      // the last meeting.
-      const float sum = (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
-      float total;
-      if (single) {                                           // one step: one group's matter, the other goes on
-        if (!mine) continue;
-        float* slot = sums + 1024 + group * 512 + (n_single++ & 1) * 256;
-        slot[half * 128 + key] = sum;
-        asm volatile("bar.sync %0, %1;" ::"r"(2 + group), "n"(kSumWarps * 16) : "memory");
-        total = slot[key] + slot[128 + key];
-      } else {
-        float* slot = sums + (n_all++ & 1) * 512;
-        slot[(group * 2 + half) * 128 + key] = sum;
-        asm volatile("bar.sync 1, %0;" ::"n"(kSumWarps * 32) : "memory");
-        total = (slot[key] + slot[128 + key]) + (slot[256 + key] + slot[384 + key]);
-      }
-      if (s.slot >= 0) {
-        if (half == 0 && (single || group == 0)) p.part[(long long)s.slot * 128 + key] = total;
-      } else if (writer) {
-        *out = before + total;
-      }
+      if (lane == 0) ptx::mbar_arrive(&bars[C::b_z_free + zb]);
+      __syncwarp();
     }
   }
   __syncwarp();
@@ -419,16 +435,16 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
   if (warp == 2) ptx::tmem_dealloc(tmem, 512);
 }
 
-// adds up the pieces of a cut key tile, in order
-__global__ void __launch_bounds__(128) mass_join_kernel(const MassParams p) {
+// adds up the pieces of a cut unit, in order
+__global__ void __launch_bounds__(kUnitKeys) mass_join_kernel(const MassParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Cut cut = p.ranges.cuts[blockIdx.x];
   if (cut.count == 0) return;
   const Cursor c(p.ranges, p.a, cut.unit);
-  const int n = c.u * kKeys + threadIdx.x;
+  const int n = c.u * kUnitKeys + threadIdx.x;
   if (n >= c.len.keys) return;
   float total = 0.f;
-  for (int i = 0; i < cut.count; ++i) total += p.part[(long long)piece_slot(cut, i) * 128 + threadIdx.x];
+  for (int i = 0; i < cut.count; ++i) total += p.part[(long long)piece_slot(cut, i) * kUnitKeys + threadIdx.x];
   p.a.mass[((long long)c.b * p.a.Hkv + c.hg) * p.a.mass_stride + n] += total;
 }
 
@@ -436,11 +452,11 @@ struct Plan { Tiling t; int per_row, grid; size_t total; };
 Plan plan_of(int B, int Hq, int Hkv, int T, int N) {
   Plan x;
   x.t = tiling_of(Hq, Hkv);
-  x.per_row = (N + kKeys - 1) / kKeys;
+  x.per_row = (N + kUnitKeys - 1) / kUnitKeys;
   const long long tiles = (long long)B * Hkv * x.per_row * x.t.GC * ((T + x.t.Tt - 1) / x.t.Tt);
   const int n_sm = sm_count(), most = n_sm < kMaxGrid ? n_sm : kMaxGrid;
   x.grid = (int)(tiles < most ? tiles : most);
-  x.total = ranges_bytes(B, x.per_row, x.grid) + (size_t)2 * x.grid * 128 * 4;
+  x.total = ranges_bytes(B, x.per_row, x.grid) + (size_t)2 * x.grid * kUnitKeys * 4;
   return x;
 }
 
@@ -453,10 +469,10 @@ int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
   p.t = x.t;
   p.ranges = Ranges{a.B, a.Hkv, x.per_row, x.grid, nullptr, nullptr, nullptr};
   p.box = box_rows(a);
-  // one query tile in all: it stays, keys stream; else queries stream past a key tile
+  // one query tile in all: it stays, keys stream; else queries stream past two key tiles
   const bool one = x.t.GC == 1 && a.T <= x.t.Tt;
-  p.q_stages = one ? 1 : C::tiles - (D == 256 ? 1 : 2);
-  p.k_stages = C::tiles - p.q_stages;
+  p.q_stages = one ? C::NS : C::stages - 2 * C::NS;
+  p.k_stages = C::stages - p.q_stages;
   p.scale_log2 = a.scale * kLog2e;
   p.part = reinterpret_cast<float*>(ranges_at(p.ranges, reinterpret_cast<uint8_t*>(a.workspace)));
   CUtensorMap mq, mk;
@@ -479,7 +495,7 @@ int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = C::total;
   DFLASH_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, mq, mk, p));
-  cfg.blockDim = dim3(128);
+  cfg.blockDim = dim3(kUnitKeys);
   cfg.dynamicSmemBytes = 0;
   DFLASH_CUDA_CHECK(cudaLaunchKernelEx(&cfg, mass_join_kernel, p));
   count_launch(3);
