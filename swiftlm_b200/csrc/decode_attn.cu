@@ -18,9 +18,9 @@
 //   barriers a tile.  O is rescaled only when a maximum grows by more than 2^8 (its scale is exact in fp32).
 //   P is rounded to the inputs' type (the sum of the weights is not): the product needs a 16-bit operand.
 // * A unit that one CTA covers is normalised and written at once; the others leave (O, maximum, sum) in the workspace
-//   and decode_combine_kernel, chained by a programmatic launch, joins them in a fixed order.
+//   and decode_finish_kernel, chained by a programmatic launch, joins them in a fixed order.
 // * With `mass`, the scaled scores of the visible tokens are kept (4 bytes per head and key, 3 % of the bytes read at
-//   D = 256, G = 8) and decode_mass_kernel turns them into weights when every head's sum is known: reading K a second
+//   D = 256, G = 8) and decode_finish_kernel turns them into weights when every head's sum is known: reading K a second
 //   time would cost sixteen times as much.
 #include <type_traits>
 
@@ -57,6 +57,7 @@ struct DecodeParams {
   CacheArgs a;
   int b0, nb;                  // the launch's sequences
   int G, GC;                   // heads per KV head, head groups per KV head
+  int heads;                   // query heads a block of decode_finish_kernel joins
   int max_chunks;              // upper bound of a unit's chunks
   float scale_log2;
   float *part_o, *part_m, *part_l;   // [2 * grid][8 NT][D], [2 * grid][8 NT] twice
@@ -425,106 +426,134 @@ __global__ void __launch_bounds__(Shape<D>::W * 32, Shape<D>::per_sm) decode_ker
   }
 }
 
-// Joins the ranges of one (sequence, query head): weights 2^(m_r - max m), summed in the order of the ranges.
-constexpr int kCombineThreads = 256;
+// Behind the main kernel, one launch for two things.
+// Join: the ranges of a cut unit with weights 2^(m_r - max m), summed in the order of the ranges.  A block takes p.heads heads of
+// one unit; where a unit has few ranges a group of D / 4 threads takes a head each, else all groups share a head's ranges.
+// Mass: mass[b, h, n] += sum over the heads of 2^(score - lse), one thread per visible key, the heads in order.  The
+// log-sum-exps of a cut unit's heads are computed again by every block that needs them: a few loads, against a launch.
+constexpr int kFinishThreads = 256;
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kCombineThreads) decode_combine_kernel(const DecodeParams p) {
-  constexpr int H = 8 * NT, V = D / 4, R = kCombineThreads / V;      // float4 columns, groups of ranges
-  __shared__ float wt[256];
-  __shared__ float red[2 * kCombineThreads / 32];
-  __shared__ float4 acc[R][V];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+__global__ void __launch_bounds__(kFinishThreads) decode_finish_kernel(const DecodeParams p) {
+  constexpr int H = 8 * NT, V = D / 4, R = kFinishThreads / V;       // float4 columns, groups of threads
+  __shared__ float acc_s[R][V][4];
+  __shared__ float zs[H];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const CacheArgs& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int hq = blockIdx.x, b = p.b0 + blockIdx.y, h = hq / p.G, g = hq % p.G;
-  const long long unit = ((long long)b * a.Hkv + h) * p.GC + g / H;
-  const int j = g % H;
-  const int2 info = p.unit_info[unit];
-  const int n = info.y;
-  if (n == 0) return;
-  auto slot_of = [&](int r) { return 2 * (info.x + r) + (r == 0 ? 1 : 0); };
-  float top = -INFINITY;
-  for (int r = tid; r < n; r += kCombineThreads) top = fmaxf(top, p.part_m[slot_of(r) * H + j]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) red[warp] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kCombineThreads / 32; ++w) top = fmaxf(top, red[w]);
-  const float z = top == -INFINITY ? 0.f : top;
-  const int col = tid % V, grp = tid / V;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-  for (int r0 = 0; r0 < n; r0 += 256) {
-    const int cnt = n - r0 < 256 ? n - r0 : 256;
-    __syncthreads();
-    if (tid < cnt) {
-      const int sl = slot_of(r0 + tid) * H + j;
+  const int blocks = (p.G < H ? p.G + p.heads - 1 : H + p.heads - 1) / p.heads;      // head blocks of a unit
+  const int u = blockIdx.x / blocks, j0 = (blockIdx.x - u * blocks) * p.heads;
+  const int bh = u / p.GC, gc = u - bh * p.GC, b = p.b0 + bh / a.Hkv, h = bh % a.Hkv;
+  auto slot_of = [&](const int2& info, int r) { return 2 * (info.x + r) + (r == 0 ? 1 : 0); };
+  if (blockIdx.y == 0) {
+    const long long unit = ((long long)b * a.Hkv + h) * p.GC + gc;
+    const int2 info = p.unit_info[unit];
+    const int n = info.y, col = tid % V, grp = tid / V;
+    int j1 = p.G - gc * H < H ? p.G - gc * H : H;            // heads of the unit
+    if (j1 > j0 + p.heads) j1 = j0 + p.heads;
+    auto store = [&](int j, float4 o, float top, float sum) {
+      const long long row = (long long)b * a.Hq + h * p.G + gc * H + j;
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      uint2 pk;
+      pk.x = mma::pack<T>(o.x * inv, o.y * inv);
+      pk.y = mma::pack<T>(o.z * inv, o.w * inv);
+      *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + row * D + col * 4) = pk;
+      if (col == 0 && a.lse) a.lse[row] = sum > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+    };
+    auto add = [&](int j, int r, float z, float4& o, float& sum) {
+      const int sl = slot_of(info, r) * H + j;
       const float w = mma::exp2_approx(p.part_m[sl] - z);
-      wt[tid] = w;
       sum = fmaf(w, p.part_l[sl], sum);
-    }
-    __syncthreads();
-#pragma unroll 4
-    for (int r = grp; r < cnt; r += R) {
-      const float w = wt[r];
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + ((long long)slot_of(r0 + r) * H + j) * D + col * 4);
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + (long long)sl * D + col * 4);
       o.x = fmaf(w, v.x, o.x); o.y = fmaf(w, v.y, o.y); o.z = fmaf(w, v.z, o.z); o.w = fmaf(w, v.w, o.w);
+    };
+    if (n > 0 && n <= 8 && j1 - j0 > 1) {
+      for (int j = j0 + grp; j < j1; j += R) {
+        float top = -INFINITY, sum = 0.f;
+        for (int r = 0; r < n; ++r) top = fmaxf(top, p.part_m[slot_of(info, r) * H + j]);
+        const float z = top == -INFINITY ? 0.f : top;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int r = 0; r < n; ++r) add(j, r, z, o, sum);
+        store(j, o, top, sum);
+      }
+    } else if (n > 0) {
+      for (int j = j0; j < j1; ++j) {
+        float top = -INFINITY, sum = 0.f;
+        for (int r = lane; r < n; r += 32) top = fmaxf(top, p.part_m[slot_of(info, r) * H + j]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float z = top == -INFINITY ? 0.f : top;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int r = grp; r < n; r += R) add(j, r, z, o, sum);      // this group's ranges
+        *reinterpret_cast<float4*>(acc_s[grp][col]) = o;
+        sum = 0.f;                                               // of all ranges, by every warp alike
+        for (int r = lane; r < n; r += 32) {
+          const int sl = slot_of(info, r) * H + j;
+          sum = fmaf(mma::exp2_approx(p.part_m[sl] - z), p.part_l[sl], sum);
+        }
+#pragma unroll
+        for (int q = 16; q > 0; q >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, q);
+        __syncthreads();
+        if (grp == 0) {                                          // the groups' shares, in order
+#pragma unroll
+          for (int k = 1; k < R; ++k) {
+            const float4 v = *reinterpret_cast<const float4*>(acc_s[k][col]);
+            o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+          }
+          store(j, o, top, sum);
+        }
+        __syncthreads();
+      }
     }
+    return;
   }
-#pragma unroll
-  for (int sh = 16; sh > 0; sh >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, sh);
-  if (lane == 0) red[kCombineThreads / 32 + warp] = sum;
-  acc[grp][col] = o;
-  __syncthreads();
-  sum = 0.f;
-#pragma unroll
-  for (int w = 0; w < kCombineThreads / 32; ++w) sum += red[kCombineThreads / 32 + w];
-  if (grp == 0) {
-#pragma unroll
-    for (int k = 1; k < R; ++k) {
-      const float4 v = acc[k][col];
-      o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
-    }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    const long long row = (long long)b * a.Hq + hq;
-    uint2 pk;
-    pk.x = mma::pack<T>(o.x * inv, o.y * inv);
-    pk.y = mma::pack<T>(o.z * inv, o.w * inv);
-    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + row * D + col * 4) = pk;
-    if (tid == 0) {
-      const float y = sum > 0.f ? top + log2f(sum) : -INFINITY;
-      if (a.lse) a.lse[row] = y * kLn2;
-      if (p.lse2) p.lse2[row] = y;
-    }
-  }
-}
-
-// mass[b, h, n] += sum over the heads of 2^(score - lse): one thread per visible key, the heads in order.
-template <int NT>
-__global__ void __launch_bounds__(256) decode_mass_kernel(const DecodeParams p) {
-  constexpr int H = 8 * NT;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const CacheArgs& a = p.a;
-  const int bh = blockIdx.x, b = p.b0 + bh / a.Hkv, h = bh % a.Hkv;
+  if (gc != 0 || j0 != 0) return;              // rows of blocks from 1 on: mass
   const Visible v = visible_of(a, lens_of(a, b).keys);
-  for (long long e = (long long)blockIdx.y * 256 + threadIdx.x; e < (long long)v.count * 16; e += (long long)gridDim.y * 256) {
-    const int n = chunk_key(v, (int)(e >> 4)) + ((int)e & 15);
-    if (n >= v.n || !(n >= v.lo || n < v.sinks)) continue;
+  const long long keys = (long long)v.count * 16;
+  const long long first = (long long)(blockIdx.y - 1) * kFinishThreads;
+  for (long long e0 = first; e0 < keys; e0 += (long long)(gridDim.y - 1) * kFinishThreads) {
+    const long long e = e0 + tid;
+    const int n = e < keys ? chunk_key(v, (int)(e >> 4)) + ((int)e & 15) : 0;
+    const bool on = e < keys && n < v.n && (n >= v.lo || n < v.sinks);
     float total = 0.f;
-    for (int gc = 0; gc < p.GC; ++gc) {
-      const long long unit = ((long long)b * a.Hkv + h) * p.GC + gc;
+    for (int g = 0; g < p.GC; ++g) {
+      const long long unit = ((long long)b * a.Hkv + h) * p.GC + g;
+      const int heads = p.G - g * H < H ? p.G - g * H : H;
+      const int2 info = p.unit_info[unit];
+      const bool known = p.GC == 1 && e0 > first;              // one group of heads: its log-sum-exps stay in shared memory
+      __syncthreads();
+      for (int j = known ? heads : warp; j < heads; j += kFinishThreads / 32) {
+        float z;
+        if (info.y == 0) {
+          z = p.lse2[(long long)b * a.Hq + h * p.G + g * H + j];
+        } else {
+          float top = -INFINITY, sum = 0.f;
+          for (int r = lane; r < info.y; r += 32) top = fmaxf(top, p.part_m[slot_of(info, r) * H + j]);
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          const float zz = top == -INFINITY ? 0.f : top;
+          for (int r = lane; r < info.y; r += 32) {
+            const int sl = slot_of(info, r) * H + j;
+            sum = fmaf(mma::exp2_approx(p.part_m[sl] - zz), p.part_l[sl], sum);
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          z = sum > 0.f ? top + log2f(sum) : -INFINITY;
+        }
+        if (lane == 0) zs[j] = z;
+      }
+      __syncthreads();
+      if (!on) continue;
       const float* sc = p.scores + (unit * p.max_chunks * 16 + e) * H;
-      const float* z = p.lse2 + (long long)b * a.Hq + h * p.G + gc * H;
       float x[H];
 #pragma unroll
       for (int i = 0; i < H; i += 4) *reinterpret_cast<float4*>(&x[i]) = *reinterpret_cast<const float4*>(sc + i);
 #pragma unroll
       for (int i = 0; i < H; ++i)
-        if (gc * H + i < p.G) total += mma::exp2_approx(x[i] - z[i]);
+        if (i < heads) total += mma::exp2_approx(x[i] - zs[i]);
     }
-    a.mass[((long long)b * a.Hkv + h) * a.mass_stride + n] += total;
+    if (on) a.mass[((long long)b * a.Hkv + h) * a.mass_stride + n] += total;
   }
 }
 
@@ -602,14 +631,17 @@ int32_t launch_typed(const CacheArgs& a, const Plan& t, cudaStream_t stream) {
     const int grid = (int)(tiles < t.grid_max ? tiles : t.grid_max);
     kernel<<<grid, L::W * 32, L::fixed + p.nb * 8, stream>>>(p);
     DFLASH_LAUNCH_CHECK();
-    DFLASH_CUDA_CHECK(launch_chained(decode_combine_kernel<T, D, NT>, dim3(a.Hq, p.nb), kCombineThreads, p, stream));
+    // Units that are hardly cut: a block for all heads of one (64 sequences of 8 KV heads with a window: 58 us the whole
+    // call, 60 with 2048 blocks of a head each).  A unit in many ranges: a block a head.
+    const long long units = (long long)p.nb * a.Hkv * t.GC;
+    const int heads = t.G < 8 * NT ? t.G : 8 * NT;
+    p.heads = units >= grid / 4 ? heads : 1;
+    const long long x = units * ((heads + p.heads - 1) / p.heads), blocks = 1 + (a.mass ? ((long long)t.max_chunks * 16 + kFinishThreads - 1) / kFinishThreads : 0);
+    // enough blocks for the mass to fill the GPU once: each finds the log-sum-exps for itself
+    const long long once = 1 + (6 * (long long)sm_count() + x - 1) / x;
+    const unsigned y = (unsigned)(blocks < once ? blocks : (once < 65535 ? once : 65535));
+    DFLASH_CUDA_CHECK(launch_chained(decode_finish_kernel<T, D, NT>, dim3((unsigned)x, y), kFinishThreads, p, stream));
     count_launch(2);
-    if (a.mass) {
-      const long long blocks = ((long long)t.max_chunks * 16 + 255) / 256;
-      const unsigned mass_y = (unsigned)(blocks < 65535 ? blocks : 65535);
-      DFLASH_CUDA_CHECK(launch_chained(decode_mass_kernel<NT>, dim3(p.nb * a.Hkv, mass_y), 256, p, stream));
-      count_launch();
-    }
   }
   return DFLASH_OK;
 }
