@@ -368,6 +368,8 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
       const Step s = step_at(n);
       if (s.flags & kEnd) break;
       const uint32_t zb = n % kBuffers;
+      // waited for by the warps that have no tile here too: running ahead, they would arrive twice in one phase of z_free
+      wait(C::b_z_full + zb, (n / kBuffers) & 1);
       if (tile == 0 || !(s.flags & kOneTile)) {
         const int n0 = s.n0 + tile * kKeys, nn = n0 + key;
         float* out = a.mass + ((long long)s.b * a.Hkv + s.h) * a.mass_stride + nn;
@@ -379,7 +381,6 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         const int buf = (n & 1) * 2 + tile;
         wait(C::b_s_full + buf, phase >> (n & 1) & 1);
         phase ^= 1u << (n & 1);
-        wait(C::b_z_full + zb, (n / kBuffers) & 1);
         __syncwarp();
         ptx::tc_fence_after();
         const int p0 = s.keys - s.rows + s.t0, p1 = p0 + p.t.Tt - 1;              // positions of the tile's tokens

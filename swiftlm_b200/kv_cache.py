@@ -32,7 +32,7 @@ class KVCacheFull(RuntimeError):
 
 class PagedKVCache:
     def __init__(self, batch: int, kv_heads: int, head_dim: int, page_tokens: int, num_pages: int, max_pages: int,
-                 dtype: torch.dtype = torch.bfloat16, device="cuda", block: int = 16):
+                 dtype: torch.dtype = torch.bfloat16, device="cuda", block: int = 16, track_mass: bool = False):
         self.B, self.Hkv, self.D = batch, kv_heads, head_dim
         self.page_tokens, self.num_pages, self.max_pages, self.block = page_tokens, num_pages, max_pages, block
         self.k_pool = torch.zeros(num_pages, kv_heads, page_tokens, head_dim, dtype=dtype, device=device)
@@ -43,6 +43,8 @@ class PagedKVCache:
         self.page_table = self._table_host.to(device)
         self.kv_len = torch.zeros(batch, dtype=torch.int32, device=device)        # committed tokens per sequence
         self.kv_len_block = torch.zeros(batch, dtype=torch.int32, device=device)  # committed + the block just appended
+        # attention weight received so far, per KV head and position; 0 for a token that has just been appended
+        self.mass = torch.zeros(batch, kv_heads, max_pages * page_tokens, device=device) if track_mass else None
         self._free: List[int] = list(range(num_pages - 1, -1, -1))                # pop() hands out page 0 first
         self._pages: List[List[int]] = [[] for _ in range(batch)]
         self._upper = [0] * batch            # host upper bound of kv_len
@@ -93,6 +95,9 @@ class PagedKVCache:
         self._flush_table()
         kernels.kv_append(k_new.contiguous(), v_new.contiguous(), self.k_pool, self.v_pool, kv_len=self.kv_len,
                           page_table=self.page_table, kv_len_out=self.kv_len_block)
+        if self.mass is not None:                    # rows rejected earlier may have left their weight in these places
+            at = (self.kv_len.long()[:, None] + torch.arange(T, device=self.kv_len.device)).clamp_(max=self.mass.shape[2] - 1)
+            self.mass.scatter_(2, at[:, None].expand(-1, self.Hkv, -1), 0.0)
         self._appended = T
         return self.kv_len_block
 
@@ -116,6 +121,49 @@ class PagedKVCache:
         self.append_block(k, v)
         self.commit(lens_dev)
 
+    # ---- outside the verify cycle ----
+    def _n_max(self, extra: int = 0) -> int:
+        return max(1, min(max(self._upper) + extra, self.max_pages * self.page_tokens))
+
+    def attend_one(self, queries: torch.Tensor, scale: float, window: int = 0, sinks: int = 0, return_lse: bool = False):
+        """Attention of one new token per sequence, queries [B,Hq,D], over the committed tokens and the one just appended
+        (append_block with one row).  With track_mass its weights are added to the mass."""
+        if self._appended != 1:
+            raise RuntimeError("attend_one() follows append_block() of one row")
+        return kernels.decode_sdpa(queries, self.k_pool, self.v_pool, scale, kv_len=self.kv_len_block, page_table=self.page_table,
+                                   window=window, sinks=sinks, mass=self.mass, return_lse=return_lse, n_max=self._n_max(1))
+
+    def attend_prompt(self, queries: torch.Tensor, scale: float, q_len: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0,
+                      return_lse: bool = False, out: Optional[torch.Tensor] = None):
+        """Attention of the committed tokens' last rows, queries [B,Hq,T,D] (after extend(), or a commit): row r of sequence b is
+        token kv_len[b] - q_len[b] + r (q_len int32[B]; default T)."""
+        return kernels.prompt_sdpa(queries, self.k_pool, self.v_pool, scale, q_len=q_len, kv_len=self.kv_len, page_table=self.page_table,
+                                   window=window, sinks=sinks, return_lse=return_lse, out=out, n_max=self._n_max())
+
+    def add_mass(self, queries: torch.Tensor, lse: torch.Tensor, scale: float, q_len: Optional[torch.Tensor] = None, window: int = 0,
+                 sinks: int = 0) -> None:
+        """Adds the weights of attend_prompt()'s rows (all of them, or the last ones) to the mass."""
+        if self.mass is None:
+            raise RuntimeError("the cache was made without track_mass")
+        kernels.attention_mass(queries, self.k_pool, lse, scale, self.mass, q_len=q_len, kv_len=self.kv_len, page_table=self.page_table,
+                               window=window, sinks=sinks, n_max=self._n_max())
+
+    def evict(self, budget: int, recent: int, sinks: int = 0) -> None:
+        """Cuts every sequence longer than `budget` tokens to it: the first `sinks`, the last `recent` and the heaviest of
+        the others stay, per KV head.  Positions are those of the shorter cache afterwards; pages behind the budget
+        return to the pool.  No host read of the lengths."""
+        if self.mass is None:
+            raise RuntimeError("the cache was made without track_mass")
+        if self._appended:
+            raise RuntimeError("evict() between append_block() and commit()")
+        kernels.kv_evict(self.k_pool, self.v_pool, self.mass, self.kv_len, budget, recent, sinks=sinks, page_table=self.page_table,
+                         n_max=self._n_max())
+        for b in range(self.B):
+            if self._upper[b] > budget:
+                self._upper[b] = budget
+                self._shrink(b, budget)
+        self._flush_table()
+
     def sync(self) -> np.ndarray:
         """Reads the committed lengths (one device-to-host copy), tightens the host bounds and returns the pages
         beyond every sequence's committed length to the pool."""
@@ -131,6 +179,8 @@ class PagedKVCache:
         self._shrink(b, 0)
         self._upper[b] = 0
         self.kv_len[b] = 0
+        if self.mass is not None:
+            self.mass[b] = 0
         self._flush_table()
 
     # ---- inspection (tests) ----

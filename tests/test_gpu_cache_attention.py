@@ -161,6 +161,9 @@ PROMPT = [
     (1, 2, 1, 513, 128, 513, "bf16", 0, None, None, 1, 0),
     (1, 2, 1, 257, 64, 2000, "bf16", 64, None, None, 64, 300),
     (1, 4, 4, 640, 64, 640, "f16", 0, None, None, 0, 0),
+    (3, 16, 2, 300, 256, 300, "bf16", 256, [300, 100, 257], [300, 100, 257], 0, 0),      # several query tiles, one key tile of two
+    (2, 48, 1, 50, 128, 120, "bf16", 0, [120, 60], [50, 50], 0, 0),                      # 2 tokens a query tile
+    (1, 260, 2, 6, 64, 70, "f16", 0, None, None, 0, 0),                                  # more heads in a group than rows in a tile
     (9, 6, 2, 5, 128, 50, "f16", 0, [50, 5, 7, 49, 33, 16, 17, 5, 5], None, 3, 2),
 ]
 
