@@ -480,6 +480,7 @@ int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
   CUresult r = encode_q(&mq, a, x.t);
   if (r == CUDA_SUCCESS) r = encode_kv(&mk, a.k, a, p.box);
   if (r != CUDA_SUCCESS) { set_error("attention_mass: cuTensorMapEncodeTiled failed with CUresult %d", (int)r); return DFLASH_ERR_CUDA; }
+  if (!ranges_fit(a.B, x.per_row)) { set_error("attention_mass: unsupported: more than 2^30 units of work"); return DFLASH_ERR_UNSUPPORTED; }
   auto kernel = mass_kernel<T, D>;
   static std::atomic<uint64_t> ready{0};
   DFLASH_CUDA_CHECK(allow_shared(ready, kernel, C::total));

@@ -62,8 +62,7 @@ template <int D> struct Cfg {
   static constexpr int k = QT * NC * kChunk, v = k + KS * k_stage;
   static constexpr int bars = v + VS * v_stage;
   // barriers
-  static constexpr int b_q_full = 0, b_q_empty = 1, b_s_full = 2, b_p_half = 4, b_s_free = 8, b_pv_done = 10,
-                       b_tail = 12, b_k_full = 13, b_k_empty = b_k_full + KS, b_v_full = b_k_empty + KS, b_v_empty = b_v_full + VS,
+  static constexpr int b_q_full = 0, b_q_empty = 1, b_s_full = 2, b_p_half = 4, b_pv_done = 8, b_tail = 10, b_k_full = 11, b_k_empty = b_k_full + KS, b_v_full = b_k_empty + KS, b_v_empty = b_v_full + VS,
                        n_bars = b_v_empty + VS;
   static constexpr int misc = bars + (8 * n_bars + 15) / 16 * 16;   // tensor-memory base, abort flag
   static constexpr int xch = misc + 16;                     // row maxima (sums) of the two halves: [QT][slots][2][128]
@@ -314,7 +313,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             for (int qi = 0; ok && qi < nq; ++qi) {
               // the buffer is free once the product that read P from it has retired
               const int buf = PAIR ? (int)(drain & 1) : qi;
-              if (n_s[buf] > 0) ok = wait(C::b_s_free + buf, (n_s[buf] - 1) & 1);
+              if (n_s[buf] > 0) ok = wait(C::b_pv_done + buf, (n_s[buf] - 1) & 1);
               if (!ok) break;
               ptx::tc_fence_after();
               if (ptx::elect_one()) {
@@ -374,8 +373,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                     else ptx::umma_ts(d, pt + pc, db + (uint64_t)k * 128, kI, j > s.lo || half + i > 0);
                   }
                   if (half) {
-                    commit(C::b_pv_done + qi);
-                    commit(C::b_s_free + buf);
+                    commit(C::b_pv_done + buf);
                     if (qi == nq - 1) commit(C::b_v_empty + st);
                   }
                 }
@@ -401,6 +399,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     const int col0 = grp * 64;
     float* xch = reinterpret_cast<float*>(sm + C::xch) + qi * C::slots * 256;
     uint32_t n_s = 0, n_x = 0;                                // score tiles and exchanges done
+    auto pv_done = [&](uint32_t n) { wait(C::b_pv_done + (PAIR ? (int)(n & 1) : qi), PAIR ? (n >> 1) & 1 : n & 1); };
     // Value of the thread that has the other half of this row; the two warps always meet the same number of times.  With
     // one slot the next value is written only after this one has been read: the next tile's scores take both threads' P.
     auto other_half = [&](float mine) {
@@ -466,7 +465,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         // the last product is done with the accumulator
         if (rescale) {
           constexpr int kCols = D / 2;
-          wait(C::b_pv_done + qi, (n_s - 1) & 1);
+          pv_done(n_s - 1);
           __syncwarp();
           ptx::tc_fence_after();
 #pragma unroll 1
@@ -505,14 +504,14 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
           ptx::tc_fence_before();
           // Every phase is waited for, in order (a parity wait that skips one cannot tell "done" from "two phases behind"),
           // and before the next one can end, which takes this warp's arrival.
-          if (half && n_s > 0) wait(C::b_pv_done + qi, (n_s - 1) & 1);
+          if (half && n_s > 0) pv_done(n_s - 1);
           __syncwarp();
           if (lane == 0) arrive_leader(C::b_p_half + 2 * half + buf);
         }
         l += (add[0].x + add[0].y) + (add[1].x + add[1].y);
       }
       // ---- the segment's result ----
-      wait(C::b_pv_done + qi, (n_s - 1) & 1);
+      pv_done(n_s - 1);
       __syncwarp();
       ptx::tc_fence_after();
       {                                                        // the same order of the two halves in both threads
@@ -662,6 +661,7 @@ int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
   if (r == CUDA_SUCCESS) r = encode_kv(&mk, a.k, a, p.box < C::k_rows ? p.box : C::k_rows);
   if (r == CUDA_SUCCESS) r = encode_kv(&mv, a.v, a, p.box);
   if (r != CUDA_SUCCESS) { set_error("prompt_sdpa: cuTensorMapEncodeTiled failed with CUresult %d", (int)r); return DFLASH_ERR_CUDA; }
+  if (!ranges_fit(a.B, x.per_row)) { set_error("prompt_sdpa: unsupported: more than 2^30 units of work"); return DFLASH_ERR_UNSUPPORTED; }
   auto kernel = prompt_kernel<T, D>;
   static std::atomic<uint64_t> ready{0};
   DFLASH_CUDA_CHECK(allow_shared(ready, kernel, C::total));

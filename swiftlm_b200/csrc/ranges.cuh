@@ -12,16 +12,19 @@ namespace dflash {
 
 constexpr int kMinCut = 4;                   // steps of the smallest piece of a cut unit
 constexpr int kMaxGrid = 1023;               // workers at most: a boundary for each thread of plan_ranges
+constexpr int kNearCosts = 2048;             // entries of the cost table that are kept in shared memory: searching the other
+                                             // way, through L2, was 5 of the plan's 8 us
 
 struct Boundary { long long unit; int off, pad; };   // in front of step `off` of a unit
 struct Cut { long long unit; int first, count; };    // a unit in `count` pieces, of the workers first, first + 1, ...
 struct Ranges {
   int B, HG, per_row, grid;
-  long long* cost;             // [B * per_row + 1] cost of what is in front of every (sequence, unit)
+  long long* cost;             // [B * per_row + 1] cost of what is in front of every (sequence, unit), where that is a long table
   Boundary* bounds;            // [grid + 1]
   Cut* cuts;                   // [grid]
 };
 
+inline bool ranges_fit(long long B, long long per_row) { return B * per_row < (1ll << 30); }
 inline size_t ranges_bytes(long long B, long long per_row, int grid) {
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   return up((size_t)(B * per_row + 1) * 8) + up((size_t)(grid + 1) * sizeof(Boundary)) + up((size_t)grid * sizeof(Cut));
@@ -38,20 +41,25 @@ inline uint8_t* ranges_at(Ranges& r, uint8_t* ws) {
 }
 
 // One block of 1024 threads.  steps(len, unit in its row): 0 for a unit without work.
+static_assert(sizeof(Boundary) * (kMaxGrid + 1) <= 8 * (kNearCosts + 2), "the boundaries take the costs' place");
 template <int UnitCost, typename Steps>
 __device__ __forceinline__ void plan_ranges(const Ranges& p, const CacheArgs& a, Steps steps) {
   __shared__ long long warp_sums[32];
+  __shared__ __align__(16) long long near[kNearCosts + 2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long E = (long long)p.B * p.per_row, HG = p.HG;
+  const int E = p.B * p.per_row;             // the host sees to it that this is an int
+  const long long HG = p.HG;
   auto cost = [&](RowLens len, int u) { const int n = steps(len, u); return n > 0 ? n + UnitCost : 0; };
-  const long long per_thread = (E + 1023) / 1024, e0 = tid * per_thread, e1 = e0 + per_thread < E ? e0 + per_thread : E;
+  const int per_thread = (E - 1) / 1024 + 1, e0 = tid * per_thread < E ? tid * per_thread : E, e1 = E - e0 < per_thread ? E : e0 + per_thread;
+  const bool is_near = E <= kNearCosts;
+  const long long* table = is_near ? near : p.cost;
   long long mine = 0;
   int b = -1;
   RowLens len{0, 0};
-  for (long long e = e0; e < e1; ++e) {
-    const int eb = (int)(e / p.per_row);
+  for (int e = e0; e < e1; ++e) {
+    const int eb = e / p.per_row;
     if (eb != b) { b = eb; len = lens_of(a, b, true); }
-    mine += cost(len, (int)(e - (long long)b * p.per_row));
+    mine += cost(len, e - b * p.per_row);
   }
   long long x = mine;
 #pragma unroll
@@ -63,16 +71,16 @@ __device__ __forceinline__ void plan_ranges(const Ranges& p, const CacheArgs& a,
   __syncthreads();
   long long at = x - mine;
   for (int w = 0; w < warp; ++w) at += warp_sums[w];
-  b = -1;
-  for (long long e = e0; e < e1; ++e) {
-    const int eb = (int)(e / p.per_row);
+  for (int e = e0; e < e1; ++e) {
+    (is_near ? near : p.cost)[e] = at;
+    if (e + 1 == e1) break;
+    const int eb = e / p.per_row;
     if (eb != b) { b = eb; len = lens_of(a, b); }
-    p.cost[e] = at;
-    at += cost(len, (int)(e - (long long)b * p.per_row));
+    at += cost(len, e - b * p.per_row);
   }
   long long all = 0;
   for (int w = 0; w < 32; ++w) all += warp_sums[w];
-  if (tid == 0) p.cost[E] = all;
+  if (tid == 0) (is_near ? near : p.cost)[E] = all;
   __syncthreads();               // the table is read by other threads of this block below
   const long long total = all * HG;
   const long long per = total > p.grid ? (total + p.grid - 1) / p.grid : 1;
@@ -85,16 +93,16 @@ __device__ __forceinline__ void plan_ranges(const Ranges& p, const CacheArgs& a,
       int lo = 0, hi = p.B - 1;             // the last sequence that starts at or before pos
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (p.cost[(long long)mid * p.per_row] * HG <= pos) lo = mid; else hi = mid - 1;
+        if (table[(long long)mid * p.per_row] * HG <= pos) lo = mid; else hi = mid - 1;
       }
-      const long long base = p.cost[(long long)lo * p.per_row], len_b = p.cost[(long long)(lo + 1) * p.per_row] - base;
+      const long long base = table[(long long)lo * p.per_row], len_b = table[(long long)(lo + 1) * p.per_row] - base;
       const long long hg = (pos - base * HG) / len_b, rem = pos - base * HG - hg * len_b;
       int ta = 0, tb = p.per_row - 1;             // the last unit that starts at or before rem
       while (ta < tb) {
         const int mid = (ta + tb + 1) >> 1;
-        if (p.cost[(long long)lo * p.per_row + mid] - base <= rem) ta = mid; else tb = mid - 1;
+        if (table[(long long)lo * p.per_row + mid] - base <= rem) ta = mid; else tb = mid - 1;
       }
-      const long long s = p.cost[(long long)lo * p.per_row + ta] - base, e = p.cost[(long long)lo * p.per_row + ta + 1] - base;
+      const long long s = table[(long long)lo * p.per_row + ta] - base, e = table[(long long)lo * p.per_row + ta + 1] - base;
       const long long unit = ((long long)lo * HG + hg) * p.per_row + ta;
       const int size = (int)(e - s) - UnitCost;
       int off = (int)(rem - s) - UnitCost;
@@ -105,6 +113,7 @@ __device__ __forceinline__ void plan_ranges(const Ranges& p, const CacheArgs& a,
     raw[c] = r;
   }
   __syncthreads();
+  Boundary* bounds = reinterpret_cast<Boundary*>(near);      // the costs are done with
   // equal boundaries become one, so that the pieces of a cut unit belong to workers in a row
   {
     const bool fresh = tid <= p.grid && (tid == 0 || raw[tid].unit != raw[tid - 1].unit || raw[tid].off != raw[tid - 1].off);
@@ -116,17 +125,18 @@ __device__ __forceinline__ void plan_ranges(const Ranges& p, const CacheArgs& a,
       before += w < warp ? (int)warp_sums[w] : 0;
       all_fresh += (int)warp_sums[w];
     }
-    if (fresh) p.bounds[before + __popc(in_warp & ((1u << lane) - 1u))] = raw[tid];
-    if (tid >= all_fresh && tid <= p.grid) p.bounds[tid] = Boundary{E * HG, 0, 0};
+    if (fresh) bounds[before + __popc(in_warp & ((1u << lane) - 1u))] = raw[tid];
+    if (tid >= all_fresh && tid <= p.grid) bounds[tid] = Boundary{E * HG, 0, 0};
   }
   __syncthreads();
+  if (tid <= p.grid) p.bounds[tid] = bounds[tid];
   if (tid < p.grid) {
     const int c = tid;
     Cut cut{0, 0, 0};
-    if (c >= 1 && p.bounds[c].off > 0 && !(p.bounds[c - 1].off > 0 && p.bounds[c - 1].unit == p.bounds[c].unit)) {
+    if (c >= 1 && bounds[c].off > 0 && !(bounds[c - 1].off > 0 && bounds[c - 1].unit == bounds[c].unit)) {
       int n = 1;
-      while (c + n <= p.grid && p.bounds[c + n].off > 0 && p.bounds[c + n].unit == p.bounds[c].unit) ++n;
-      cut = Cut{p.bounds[c].unit, c - 1, n + 1};
+      while (c + n <= p.grid && bounds[c + n].off > 0 && bounds[c + n].unit == bounds[c].unit) ++n;
+      cut = Cut{bounds[c].unit, c - 1, n + 1};
     }
     p.cuts[c] = cut;
   }
