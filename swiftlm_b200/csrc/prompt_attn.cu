@@ -21,6 +21,13 @@
 // * Persistent CTAs, one per SM.  plan_kernel cuts the key tiles of all units into equal ranges (ranges.cuh), so that unequal
 //   lengths, causal triangles and few query rows over a long cache all fill the GPU.  A unit cut in pieces leaves (O, m, l) per piece in the workspace and
 //   join_kernel adds them up in order.
+//
+// Measured (B200, the whole call): 16 query / 2 KV heads, D = 256, a prompt of 8192 0.46 ms = 1.21 PFLOP/s (0.74 of what cuBLAS
+// reaches in a burst, 0.86 of what it sustains under the power cap), a chunk of 2048 over 10240 tokens 0.26 ms (0.74); a key
+// tile takes 2670 clocks, 2048 of them on the tensor pipe.  32 / 8 heads, D = 128, two prompts of 8192 with a window of 1024:
+// 0.43 ms (0.39): 4300 clocks for the two tiles' 2048 of products and 2048 of exponentials, the softmax threads' waits
+// (tensor-memory loads and stores, the other half's maximum, the hand-over of P) are most of the rest.  Five prompts of up to 193:
+// 24 us, three launches' latency.
 #include "ranges.cuh"
 #include "tc_common.cuh"
 
