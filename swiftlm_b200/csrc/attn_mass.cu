@@ -57,7 +57,7 @@ template <int D> struct Cfg {
   static constexpr int SC = NC < 2 ? NC : 2, NS = NC / SC, stages = 12 / SC, stage = SC * kChunk;
   static constexpr int bars = stages * stage;
   static constexpr int b_full = 0, b_empty = stages, b_s_full = 2 * stages, b_s_free = b_s_full + 4, b_z_full = b_s_free + 4,
-                       b_z_free = b_z_full + kBuffers, b_step = b_z_free + kBuffers, n_bars = b_step + kRing;
+                       b_z_free = b_z_full + kBuffers, b_step = b_z_free + kBuffers, b_meet = b_step + kRing, n_bars = b_meet + 2;
   static constexpr int misc = bars + (8 * n_bars + 15) / 16 * 16;
   static constexpr int z = misc + 16;                       // [kBuffers][128] -log2(e) lse of the rows
   static constexpr int sums = z + kBuffers * 128 * 4;       // [2 key tiles][2][2 halves][128]
@@ -163,7 +163,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     ptx::prefetch_tensormap(&map_q);
     ptx::prefetch_tensormap(&map_k);
     for (int i = 0; i < C::n_bars; ++i)
-      ptx::mbar_init(&bars[i], i >= C::b_s_free && i < C::b_z_full ? kSumWarps / 2 : (i >= C::b_z_free && i < C::b_step ? kSumWarps : 1));
+      ptx::mbar_init(&bars[i], (i >= C::b_s_free && i < C::b_z_full) || i >= C::b_meet ? kSumWarps / 2 : (i >= C::b_z_free && i < C::b_step ? kSumWarps : 1));
     *abort_flag = (ptx::smem_u32(sm) & 1023u) != 0u;      // swizzled tiles need 1024-byte alignment; never seen violated
     if (*abort_flag) atomicExch(a.status, kStatusSmemAlign);
     ptx::fence_mbar_init();
@@ -185,7 +185,10 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
   const uint32_t tmem = *tmem_slot;
   // A wait that gives up raises the abort flag, after which every wait returns at once: the roles run through their loops
   // without results, meet at the end and leave.
-  auto wait = [&](int bar, uint32_t parity) { return ptx::mbar_wait_or_abort(&bars[bar], parity, abort_flag, a.status, kStatusMbarWait); };
+  // Every wait is made by a whole warp, whose lanes agree on the outcome: none leaves a loop that the others stay in.
+  auto wait = [&](int bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, ptx::mbar_wait_or_abort(&bars[bar], parity, abort_flag, a.status, kStatusMbarWait));
+  };
   // Warp 3 walks the CTA's steps and describes them in a ring; the others read.  (Every role walking for itself was five
   // copies of that code: an eighth of the instruction fetches missed and each step took 2350 clocks.)
   Step* ring = reinterpret_cast<Step*>(sm + C::steps);
@@ -204,7 +207,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
     // ------------------------------- keys and queries -------------------------------
     RingAt k, q;
     const int pieces = kKeys / p.box, q_bytes = SC * p.t.Gt * p.t.Tt * 128;
-    bool ok = !*abort_flag;
+    bool ok = __all_sync(0xffffffffu, !*abort_flag);
     for (uint32_t n = 0; ok; ++n) {
       const Step s = step_at(n);
       if (s.flags & kEnd) break;
@@ -213,7 +216,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         const TilePlace x0 = place_of(a, s.b, s.n0 + lane * p.box, lane < 2 * pieces ? s.keys : 0);   // lane i: box i of the unit
         for (int i = 0; i < uses; ++i) {
           const int tile = i / NS, c0 = i % NS * SC;
-          if (k.round > 0) ok = __all_sync(0xffffffffu, wait(C::b_empty + k.stage, (k.round - 1) & 1));
+          if (k.round > 0) ok = wait(C::b_empty + k.stage, (k.round - 1) & 1);
           if (!ok) break;
           if (lane == 0) ptx::mbar_arrive_expect_tx(&bars[C::b_full + k.stage], C::stage);
           __syncwarp();
@@ -228,7 +231,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
       }
       if (s.flags & kNewQueries) {
         for (int i = 0; i < NS; ++i) {
-          if (q.round > 0) ok = __all_sync(0xffffffffu, wait(C::b_empty + q0 + q.stage, (q.round - 1) & 1));
+          if (q.round > 0) ok = wait(C::b_empty + q0 + q.stage, (q.round - 1) & 1);
           if (!ok) break;
           if (lane == 0) ptx::mbar_arrive_expect_tx(&bars[C::b_full + q0 + q.stage], q_bytes);
           __syncwarp();
@@ -253,7 +256,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
       }
       if (n >= kRing - kBuffers) {
         const uint32_t done = n - (kRing - kBuffers);
-        ok = __all_sync(0xffffffffu, wait(C::b_z_free + done % kBuffers, (done / kBuffers) & 1));
+        ok = wait(C::b_z_free + done % kBuffers, (done / kBuffers) & 1);
       }
       if (lane == 0) {
         ring[n % kRing] = s;
@@ -298,7 +301,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
           more = fetch(n + kBuffers - 1, v[(k + kBuffers - 1) % kBuffers]);
           have += more;
         }
-        if (n >= kBuffers) ok = __all_sync(0xffffffffu, wait(C::b_z_free + k, (n / kBuffers - 1) & 1));
+        if (n >= kBuffers) ok = wait(C::b_z_free + k, (n / kBuffers - 1) & 1);
         float4 x;                                             // neither do rows that see nothing: their lse is -infinity
         x.x = v[k][0] > -INFINITY ? -v[k][0] * kLog2e : -INFINITY;
         x.y = v[k][1] > -INFINITY ? -v[k][1] * kLog2e : -INFINITY;
@@ -339,7 +342,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
           // a stage of new queries (keys) is used as soon as it is there
           if ((flags & kNewQueries) && tile == 0) ok = ok && wait(C::b_full + q0 + qa.stage, qa.round & 1);
           if (flags & kNewKeys) ok = ok && wait(C::b_full + ka.stage, ka.round & 1);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          if (!ok) break;
           ptx::tc_fence_after();
           if (ptx::elect_one()) {
             const uint32_t d = tmem + buf * 128, k_addr = base + ka.stage * C::stage, q_addr = base + (q0 + qa.stage) * C::stage;
@@ -422,12 +425,16 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
         if (lane == 0) ptx::mbar_arrive(&bars[C::b_s_free + buf]);
         if (s.flags & kLast) {
           // a key's two threads; the slot of two units ago was read before the last unit's meeting
-          float* slot = sums + (units++ & 1) * 256;
+          float* slot = sums + (units & 1) * 256;
           slot[half * 128 + key] = (acc[0].x + acc[0].y) + (acc[1].x + acc[1].y);
-          asm volatile("bar.sync %0, %1;" ::"r"(1 + tile), "n"(kSumWarps * 16) : "memory");
-          const float total = slot[key] + slot[128 + key];
-          if (half == 0 && s.slot >= 0) p.part[(long long)s.slot * kUnitKeys + tile * kKeys + key] = total;
-          else if (writer) *out = before + total;
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(&bars[C::b_meet + tile]);
+          // a bounded wait: after one that gave up, a tile's warps may be at different steps
+          if (wait(C::b_meet + tile, units++ & 1)) {
+            const float total = slot[key] + slot[128 + key];
+            if (half == 0 && s.slot >= 0) p.part[(long long)s.slot * kUnitKeys + tile * kKeys + key] = total;
+            else if (writer) *out = before + total;
+          }
         }
       }
       if (lane == 0) ptx::mbar_arrive(&bars[C::b_z_free + zb]);

@@ -206,8 +206,9 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     atomicExch(a.status, kStatusMbarWait);
     return false;
   };
-  auto wait = [&](int bar, uint32_t parity) { return wait_as(bar, parity, false); };
-  auto wait_pair = [&](int bar, uint32_t parity) { return wait_as(bar, parity, true); };   // the other CTA's stores among what is waited for
+  // Every wait is made by a whole warp, whose lanes agree on the outcome: none leaves a loop that the others stay in.
+  auto wait = [&](int bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_as(bar, parity, false)); };
+  auto wait_pair = [&](int bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_as(bar, parity, true)); };   // the other CTA's stores among what is waited for
   auto commit = [&](int bar) {
     if constexpr (PAIR) ptx::umma_commit_pair(&bars[bar]);
     else ptx::umma_commit(&bars[bar]);
@@ -229,9 +230,9 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     if (warp == 0) {
       // ------------------------------ queries and keys ------------------------------
       uint32_t fill = 0, seg = 0;
-      bool ok = !*abort_flag;
+      bool ok = __all_sync(0xffffffffu, !*abort_flag);
       while (ok && walk.next(s)) {
-        if (seg > 0) ok = __all_sync(0xffffffffu, wait(C::b_q_empty, (seg - 1) & 1));
+        if (seg > 0) ok = wait(C::b_q_empty, (seg - 1) & 1);
         if (!ok) break;
         if (lane == 0) {
           const int tiles = PAIR ? 2 : s.nq;                  // a pair's tile without rows in use reads as zeros
@@ -245,7 +246,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         for (int j = s.lo; j < s.hi; ++j, ++fill) {
           const int n0 = tile_key(s.u.k, j) + rank * 64;
           const uint32_t st = fill % KS;
-          if (fill >= KS) ok = __all_sync(0xffffffffu, wait(C::b_k_empty + st, (fill / KS - 1) & 1));
+          if (fill >= KS) ok = wait(C::b_k_empty + st, (fill / KS - 1) & 1);
           if (!ok) break;
           if (lane == 0 && rank == 0) ptx::mbar_arrive_expect_tx(&bars[C::b_k_full + st], (PAIR ? 2 : 1) * C::k_stage);
           __syncwarp();
@@ -262,12 +263,12 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     } else if (warp == 1) {
       // ----------------------------------- values -----------------------------------
       uint32_t fill = 0, tails = 0;
-      bool ok = !*abort_flag;
+      bool ok = __all_sync(0xffffffffu, !*abort_flag);
       while (ok && walk.next(s)) {
         for (int j = s.lo; j < s.hi; ++j, ++fill) {
           const int n0 = tile_key(s.u.k, j), rows = s.u.len.keys - n0;
           const uint32_t st = fill % VS;
-          if (fill >= VS) ok = __all_sync(0xffffffffu, wait(C::b_v_empty + st, (fill / VS - 1) & 1));
+          if (fill >= VS) ok = wait(C::b_v_empty + st, (fill / VS - 1) & 1);
           if (!ok) break;
           // Rows behind the sequence's length: a weight of zero times whatever the cache holds there would not be zero, so
           // such a tile lands under a barrier of its own and the rows are cleared before the tile is announced.
@@ -290,7 +291,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
           }
           __syncwarp();
           if (tail) {
-            ok = __all_sync(0xffffffffu, wait(C::b_tail, tails++ & 1));
+            ok = wait(C::b_tail, tails++ & 1);
             if (!ok) break;
             for (int c = 0; c < C::v_chunks; ++c)
               for (int e = (rows > 0 ? rows : 0) * 8 + lane; e < kKeys * 8; e += 32)
