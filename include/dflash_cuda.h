@@ -233,7 +233,7 @@ int32_t dflash_kv_commit(int32_t* kv_len, const int32_t* commit, int32_t B, int3
  * Shared conventions.
  *   k, v       dense [B,Hkv,N,D], or with page_table a pool [num_pages,Hkv,page_tokens,D] as for
  *              dflash_verify_sdpa, here with page_tokens any multiple of 16.  With a page table N is an upper bound
- *              of the lengths (<= max_pages * page_tokens).  A page id outside the pool reads as zeros and
+ *              of the lengths (<= max_pages * page_tokens).  N and T are at most 2^29.  A page id outside the pool reads as zeros and
  *              is reported through dflash_device_status.
  *   kv_len     int32[B] or NULL (N each): cached tokens of sequence b, the queries' own tokens among them.
  *   q_len      int32[B] or NULL (T each): query rows of sequence b that are in use.  Rows behind them are not used,

@@ -16,7 +16,7 @@
 //
 // Measured (B200, the whole call): 2048 rows of 32 / 8 heads over 16384 tokens, D = 128, 0.38 ms = 0.69 PFLOP/s; 1.0e9
 // exponentials take 0.24 ms at 16 a clock and SM.  16 rows of 32 sequences of 1.4 to 4.1 thousand tokens, D = 256: 35 us, the 94 MB
-// take 14 at the HBM's rate; half is the plan, the start of the CTAs and their unequal number of units.
+// take 14 at the HBM's rate; the plan and the start of the CTAs are behind most of the rest.
 #include "ranges.cuh"
 #include "tc_common.cuh"
 

@@ -18,6 +18,7 @@ int32_t check(const char* op, CacheArgs& a) {
   if (a.dtype != DFLASH_BF16 && a.dtype != DFLASH_F16) { set_error("%s: unsupported dtype %d (bf16 or f16)", op, a.dtype); return DFLASH_ERR_UNSUPPORTED; }
   if (a.D != 64 && a.D != 128 && a.D != 256) { set_error("%s: unsupported head_dim %d (64, 128 or 256)", op, a.D); return DFLASH_ERR_UNSUPPORTED; }
   if (a.Hq % a.Hkv != 0) { set_error("%s: unsupported heads: Hq=%d not a multiple of Hkv=%d", op, a.Hq, a.Hkv); return DFLASH_ERR_UNSUPPORTED; }
+  if (a.N > kMaxTokens || a.T > kMaxTokens) { set_error("%s: unsupported length: N=%d, T=%d (at most 2^29)", op, a.N, a.T); return DFLASH_ERR_UNSUPPORTED; }
   if (a.window < 0 || a.sinks < 0) return invalid(op, "negative window or sinks");
   if (!(a.scale >= 1e-30f && a.scale <= 1e30f)) return invalid(op, "scale must be positive and finite");   // running maxima assume its sign
   if (a.page_table) {
@@ -76,7 +77,7 @@ int32_t dflash_decode_sdpa(const void* q, const void* k, const void* v, const in
 
 size_t dflash_decode_sdpa_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t N, int32_t window,
                                           int32_t sinks, int32_t with_mass) {
-  if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || N <= 0 || Hq % Hkv != 0 || window < 0 || sinks < 0) return 0;
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || N <= 0 || N > kMaxTokens || Hq % Hkv != 0 || window < 0 || sinks < 0) return 0;
   return decode_workspace_bytes(B, Hq, Hkv, D, N, window >= N ? 0 : window, sinks > N ? N : sinks, with_mass != 0);
 }
 
@@ -96,7 +97,7 @@ int32_t dflash_prompt_sdpa(const void* q, const void* k, const void* v, const in
 }
 
 size_t dflash_prompt_sdpa_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t D, int32_t N) {
-  if (B <= 0 || Hq <= 0 || Hkv <= 0 || T <= 0 || D <= 0 || N <= 0 || Hq % Hkv != 0) return 0;
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || T <= 0 || D <= 0 || N <= 0 || N > kMaxTokens || T > kMaxTokens || Hq % Hkv != 0) return 0;
   return prompt_workspace_bytes(B, Hq, Hkv, T, D, N);
 }
 
@@ -116,7 +117,7 @@ int32_t dflash_attention_mass(const void* q, const void* k, const int32_t* page_
 }
 
 size_t dflash_attention_mass_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t D, int32_t N) {
-  if (B <= 0 || Hq <= 0 || Hkv <= 0 || T <= 0 || D <= 0 || N <= 0 || Hq % Hkv != 0) return 0;
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || T <= 0 || D <= 0 || N <= 0 || N > kMaxTokens || T > kMaxTokens || Hq % Hkv != 0) return 0;
   return mass_workspace_bytes(B, Hq, Hkv, T, D, N);
 }
 

@@ -24,6 +24,8 @@ struct CacheArgs {
   int* status;
 };
 
+constexpr int kMaxTokens = 1 << 29;   // N and T at most: sums of two positions and a window stay in 32 bits
+
 struct RowLens { int keys, rows; };   // cached tokens, query rows in use
 
 // Lengths of sequence b, clamped to [0, N] and [0, T]; one thread of the grid passes report = true.

@@ -17,7 +17,7 @@
 //
 // Measured (B200, the whole call): 32 sequences x 2 heads from 1104 to 1088 tokens (135 MB) 43 us, selection 12 and move 26 (20.6
 // at the HBM's rate); 8 x 2 heads from up to 32768 to 4096 60 us, selection 28 and move 27.
-#include "common.cuh"
+#include "cache_ops.cuh"
 #include "ptx.cuh"
 
 namespace dflash {
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(kMoveThreads) move_kernel(const EvictParams p,
 static size_t moves_bytes(int B, int Hkv) { return ((size_t)B * Hkv * sizeof(int2) + 255) / 256 * 256; }
 
 extern "C" size_t dflash_kv_evict_workspace_bytes(int32_t B, int32_t Hkv, int32_t N, int32_t budget) {
-  if (B <= 0 || Hkv <= 0 || N <= 0 || budget <= 0) return 0;
+  if (B <= 0 || Hkv <= 0 || N <= 0 || N > dflash::kMaxTokens || budget <= 0) return 0;
   return moves_bytes(B, Hkv) + (size_t)B * Hkv * (size_t)(budget < N ? budget : N) * sizeof(longlong2);
 }
 
@@ -325,6 +325,7 @@ extern "C" int32_t dflash_kv_evict(void* k_cache, void* v_cache, const int32_t* 
   if (B <= 0 || Hkv <= 0 || D <= 0 || N <= 0) return invalid("non-positive dimension");
   if (dtype != DFLASH_BF16 && dtype != DFLASH_F16 && dtype != DFLASH_F32) { set_error("kv_evict: unsupported dtype %d", dtype); return DFLASH_ERR_UNSUPPORTED; }
   if (budget <= 0 || recent < 0 || sinks < 0 || (long long)recent + sinks > budget) return invalid("need budget > 0 and sinks + recent <= budget");
+  if (N > kMaxTokens) { set_error("kv_evict: unsupported length N=%d (at most 2^29)", N); return DFLASH_ERR_UNSUPPORTED; }
   if (mass_stride < N) return invalid("mass_stride smaller than N");
   if (page_table && (page_tokens <= 0 || max_pages <= 0 || num_pages <= 0 || (long long)max_pages * page_tokens < N))
     return invalid("paged cache needs page_tokens, num_pages and max_pages * page_tokens >= N");

@@ -286,15 +286,20 @@ def _workspace_bytes(name: str, device_index: int, *sizes) -> int:
 
 
 def _on_its_device(fn):
-    """Runs fn(t, ...) with t's device current: allocation, stream and launch all go to it."""
+    """Runs fn with its first argument's device current: allocation, stream and launch all go to it."""
+    first = fn.__code__.co_varnames[0]
+
     @functools.wraps(fn)
-    def call(t, *args, **kwargs):
+    def call(*args, **kwargs):
+        t = args[0] if args else kwargs.get(first)
+        if t is None:
+            raise TypeError(f"{fn.__name__}() needs {first}")
         if not t.is_cuda:
             _need_cuda(t)
         if t.device.index == torch.cuda.current_device():
-            return fn(t, *args, **kwargs)
+            return fn(*args, **kwargs)
         with torch.cuda.device(t.device):
-            return fn(t, *args, **kwargs)
+            return fn(*args, **kwargs)
     return call
 
 
@@ -380,6 +385,7 @@ def decode_sdpa(queries, keys, values, scale: float, kv_len=None, page_table=Non
     Returns [B,Hq,D], or (that, lse fp32 [B,Hq]) with return_lse.
     """
     _cache_tensors(queries, 3, keys, values, page_table, mass, out)
+    scale, window, sinks = float(scale), int(window), int(sinks)
     B, Hq, D = queries.shape
     Hkv, device = keys.shape[1], queries.device
     page_table, N, page_tokens, max_pages, num_pages = _cache_shape(keys, page_table, n_max, B)
@@ -410,6 +416,7 @@ def prompt_sdpa(queries, keys, values, scale: float, q_len=None, kv_len=None, pa
     Returns [B,Hq,T,D], or (that, lse fp32 [B,Hq,T]) with return_lse (-inf on rows that see nothing or are not in use).
     """
     _cache_tensors(queries, 4, keys, values, page_table, out)
+    scale, window, sinks = float(scale), int(window), int(sinks)
     B, Hq, T, D = queries.shape
     Hkv, device = keys.shape[1], queries.device
     page_table, N, page_tokens, max_pages, num_pages = _cache_shape(keys, page_table, n_max, B)
@@ -432,6 +439,7 @@ def attention_mass(queries, keys, lse, scale: float, mass, q_len=None, kv_len=No
     rows and the query heads of a KV head: exp(scale * q.k - lse) with the lse [B,Hq,T] of prompt_sdpa over the same cache
     (all of a chunk's rows, or its last ones: the rows given are the last T, or q_len, tokens of the cache)."""
     _cache_tensors(queries, 4, keys, None, page_table, lse, mass)
+    scale, window, sinks = float(scale), int(window), int(sinks)
     B, Hq, T, D = queries.shape
     Hkv, device = keys.shape[1], queries.device
     if lse.dtype != torch.float32 or lse.shape != (B, Hq, T):
@@ -470,7 +478,7 @@ def kv_evict(k_cache, v_cache, mass, kv_len, budget: int, recent: int, sinks: in
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise _bad("the caches are changed in place and must be contiguous")
     B, Hkv, D = kv_len.numel(), k_cache.shape[1], k_cache.shape[3]
-    budget = int(budget)
+    budget, recent, sinks = int(budget), int(recent), int(sinks)
     page_table, N, page_tokens, max_pages, num_pages = _cache_shape(k_cache, page_table, n_max, B)
     kv_len_out = kv_len if kv_len_out is None else kv_len_out
     for t, name in ((kv_len, "kv_len"), (kv_len_out, "kv_len_out")):
@@ -488,7 +496,7 @@ def kv_evict(k_cache, v_cache, mass, kv_len, budget: int, recent: int, sinks: in
     _lib.check(_lib.lib().dflash_kv_evict(
         k_cache.data_ptr(), v_cache.data_ptr(), _ptr(page_table), kv_len.data_ptr(), mass.data_ptr(), kv_len_out.data_ptr(),
         mass_out.data_ptr(), _ptr(kept), _ptr(ws), need, B, Hkv, D, N, page_tokens, max_pages, num_pages, mass.shape[2], budget,
-        int(recent), int(sinks), _DT[k_cache.dtype], _raw_stream(device.index)))
+        recent, sinks, _DT[k_cache.dtype], _raw_stream(device.index)))
     return kv_len_out
 
 

@@ -93,3 +93,16 @@ def test_python_side_refuses_cpu_tensors():
         kernels.attention_mass(q[:, :, None], k, torch.zeros(1, 4, 1), 1.0, torch.zeros(1, 2, 8))
     with pytest.raises(RuntimeError):
         kernels.kv_evict(k, k, torch.zeros(1, 2, 8), torch.zeros(1, dtype=torch.int32), 4, 1)
+
+
+@pytest.mark.parametrize("op", ["decode", "prompt", "mass", "evict"])
+def test_lengths_whose_positions_pass_32_bits_are_refused(op):
+    for n in (2 ** 29 + 1, 2 ** 31 - 1):
+        assert call(op, N=n, mass_stride=n) == _lib.ERR_UNSUPPORTED
+        if op in ("prompt", "mass"):
+            assert call(op, T=n) == _lib.ERR_UNSUPPORTED
+    L, n = _lib.lib(), 2 ** 31 - 1
+    assert L.dflash_decode_sdpa_workspace_bytes(1, 16, 2, 256, n, 0, 0, 1) == 0
+    assert L.dflash_prompt_sdpa_workspace_bytes(1, 16, 2, 8, 256, n) == 0 and L.dflash_prompt_sdpa_workspace_bytes(1, 16, 2, n, 256, 8) == 0
+    assert L.dflash_attention_mass_workspace_bytes(1, 16, 2, 8, 256, n) == 0 and L.dflash_attention_mass_workspace_bytes(1, 16, 2, n, 256, 8) == 0
+    assert L.dflash_kv_evict_workspace_bytes(1, 2, n, 8) == 0

@@ -284,3 +284,30 @@ def test_views_are_taken_and_wrong_tensors_refused():
         cache.evict(8, 2)
     with pytest.raises(RuntimeError):
         cache.attend_one(torch.zeros(1, 2, 64, dtype=BF, device="cuda"), 1.0)
+
+
+@pytest.mark.gpu
+def test_named_arguments_and_scalars_of_other_types():
+    import numpy as np
+    from swiftlm_b200 import kernels
+    torch.manual_seed(5)
+    q = torch.randn(2, 4, 3, 64, device="cuda", dtype=torch.bfloat16)
+    k, v = (torch.randn(2, 2, 40, 64, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    one = q[:, :, -1].contiguous()
+    a = kernels.decode_sdpa(one, k, v, 0.125, window=16, sinks=2)
+    b = kernels.decode_sdpa(queries=one, keys=k, values=v, scale=np.float32(0.125), window=np.int64(16), sinks=np.int32(2))
+    assert torch.equal(a, b)
+    a, lse = kernels.prompt_sdpa(q, k, v, 0.125, window=16, sinks=2, return_lse=True)
+    b = kernels.prompt_sdpa(queries=q, keys=k, values=v, scale=torch.tensor(0.125), window=torch.tensor(16), sinks=np.int32(2))
+    assert torch.equal(a, b)
+    m1, m2 = (torch.zeros(2, 2, 40, device="cuda") for _ in range(2))
+    kernels.attention_mass(q, k, lse, 0.125, m1, window=16, sinks=2)
+    kernels.attention_mass(queries=q, keys=k, lse=lse, scale=np.float64(0.125), mass=m2, window=np.int64(16), sinks=np.int64(2))
+    assert torch.equal(m1, m2)
+    n1, n2 = (torch.full((2,), 40, dtype=torch.int32, device="cuda") for _ in range(2))
+    k1, v1, k2, v2 = k.clone(), v.clone(), k.clone(), v.clone()
+    kernels.kv_evict(k1, v1, m1, n1, 20, 4, sinks=2)
+    kernels.kv_evict(k_cache=k2, v_cache=v2, mass=m2, kv_len=n2, budget=np.int64(20), recent=np.int64(4), sinks=np.int32(2))
+    assert torch.equal(k1, k2) and torch.equal(v1, v2) and torch.equal(m1, m2) and torch.equal(n1, n2)
+    with pytest.raises(TypeError):
+        kernels.decode_sdpa(keys=k, values=v, scale=0.125)
