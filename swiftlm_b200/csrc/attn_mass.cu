@@ -14,8 +14,8 @@
 // are cut into equal ranges per CTA (ranges.cuh); pieces of a cut unit leave 256 sums in the workspace, added in order by
 // mass_join_kernel: the order of every sum is fixed.
 //
-// Measured (B200, the whole call): 2048 rows of 32 / 8 heads over 16384 tokens, D = 128, 0.38 ms = 0.69 PFLOP/s; 1.0e9
-// exponentials take 0.24 ms at 16 a clock and SM.  16 rows of 32 sequences of 1.4 to 4.1 thousand tokens, D = 256: 35 us, the 94 MB
+// Measured (B200, the whole call): 2048 rows of 32 / 8 heads over 16384 tokens, D = 128, 0.38 ms = 0.68 PFLOP/s; 1.0e9
+// exponentials take 0.24 ms at 16 a clock and SM.  16 rows of 32 sequences of 1.4 to 4.1 thousand tokens, D = 256: 36 us, the 94 MB
 // take 14 at the HBM's rate; the plan and the start of the CTAs are behind most of the rest.
 #include "ranges.cuh"
 #include "tc_common.cuh"
@@ -185,10 +185,10 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
   const uint32_t tmem = *tmem_slot;
   // A wait that gives up raises the abort flag, after which every wait returns at once: the roles run through their loops
   // without results, meet at the end and leave.
-  // Every wait is made by a whole warp, whose lanes agree on the outcome: none leaves a loop that the others stay in.
-  auto wait = [&](int bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, ptx::mbar_wait_or_abort(&bars[bar], parity, abort_flag, a.status, kStatusMbarWait));
-  };
+  // Every wait is made by a whole warp.  wait(): its lanes agree on the outcome, none leaves a loop that the others stay in;
+  // wait_lane(): where the outcome decides nothing, or the lanes agree on it behind the next wait.
+  auto wait_lane = [&](int bar, uint32_t parity) { return ptx::mbar_wait_or_abort(&bars[bar], parity, abort_flag, a.status, kStatusMbarWait); };
+  auto wait = [&](int bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_lane(bar, parity)); };
   // Warp 3 walks the CTA's steps and describes them in a ring; the others read.  (Every role walking for itself was five
   // copies of that code: an eighth of the instruction fetches missed and each step took 2350 clocks.)
   Step* ring = reinterpret_cast<Step*>(sm + C::steps);
@@ -331,18 +331,18 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
       for (int tile = 0; ok && tile < tiles; ++tile) {
         const uint32_t buf = (n & 1) * 2 + tile, par = n & 1;
         if (tile == 0) {
-          if (n >= 2) ok = wait(C::b_s_free + buf, ((n >> 1) - 1) & 1);
+          if (n >= 2) ok = wait_lane(C::b_s_free + buf, ((n >> 1) - 1) & 1);
         } else {
-          if (used >> par & 1) ok = wait(C::b_s_free + buf, used >> (2 + par) & 1);
+          if (used >> par & 1) ok = wait_lane(C::b_s_free + buf, used >> (2 + par) & 1);
           used = (used ^ (used >> par & 1) << (2 + par)) | 1u << par;
         }
         RingAt qa = q_tile;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
           // a stage of new queries (keys) is used as soon as it is there
-          if ((flags & kNewQueries) && tile == 0) ok = ok && wait(C::b_full + q0 + qa.stage, qa.round & 1);
-          if (flags & kNewKeys) ok = ok && wait(C::b_full + ka.stage, ka.round & 1);
-          if (!ok) break;
+          if ((flags & kNewQueries) && tile == 0) ok &= wait_lane(C::b_full + q0 + qa.stage, qa.round & 1);
+          if (flags & kNewKeys) ok &= wait_lane(C::b_full + ka.stage, ka.round & 1);
+          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
           ptx::tc_fence_after();
           if (ptx::elect_one()) {
             const uint32_t d = tmem + buf * 128, k_addr = base + ka.stage * C::stage, q_addr = base + (q0 + qa.stage) * C::stage;
@@ -376,7 +376,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
       if (s.flags & kEnd) break;
       const uint32_t zb = n % kBuffers;
       // waited for by the warps that have no tile here too: running ahead, they would arrive twice in one phase of z_free
-      wait(C::b_z_full + zb, (n / kBuffers) & 1);
+      wait_lane(C::b_z_full + zb, (n / kBuffers) & 1);
       if (tile == 0 || !(s.flags & kOneTile)) {
         const int n0 = s.n0 + tile * kKeys, nn = n0 + key;
         float* out = a.mass + ((long long)s.b * a.Hkv + s.h) * a.mass_stride + nn;
@@ -386,7 +386,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
           if (writer && s.slot < 0) before = *out;            // wanted at the unit's end
         }
         const int buf = (n & 1) * 2 + tile;
-        wait(C::b_s_full + buf, phase >> (n & 1) & 1);
+        wait_lane(C::b_s_full + buf, phase >> (n & 1) & 1);
         phase ^= 1u << (n & 1);
         __syncwarp();
         ptx::tc_fence_after();

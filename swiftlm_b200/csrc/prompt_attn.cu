@@ -22,12 +22,12 @@
 //   lengths, causal triangles and few query rows over a long cache all fill the GPU.  A unit cut in pieces leaves (O, m, l) per piece in the workspace and
 //   join_kernel adds them up in order.
 //
-// Measured (B200, the whole call): 16 query / 2 KV heads, D = 256, a prompt of 8192 0.46 ms = 1.21 PFLOP/s (0.74 of what cuBLAS
-// reaches in a burst, 0.86 of what it sustains under the power cap), a chunk of 2048 over 10240 tokens 0.26 ms (0.74); a key
+// Measured (B200, the whole call): 16 query / 2 KV heads, D = 256, a prompt of 8192 0.47 ms = 1.18 PFLOP/s (0.72 of what cuBLAS
+// reaches in a burst, 0.84 of what it sustains under the power cap), a chunk of 2048 over 10240 tokens 0.26 ms (0.72); a key
 // tile takes 2670 clocks, 2048 of them on the tensor pipe.  32 / 8 heads, D = 128, two prompts of 8192 with a window of 1024:
-// 0.43 ms (0.39): 4300 clocks for the two tiles' 2048 of products and 2048 of exponentials, the softmax threads' waits
+// 0.42 ms (0.40): 4300 clocks for the two tiles' 2048 of products and 2048 of exponentials, the softmax threads' waits
 // (tensor-memory loads and stores, the other half's maximum, the hand-over of P) are most of the rest.  Five prompts of up to 193:
-// 24 us, three launches' latency.
+// 23 us, three launches' latency.
 #include "ranges.cuh"
 #include "tc_common.cuh"
 
@@ -206,7 +206,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     atomicExch(a.status, kStatusMbarWait);
     return false;
   };
-  // Every wait is made by a whole warp, whose lanes agree on the outcome: none leaves a loop that the others stay in.
+  // Every wait is made by a whole warp, whose lanes agree on the outcome: none leaves a loop that the others stay in.  (The
+  // softmax warps' loops do not depend on it: they call wait_as.)
   auto wait = [&](int bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_as(bar, parity, false)); };
   auto wait_pair = [&](int bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_as(bar, parity, true)); };   // the other CTA's stores among what is waited for
   auto commit = [&](int bar) {
@@ -407,7 +408,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     const int col0 = grp * 64;
     float* xch = reinterpret_cast<float*>(sm + C::xch) + qi * C::slots * 256;
     uint32_t n_s = 0, n_x = 0;                                // score tiles and exchanges done
-    auto pv_done = [&](uint32_t n) { wait(C::b_pv_done + (PAIR ? (int)(n & 1) : qi), PAIR ? (n >> 1) & 1 : n & 1); };
+    auto pv_done = [&](uint32_t n) { wait_as(C::b_pv_done + (PAIR ? (int)(n & 1) : qi), PAIR ? (n >> 1) & 1 : n & 1, false); };
     // Value of the thread that has the other half of this row; the two warps always meet the same number of times.  With
     // one slot the next value is written only after this one has been read: the next tile's scores take both threads' P.
     auto other_half = [&](float mine) {
@@ -426,7 +427,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       float m = -INFINITY, l = 0.f;
       for (int j = s.lo; j < s.hi; ++j, ++n_s) {
         const int buf = PAIR ? (int)(n_s & 1) : qi;
-        wait(C::b_s_full + buf, PAIR ? (n_s >> 1) & 1 : n_s & 1);
+        wait_as(C::b_s_full + buf, PAIR ? (n_s >> 1) & 1 : n_s & 1, false);
         __syncwarp();
         ptx::tc_fence_after();
         const uint32_t s_addr = lane_addr + C::col_s(buf) + col0;
