@@ -8,15 +8,16 @@
 // histogram in each CTA's shared memory per digit, added up through distributed shared memory), then one pass that writes
 // the kept places in ascending order by counts in front: a token stays when its key is above the threshold, or equal to it and
 // among the first (need - above) equals.  No atomic decides an order, so ties go to the lowest index on every run.
-// Masses are read four times, from L2; one CTA for 32768 tokens took 38 us.
+// Up to 32768 tokens masses are read once and stay in shared memory, beyond that four times; one CTA for 32768 tokens took 38 us.
 // move_kernel: a kept row only moves towards the front (its new place j <= its old place) and the places ascend,
 // so a CTA that owns one column slice of one (sequence, KV head) may go through the rows in chunks in place: it loads a whole
 // chunk, meets at a barrier, and stores it.  What later chunks still have to read lies at or behind their own places,
 // in front of which the stores of this chunk end: the next chunk's loads are in flight while this one is stored, and one
 // barrier a chunk is enough.  Bound by HBM: every row that moves is read once and written once.
 //
-// Measured (B200, the whole call): 32 sequences x 2 heads from 1104 to 1088 tokens (135 MB) 43 us, selection 12 and move 26 (20.6
-// at the HBM's rate); 8 x 2 heads from up to 32768 to 4096 60 us, selection 28 and move 27.
+// Measured (B200, the whole call): 32 sequences x 2 heads from 1104 to 1088 tokens (135 MB) 41 us, selection 11 and move 26 (20.6
+// at the HBM's rate); 8 x 2 heads from up to 32768 to 4096 53 us, selection 22 and move 27.  (With masses read once a digit, a
+// second meeting a digit and places written by the threads that found them: 43 and 60 us.)
 #include "cache_ops.cuh"
 #include "ptx.cuh"
 
@@ -83,10 +84,13 @@ __device__ __forceinline__ uint32_t peer_load(const uint32_t* mine, uint32_t ran
 }
 
 __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParams p, int C) {
-  __shared__ uint32_t hist[2048], hist_all[2048];          // this CTA's counts, the cluster's
+  __shared__ uint32_t hist[2048], hist_all[5120];          // this CTA's counts; the cluster's, for each of the three digits
+  __shared__ float vals[kChunk];                           // masses of this CTA's tokens of a round
   __shared__ uint32_t warp_sums[32];
   __shared__ uint32_t s_digit, s_left, s_count, s_counts[kMaxCluster], s_first;
-  const int unit = blockIdx.x / C, b = unit / p.Hkv, tid = threadIdx.x;
+  uint16_t* list = reinterpret_cast<uint16_t*>(hist);      // when the digits are known: tokens that stay, from the round's first
+  static_assert(kChunk * sizeof(uint16_t) <= sizeof(hist) && kChunk <= 65536, "list");
+  const int unit = blockIdx.x / C, b = unit / p.Hkv, h = unit - b * p.Hkv, tid = threadIdx.x;
   const uint32_t rank = blockIdx.x - unit * C;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   auto meet = [&]() {
@@ -96,7 +100,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParam
   };
   int n = p.kv_len[b];
   if (n < 0 || n > p.N) {
-    if (tid == 0 && unit == b * p.Hkv && rank == 0) atomicExch(p.status, kStatusCacheLen);
+    if (tid == 0 && h == 0 && rank == 0) atomicExch(p.status, kStatusCacheLen);
     n = n < 0 ? 0 : p.N;
   }
   const float* mass = p.mass + (long long)unit * p.mass_stride;
@@ -118,18 +122,38 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParam
   const int lo = p.sinks, hi = n - p.recent;
   uint32_t need = (uint32_t)(p.budget - p.sinks - p.recent);
   if (tid == 0) s_first = (uint32_t)left;
+  // A round is C * span tokens, CTA r of the cluster has the r-th span of it, a thread `per` of these in a row.  Up to
+  // 4096 tokens a CTA there is one round, and the masses are read once.
+  const int even = ((n - 1) / stride + 1) * kSelThreads, span = even < kChunk ? even : kChunk, per = span / kSelThreads;
+  const bool once = n <= C * span;
+  auto fetch = [&](int base) {                              // this thread reads back what it has written
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int i = base + (int)rank * span + k * kSelThreads + tid;
+      if (k < per) vals[k * kSelThreads + tid] = i < n ? mass[i] : 0.f;
+    }
+  };
+  if (once) fetch(0);
   // ---- the need-th largest key of [lo, hi), digit by digit ----
   uint32_t threshold = 0, mask = 0;
   if (need > 0) {
-    for (int i = tid; i < 2048; i += kSelThreads) hist[i] = hist_all[i] = 0;
+    for (int i = tid; i < 2048; i += kSelThreads) hist[i] = 0;
+    for (int i = tid; i < 5120; i += kSelThreads) hist_all[i] = 0;
     meet();
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048, per = bins / kSelThreads;
-#pragma unroll 8
-      for (int i = lo + all; i < hi; i += stride) {
-        const uint32_t key = order_key(mass[i]);
-        if ((key & mask) == threshold) atomicAdd(&hist[(key >> shift) & (bins - 1)], 1u);
+      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048, bins_thread = bins / kSelThreads;
+      uint32_t* sums = hist_all + pass * 2048;
+      uint32_t* mine = C > 1 ? hist : sums;
+      for (int base = 0; base < n; base += C * span) {
+        if (!once) fetch(base);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+          const int i = base + (int)rank * span + k * kSelThreads + tid;
+          if (k >= per || i < lo || i >= hi) continue;
+          const uint32_t key = order_key(vals[k * kSelThreads + tid]);
+          if ((key & mask) == threshold) atomicAdd(&mine[(key >> shift) & (bins - 1)], 1u);
+        }
       }
       if (C > 1) {
         // Masses have few leading digits: a CTA adds its few counts to every CTA's sums.  (Each thread reading its bins
@@ -137,120 +161,112 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParam
         __syncthreads();
         for (int i = tid; i < bins; i += kSelThreads) {
           const uint32_t c = hist[i];
-          if (c)
-            for (int r = 0; r < C; ++r) peer_add(&hist_all[i], r, c);
+          if (c) {
+            for (int r = 0; r < C; ++r) peer_add(&sums[i], r, c);
+            hist[i] = 0;
+          }
         }
       }
       meet();
       // from the top: the digit in which the running count reaches `need`; thread 0 has the highest of 4 or 2 bins a thread
-      uint32_t* sums = C > 1 ? hist_all : hist;
-      const int top = bins - 1 - tid * per;
+      const int top = bins - 1 - tid * bins_thread;
       uint32_t c[4], total;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) c[j] = j < per ? sums[top - j] : 0u;
+      for (int j = 0; j < 4; ++j) c[j] = j < bins_thread ? sums[top - j] : 0u;
       uint32_t before = block_prefix(c[0] + c[1] + c[2] + c[3], total, warp_sums);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (before < need && need <= before + c[j]) { s_digit = top - j; s_left = need - before; }
         before += c[j];
       }
-      for (int i = tid; i < 2048; i += kSelThreads) hist[i] = hist_all[i] = 0;     // all threads have read theirs
-      meet();
+      __syncthreads();
       threshold |= s_digit << shift;
       mask |= (uint32_t)(bins - 1) << shift;
       need = s_left;
-      __syncthreads();
     }
   }
   const uint32_t equals = need;                          // how many tokens equal to the threshold stay
   const bool any = p.budget > p.sinks + p.recent;
-  // ---- kept places, ascending: CTA r of the cluster takes chunk r of every round, a thread kPer tokens in a row ----
-  uint32_t done = 0, eq_done = 0;
-  for (int base = 0; base < n; base += C * kChunk) {
-    const int i0 = base + (int)rank * kChunk + tid * kPer;
-    float w[kPer];
+  // ---- kept places, ascending ----
+  uint32_t done = 0, eq_done = 0, first = 0xffffffffu;
+  for (int base = 0; base < n; base += C * span) {
+    const int from = base + (int)rank * span;
+    if (!once) fetch(base);
+    __syncthreads();
     uint32_t sure = 0, eq = 0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) w[j] = i0 + j < n ? mass[i0 + j] : 0.f;
-#pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      const int i = i0 + j;
-      if (i >= n) continue;
+      const int at = tid * per + j, i = from + at;
+      if (j >= per || i >= n) continue;
       if (i < lo || i >= hi) sure |= 1u << j;
       else if (any) {
-        const uint32_t key = order_key(w[j]);
+        const uint32_t key = order_key(vals[at]);
         sure |= key > threshold ? 1u << j : 0u;
         eq |= key == threshold ? 1u << j : 0u;
       }
     }
-    uint32_t total;                                       // both counts of a chunk are at most 4096
+    uint32_t total;                                       // both counts of a span are at most 4096
     const uint32_t at = block_prefix(__popc(sure) | (__popc(eq) << 16), total, warp_sums);
     if (tid == 0) s_count = total;
-    meet();                                               // every CTA has read its chunk and counted
+    meet();                                               // every CTA has read its span and counted
     if (tid < C) s_counts[tid] = C == 1 ? total : peer_load(&s_count, tid);
     __syncthreads();
-    uint32_t sure_at = done + (at & 0xffffu), eq_at = eq_done + (at >> 16);
+    uint32_t cta_sure = done, cta_eq = eq_done;
     for (int r = 0; r < C; ++r) {
       const uint32_t c = s_counts[r];
-      if (r < (int)rank) { sure_at += c & 0xffffu; eq_at += c >> 16; }
+      if (r < (int)rank) { cta_sure += c & 0xffffu; cta_eq += c >> 16; }
       done += c & 0xffffu;
       eq_done += c >> 16;
     }
-    uint32_t first = 0xffffffffu;
-    int slot[kPer];
-    int page_from[kPer], page_to[kPer];
+    // What stays of a span goes to places in a row: first into a list, so that the rows are shared out evenly below (few threads
+    // have many, where much stays; most have none, where little does).
+    auto place = [&](uint32_t n_sure, uint32_t n_eq) { return n_sure + (n_eq < equals ? n_eq : equals); };
+    const uint32_t slot0 = place(cta_sure, cta_eq), slot1 = place(cta_sure + (total & 0xffffu), cta_eq + (total >> 16));
+    uint32_t sure_at = cta_sure + (at & 0xffffu), eq_at = cta_eq + (at >> 16);
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      const bool e = (eq >> j) & 1u, on = ((sure >> j) & 1u) || (e && eq_at < equals);
-      slot[j] = on ? (int)(sure_at + (eq_at < equals ? eq_at : equals)) : -1;
-      if (on && slot[j] != i0 + j && (uint32_t)slot[j] < first) first = (uint32_t)slot[j];
-      sure_at += (sure >> j) & 1u;
+      const bool s = (sure >> j) & 1u, e = (eq >> j) & 1u;
+      if (s || (e && eq_at < equals)) list[place(sure_at, eq_at) - slot0] = (uint16_t)(tid * per + j);
+      sure_at += s;
       eq_at += e;
     }
+    __syncthreads();
     // Addresses are looked up here, once a row, and not by every thread that moves a part of it.
-    const int h = unit - b * p.Hkv;
-    if (p.page_table) {
-      const int32_t* table = p.page_table + (long long)b * p.max_pages;
-#pragma unroll
-      for (int j = 0; j < kPer; ++j)
-        if (slot[j] >= 0) {
-          page_from[j] = table[p.by_page(i0 + j)];
-          page_to[j] = table[p.by_page(slot[j])];
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      if (slot[j] < 0) continue;
-      if (kept) kept[slot[j]] = i0 + j;
-      mass_out[slot[j]] = w[j];                           // slot <= token, and this round has been read
+    const int32_t* table = p.page_table ? p.page_table + (long long)b * p.max_pages : nullptr;
+#pragma unroll 2
+    for (int slot = (int)slot0 + tid; slot < (int)slot1; slot += kSelThreads) {
+      const int at = list[slot - slot0], i = from + at;
+      if (kept) kept[slot] = i;
+      mass_out[slot] = vals[at];                          // slot <= token, and this round has been read
       longlong2 at2 = make_longlong2(-1, -1);
-      if (slot[j] != i0 + j) {
-        if (!p.page_table) {
-          const long long base = ((long long)b * p.Hkv + h) * p.N;
-          at2 = make_longlong2((base + i0 + j) * p.row_bytes, (base + slot[j]) * p.row_bytes);
-        } else if ((unsigned)page_from[j] >= (unsigned)p.num_pages || (unsigned)page_to[j] >= (unsigned)p.num_pages) {
-          atomicExch(p.status, kStatusKvRange);           // a page outside the pool: the row is skipped
+      if (slot != i) {
+        if ((uint32_t)slot < first) first = (uint32_t)slot;
+        if (!table) {
+          const long long row = (long long)unit * p.N;
+          at2 = make_longlong2((row + i) * p.row_bytes, (row + slot) * p.row_bytes);
         } else {
-          const int rf = i0 + j - p.by_page(i0 + j) * p.page_tokens, rt = slot[j] - p.by_page(slot[j]) * p.page_tokens;
-          at2 = make_longlong2((((long long)page_from[j] * p.Hkv + h) * p.page_tokens + rf) * p.row_bytes,
-                               (((long long)page_to[j] * p.Hkv + h) * p.page_tokens + rt) * p.row_bytes);
+          const int page_i = p.by_page(i), page_s = p.by_page(slot), pf = table[page_i], pt = table[page_s];
+          if ((unsigned)pf >= (unsigned)p.num_pages || (unsigned)pt >= (unsigned)p.num_pages) {
+            atomicExch(p.status, kStatusKvRange);         // a page outside the pool: the row is skipped
+          } else {
+            at2 = make_longlong2((((long long)pf * p.Hkv + h) * p.page_tokens + i - page_i * p.page_tokens) * p.row_bytes,
+                                 (((long long)pt * p.Hkv + h) * p.page_tokens + slot - page_s * p.page_tokens) * p.row_bytes);
+          }
         }
       }
-      places[slot[j]] = at2;
+      places[slot] = at2;
     }
-    first = __reduce_min_sync(0xffffffffu, first);
-    if ((tid & 31) == 0 && first < s_first) atomicMin(&s_first, first);
-    meet();                                               // the counts are used again
+    if (!once) meet();                                    // the counts, the masses and the list are used again
   }
+  first = __reduce_min_sync(0xffffffffu, first);
+  if ((tid & 31) == 0 && first != 0xffffffffu) atomicMin(&s_first, first);
   for (int i = left + all; i < n; i += stride) mass_out[i] = 0.f;
+  meet();
   // the first row that moves
-  if (tid == 0 && rank == 0) {
-    uint32_t first = s_first;
-    for (int r = 1; r < C; ++r) {
-      const uint32_t x = peer_load(&s_first, r);
-      first = x < first ? x : first;
-    }
-    p.moves[unit] = make_int2(left, (int)first);
+  if (rank == 0 && tid < 32) {
+    uint32_t x = tid < C ? (C == 1 ? s_first : peer_load(&s_first, tid)) : 0xffffffffu;
+    x = __reduce_min_sync(0xffffffffu, x);
+    if (tid == 0) p.moves[unit] = make_int2(left, (int)x);
   }
   meet();                                                 // no CTA leaves while another reads its shared memory
 }
