@@ -23,8 +23,8 @@
 //   D = 256, G = 8) and decode_finish_kernel turns them into weights when every head's sum is known: reading K a second
 //   time would cost sixteen times as much.
 //
-// Measured (B200, the whole call; of the 6.57 TB/s that a copy reaches): 8 sequences of 30 to 102 thousand tokens at D = 256
-// 188 us (0.94); 32 of 3 to 8 thousand with weights 78 us (0.71: the main kernel is at 0.86, the rest is the second launch and
+// Measured (B200, the whole call; of the 6.57 TB/s that a copy reaches): 8 sequences of 34 to 102 thousand tokens at D = 256
+// 189 us (0.94); 32 of 3 to 8 thousand with weights 78 us (0.71: the main kernel is at 0.86, the rest is the second launch and
 // the scores); 64 sequences x 8 KV heads at D = 128 with a window of 1024 and 64 sinks 58 us (0.75); one sequence of
 // 517 tokens 18 us, bound by the host (12 us of kernels).
 #include <type_traits>
