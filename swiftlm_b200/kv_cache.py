@@ -136,7 +136,10 @@ class PagedKVCache:
     def attend_prompt(self, queries: torch.Tensor, scale: float, q_len: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0,
                       return_lse: bool = False, out: Optional[torch.Tensor] = None):
         """Attention of the committed tokens' last rows, queries [B,Hq,T,D] (after extend(), or a commit): row r of sequence b is
-        token kv_len[b] - q_len[b] + r (q_len int32[B]; default T)."""
+        token kv_len[b] - q_len[b] + r (q_len int32[B]; default T).  Not between append_block() and commit(): the block's own
+        rows would be taken for the tokens in front of it."""
+        if self._appended:
+            raise RuntimeError("attend_prompt() between append_block() and commit()")
         return kernels.prompt_sdpa(queries, self.k_pool, self.v_pool, scale, q_len=q_len, kv_len=self.kv_len, page_table=self.page_table,
                                    window=window, sinks=sinks, return_lse=return_lse, out=out, n_max=self._n_max())
 
@@ -145,6 +148,8 @@ class PagedKVCache:
         """Adds the weights of attend_prompt()'s rows (all of them, or the last ones) to the mass."""
         if self.mass is None:
             raise RuntimeError("the cache was made without track_mass")
+        if self._appended:
+            raise RuntimeError("add_mass() between append_block() and commit()")
         kernels.attention_mass(queries, self.k_pool, lse, scale, self.mass, q_len=q_len, kv_len=self.kv_len, page_table=self.page_table,
                                window=window, sinks=sinks, n_max=self._n_max())
 
