@@ -171,11 +171,11 @@ class PagedKVCache:
 
     def sync(self) -> np.ndarray:
         """Reads the committed lengths (one device-to-host copy), tightens the host bounds and returns the pages
-        beyond every sequence's committed length to the pool."""
+        beyond every sequence's committed length, and beyond a block that waits for commit(), to the pool."""
         lens = self.kv_len.cpu().numpy()
         for b in range(self.B):
             self._upper[b] = int(lens[b])
-            self._shrink(b, self._upper[b])
+            self._shrink(b, self._upper[b] + self._appended)
         self._flush_table()
         return lens
 

@@ -47,3 +47,17 @@ def test_attention_over_the_committed_tokens_is_refused_between_append_and_commi
     cache.attend_prompt(q, 1.0)
     cache.add_mass(q, lse, 1.0)
     assert [c[0] for c in cache.calls] == ["prompt_sdpa", "attention_mass"] * 2
+
+
+def test_sync_between_append_and_commit_keeps_the_pages_of_the_block(cache):
+    cache.extend(rows(4), rows(4), [4, 3])
+    cache.extend(rows(4), rows(4), [2, 1])          # upper bounds 8 and 8, committed 6 and 4
+    cache.append_block(rows(3), rows(3))            # rows 6 .. 8 and 4 .. 6: three and two pages
+    before = [cache.pages_of(b) for b in range(2)]
+    assert cache.sync().tolist() == [6, 4]
+    assert cache.pages_of(0) == before[0][:3] and cache.pages_of(1) == before[1][:2]
+    for b, n in enumerate((3, 2)):
+        assert cache.page_table[b, :n].tolist() == before[b][:n] and (cache.page_table[b, n:] == -1).all()
+    cache.commit(torch.tensor([3, 3], dtype=torch.int32))
+    assert cache.sync().tolist() == [9, 7]
+    assert len(cache.pages_of(0)) == 3 and len(cache.pages_of(1)) == 2
