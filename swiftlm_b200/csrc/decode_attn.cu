@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(Shape<D>::W * 32, Shape<D>::per_sm) decode_ker
         if (whole) {
           if (g < p.G) {
             const long long row = (long long)s.b * a.Hq + s.h * p.G + g;
-            const float inv = sum > 0.f ? 1.f / sum : 0.f;
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;     // 0: nothing was visible; NaN stays NaN
             T* dst = reinterpret_cast<T*>(a.out) + row * D + warp * (D / W) + (lane >> 2);
 #pragma unroll
             for (int k = 0; k < MT; ++k) {
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(Shape<D>::W * 32, Shape<D>::per_sm) decode_ker
               dst[k * 16 + 8] = from_f32<T>(o[k][t][i + 2] * inv);
             }
             if (warp == 0 && lane < 4) {
-              const float z = sum > 0.f ? m[t][i] + log2f(sum) : -INFINITY;
+              const float z = sum == 0.f ? -INFINITY : m[t][i] + log2f(sum);
               if (a.lse) a.lse[row] = z * kLn2;
               if (p.lse2) p.lse2[row] = z;
             }
@@ -457,12 +457,12 @@ __global__ void __launch_bounds__(kFinishThreads) decode_finish_kernel(const Dec
     if (j1 > j0 + p.heads) j1 = j0 + p.heads;
     auto store = [&](int j, float4 o, float top, float sum) {
       const long long row = (long long)b * a.Hq + h * p.G + gc * H + j;
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
       uint2 pk;
       pk.x = mma::pack<T>(o.x * inv, o.y * inv);
       pk.y = mma::pack<T>(o.z * inv, o.w * inv);
       *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + row * D + col * 4) = pk;
-      if (col == 0 && a.lse) a.lse[row] = sum > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+      if (col == 0 && a.lse) a.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
     };
     auto add = [&](int j, int r, float z, float4& o, float& sum) {
       const int sl = slot_of(info, r) * H + j;
@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(kFinishThreads) decode_finish_kernel(const Dec
           }
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          z = sum > 0.f ? top + log2f(sum) : -INFINITY;
+          z = sum == 0.f ? -INFINITY : top + log2f(sum);
         }
         if (lane == 0) zs[j] = z;
       }

@@ -1,0 +1,40 @@
+"""The cache operators where a row's softmax or a call's size leaves the ordinary path: queries that are no numbers, weights
+far below the largest, tables and loops that only large batches reach.  Plain forms in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_cache_attention import K, Problem
+
+pytestmark = pytest.mark.gpu
+INF, NAN = math.inf, math.nan
+
+
+# head dimension 64, 128, 256; one CTA for a unit, and units cut into pieces that are joined
+@pytest.mark.parametrize("D,N,page", [(64, 70, 0), (128, 300, 16), (256, 300, 64), (256, 30000, 0)])
+@pytest.mark.parametrize("value", [NAN, INF])
+def test_decode_of_a_query_that_is_no_number(D, N, page, value):
+    """Scores q.k of which one is NaN or +infinity have no softmax: out, lse and the weights of that head are NaN, and nothing of
+    it reaches another head's output."""
+    B, Hq, Hkv = 2, 6, 2
+    x = Problem(B, Hq, Hkv, 1, D, N, "bf16", page, [N, max(1, N // 3)], seed=D + N)
+    q = x.q[:, :, 0].clone()
+    q[0, 1, 3] = value                                    # a head of KV head 0 of sequence 0
+    cap = N if not page else x.table.shape[1] * page
+    mass, clean_mass = (torch.full((B, Hkv, cap), 0.25, device="cuda") for _ in range(2))
+    window = 40 if N < 1000 else 20000
+    args = dict(kv_len=x.kv_len, page_table=x.table, window=window, sinks=3)
+    clean, clean_lse = K().decode_sdpa(x.q[:, :, 0], x.k, x.v, x.scale, mass=clean_mass, return_lse=True, **args)
+    got, lse = K().decode_sdpa(q, x.k, x.v, x.scale, mass=mass, return_lse=True, **args)
+    K().device_status()
+    hit = torch.zeros(B, Hq, dtype=torch.bool, device="cuda")
+    hit[0, 1] = True
+    assert torch.isnan(got[hit]).all() and torch.isnan(lse[hit]).all()
+    assert torch.equal(got[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit])
+    n = torch.arange(cap, device="cuda")
+    seen = (n < N) & ((n >= N - window) | (n < 3))
+    assert torch.isnan(mass[0, 0, seen]).all()
+    keep = torch.ones_like(mass, dtype=torch.bool)
+    keep[0, 0] = ~seen
+    assert torch.equal(mass[keep], clean_mass[keep])
