@@ -530,7 +530,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       }
       constexpr int kCols = D / 2;
       const int c0 = grp * kCols;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = l == 0.f ? 0.f : 1.f / l;             // 0: nothing was visible; NaN stays NaN
 #pragma unroll 1
       for (int c = 0; c < kCols; c += 32) {
         uint32_t o[32];
@@ -561,7 +561,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       ptx::tc_fence_before();              // the next segment's first half of P says that the accumulator has been read
       if (grp == 0) {
         if (s.slot >= 0) p.part_ml[(long long)s.slot * 256 + tile * 128 + r] = make_float2(m * p.scale_log2, l);
-        else if (used && a.lse) a.lse[row] = l > 0.f ? (m * p.scale_log2 + log2f(l)) * kLn2 : -INFINITY;
+        else if (used && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m * p.scale_log2 + log2f(l)) * kLn2;
       }
     }
   }
@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(128) join_kernel(const PromptParams p) {
       o[k].x = fmaf(w, v.x, o[k].x); o[k].y = fmaf(w, v.y, o[k].y); o[k].z = fmaf(w, v.z, o[k].z); o[k].w = fmaf(w, v.w, o[k].w);
     }
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint4 x[2];
   uint32_t* xp = reinterpret_cast<uint32_t*>(x);
 #pragma unroll
@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(128) join_kernel(const PromptParams p) {
   uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.a.out) + row * D + col);
   dst[0] = x[0];
   dst[1] = x[1];
-  if (p.a.lse && blockIdx.z == 0 && warp == 0) p.a.lse[row] = sum > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+  if (p.a.lse && blockIdx.z == 0 && warp == 0) p.a.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }

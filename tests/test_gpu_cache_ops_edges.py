@@ -38,3 +38,29 @@ def test_decode_of_a_query_that_is_no_number(D, N, page, value):
     keep = torch.ones_like(mass, dtype=torch.bool)
     keep[0, 0] = ~seen
     assert torch.equal(mass[keep], clean_mass[keep])
+
+
+@pytest.mark.parametrize("Hq,Hkv,T,D,N,page,window,sinks", [
+    (4, 2, 70, 64, 90, 0, 0, 0),                           # whole units
+    (6, 2, 40, 128, 300, 16, 30, 3),
+    (4, 2, 130, 256, 300, 64, 0, 0),                       # a pair of CTAs
+    (4, 1, 9, 256, 30000, 0, 0, 0),                        # units cut into pieces
+    (4, 1, 9, 64, 30000, 0, 0, 0),
+])
+@pytest.mark.parametrize("value", [NAN, INF])
+def test_prompt_row_that_is_no_number(Hq, Hkv, T, D, N, page, window, sinks, value):
+    """out and lse of that row are NaN; every other row has the bits that it has without it."""
+    B = 2
+    x = Problem(B, Hq, Hkv, T, D, N, "bf16", page, [N, N - 5], seed=D + N)
+    q = x.q.clone()
+    rows = [(0, 1, T - 1), (1, Hq - 1, T // 2)]
+    hit = torch.zeros(B, Hq, T, dtype=torch.bool, device="cuda")
+    for b, h, t in rows:
+        q[b, h, t, 5] = value
+        hit[b, h, t] = True
+    args = dict(kv_len=x.kv_len, page_table=x.table, window=window, sinks=sinks, return_lse=True)
+    clean, clean_lse = K().prompt_sdpa(x.q, x.k, x.v, x.scale, **args)
+    got, lse = K().prompt_sdpa(q, x.k, x.v, x.scale, **args)
+    K().device_status()
+    assert torch.isnan(got[hit]).all() and torch.isnan(lse[hit]).all()
+    assert torch.equal(got[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit])
