@@ -243,6 +243,8 @@ int32_t dflash_kv_commit(int32_t* kv_len, const int32_t* commit, int32_t B, int3
  *              n <= p and (window == 0 or n > p - window or n < sinks).  window counts the query's own
  *              token.  A row that sees nothing has out = 0 and lse = -infinity.
  *   values     K and V rows [0, kv_len[b]) are finite; rows behind them are never used, whatever they hold.
+ *              Queries may be anything: a row with a score of NaN or +infinity has out, lse and the weights it gives NaN, and
+ *              changes no other row.  A row whose visible scores are all -infinity is like one that sees nothing.
  *   lse        fp32, natural logarithm of the sum of exp(scale * q.k) over the visible tokens.
  *   mass       fp32 [B,Hkv,mass_stride], mass_stride >= N: the weight every cached token has received, summed over
  *              the query heads of its KV head.  Always added to, in an order that does not change from run to run.
@@ -272,7 +274,8 @@ int32_t dflash_prompt_sdpa(const void* q, const void* k, const void* v, const in
 size_t dflash_prompt_sdpa_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t D, int32_t N);
 
 /* mass[b,h,n] += sum over query rows r and query heads of h of exp(scale * q.k - lse) on the tokens the rows see,
- * with the lse [B,Hq,T] of an attention over the same cache (a row whose lse is -infinity adds nothing). */
+ * with the lse [B,Hq,T] of an attention over the same cache (a row whose lse is -infinity adds nothing; one whose lse is NaN
+ * makes the masses of the tokens it sees NaN, and no others). */
 int32_t dflash_attention_mass(const void* q, const void* k, const int32_t* page_table, const int32_t* q_len,
                               const int32_t* kv_len, const float* lse, float* mass, void* workspace,
                               size_t workspace_bytes, int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t D, int32_t N,

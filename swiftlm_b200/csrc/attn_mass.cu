@@ -39,6 +39,7 @@ struct MassParams {
   int box, k_stages, q_stages; // stages of keys and of queries in shared memory
   float scale_log2;
   float* part;                 // [2 * grid][256]
+  int* nan_seen;               // a row in use has an lse of NaN
 };
 
 // One step: a key tile against a query tile.
@@ -103,6 +104,7 @@ __device__ __forceinline__ int next_unit(const CacheArgs& a, RowLens len, int u,
 
 __global__ void __launch_bounds__(1024) mass_plan_kernel(const MassParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) *p.nan_seen = 0;
   plan_ranges<kUnitCost>(p.ranges, p.a, [&](RowLens len, int u) { return unit_steps(p.a, p.t, len, u); });
 }
 
@@ -158,6 +160,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + C::bars);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + C::misc + 4);
+  int* nan_flag = reinterpret_cast<int*>(sm + C::misc + 8);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
     ptx::prefetch_tensormap(&map_q);
@@ -166,6 +169,7 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
       ptx::mbar_init(&bars[i], (i >= C::b_s_free && i < C::b_z_full) || i >= C::b_meet ? kSumWarps / 2 : (i >= C::b_z_free && i < C::b_step ? kSumWarps : 1));
     *abort_flag = (ptx::smem_u32(sm) & 1023u) != 0u;      // swizzled tiles need 1024-byte alignment; never seen violated
     if (*abort_flag) atomicExch(a.status, kStatusSmemAlign);
+    *nan_flag = 0;
     ptx::fence_mbar_init();
   }
   // rows of a query tile behind Gt * Tt are never loaded: zeros, so that their scores are numbers
@@ -302,7 +306,10 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
           have += more;
         }
         if (n >= kBuffers) ok = wait(C::b_z_free + k, (n / kBuffers - 1) & 1);
-        float4 x;                                             // neither do rows that see nothing: their lse is -infinity
+        // Neither do rows that see nothing (their lse is -infinity), nor those whose lse is NaN: it would reach the keys that the
+        // row does not see, by way of their score of -infinity.  mass_join_kernel marks what such rows see.
+        if (v[k][0] != v[k][0] || v[k][1] != v[k][1] || v[k][2] != v[k][2] || v[k][3] != v[k][3]) *nan_flag = 1;
+        float4 x;
         x.x = v[k][0] > -INFINITY ? -v[k][0] * kLog2e : -INFINITY;
         x.y = v[k][1] > -INFINITY ? -v[k][1] * kLog2e : -INFINITY;
         x.z = v[k][2] > -INFINITY ? -v[k][2] * kLog2e : -INFINITY;
@@ -443,21 +450,51 @@ mass_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ C
   }
   __syncwarp();
   __syncthreads();
+  if (threadIdx.x == 0 && *nan_flag) *p.nan_seen = 1;
   if (*abort_flag) __nanosleep(100000);        // copies that were still in flight land before the memory is given back
   if (warp == 2) ptx::tmem_dealloc(tmem, 512);
 }
 
-// adds up the pieces of a cut unit, in order
+// does a row that sees key n of (b, h) have an lse of NaN?
+__device__ __forceinline__ bool nan_row(const MassParams& p, int b, int h, RowLens len, int n) {
+  const CacheArgs& a = p.a;
+  const int past = len.keys - len.rows, first = n > past ? n - past : 0;
+  int end = len.rows;
+  if (a.window > 0 && n >= a.sinks && n + a.window - past < end) end = n + a.window - past;
+  const float* lse = a.lse + ((long long)b * a.Hq + h * p.t.G) * a.T;
+  for (int g = 0; g < p.t.G; ++g, lse += a.T)
+    for (int i = first; i < end; ++i)
+      if (lse[i] != lse[i]) return true;
+  return false;
+}
+
+// Adds up the pieces of a cut unit, in order.  Where some row has an lse of NaN, which a working program never meets, every key
+// is looked at again here, for all rows that see it: done by the summing threads of mass_kernel it cost every call 2 to 5 %
+// (387 to 400 us for 381 in 2048 rows over 16384 tokens, with bits of such rows beside each step's log-sum-exps or a flag a unit; 385 so).
 __global__ void __launch_bounds__(kUnitKeys) mass_join_kernel(const MassParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Cut cut = p.ranges.cuts[blockIdx.x];
-  if (cut.count == 0) return;
-  const Cursor c(p.ranges, p.a, cut.unit);
-  const int n = c.u * kUnitKeys + threadIdx.x;
-  if (n >= c.len.keys) return;
-  float total = 0.f;
-  for (int i = 0; i < cut.count; ++i) total += p.part[(long long)piece_slot(cut, i) * kUnitKeys + threadIdx.x];
-  p.a.mass[((long long)c.b * p.a.Hkv + c.hg) * p.a.mass_stride + n] += total;
+  const bool nan = *p.nan_seen != 0;
+  auto at = [&](const Cursor& c, int n) { return p.a.mass + ((long long)c.b * p.a.Hkv + c.hg) * p.a.mass_stride + n; };
+  if (cut.count > 0) {
+    const Cursor c(p.ranges, p.a, cut.unit);
+    const int n = c.u * kUnitKeys + threadIdx.x;
+    if (n < c.len.keys) {
+      float total = 0.f;
+      for (int i = 0; i < cut.count; ++i) total += p.part[(long long)piece_slot(cut, i) * kUnitKeys + threadIdx.x];
+      if (nan && nan_row(p, c.b, c.hg, c.len, n)) total = __int_as_float(0x7fffffff);
+      *at(c, n) += total;
+    }
+  }
+  if (!nan) return;
+  const long long units = (long long)p.a.B * p.a.Hkv * p.ranges.per_row;
+  for (long long unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    bool is_cut = false;                       // another block adds to it
+    for (int i = 0; i < p.ranges.grid; ++i) is_cut |= p.ranges.cuts[i].count > 0 && p.ranges.cuts[i].unit == unit;
+    const Cursor c(p.ranges, p.a, unit);
+    const int n = c.u * kUnitKeys + threadIdx.x;
+    if (!is_cut && n < c.len.keys && nan_row(p, c.b, c.hg, c.len, n)) *at(c, n) = __int_as_float(0x7fffffff);
+  }
 }
 
 struct Plan { Tiling t; int per_row, grid; size_t total; };
@@ -468,7 +505,7 @@ Plan plan_of(int B, int Hq, int Hkv, int T, int N) {
   const long long tiles = (long long)B * Hkv * x.per_row * x.t.GC * ((T + x.t.Tt - 1) / x.t.Tt);
   const int n_sm = sm_count(), most = n_sm < kMaxGrid ? n_sm : kMaxGrid;
   x.grid = (int)(tiles < most ? tiles : most);
-  x.total = ranges_bytes(B, x.per_row, x.grid) + (size_t)2 * x.grid * kUnitKeys * 4;
+  x.total = ranges_bytes(B, x.per_row, x.grid) + (size_t)2 * x.grid * kUnitKeys * 4 + 16;
   return x;
 }
 
@@ -487,6 +524,7 @@ int32_t launch_typed(const CacheArgs& a, cudaStream_t stream) {
   p.k_stages = C::stages - p.q_stages;
   p.scale_log2 = a.scale * kLog2e;
   p.part = reinterpret_cast<float*>(ranges_at(p.ranges, reinterpret_cast<uint8_t*>(a.workspace)));
+  p.nan_seen = reinterpret_cast<int*>(p.part + (size_t)2 * x.grid * kUnitKeys);
   CUtensorMap mq, mk;
   CUresult r = encode_q(&mq, a, x.t);
   if (r == CUDA_SUCCESS) r = encode_kv(&mk, a.k, a, p.box);

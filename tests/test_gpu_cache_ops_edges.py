@@ -64,3 +64,37 @@ def test_prompt_row_that_is_no_number(Hq, Hkv, T, D, N, page, window, sinks, val
     K().device_status()
     assert torch.isnan(got[hit]).all() and torch.isnan(lse[hit]).all()
     assert torch.equal(got[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit])
+
+
+@pytest.mark.parametrize("Hq,Hkv,T,D,N,page,window,sinks", [
+    (4, 2, 70, 64, 90, 0, 0, 0),
+    (6, 2, 40, 128, 300, 16, 30, 3),
+    (3, 1, 16, 256, 700, 64, 0, 0),                        # 126 rows of a query tile in use
+    (4, 1, 300, 128, 5000, 0, 0, 0),                       # several query tiles, units cut into pieces
+    (160, 1, 5, 64, 400, 0, 100, 7),                       # two groups of heads
+])
+@pytest.mark.parametrize("case", ["lse", NAN, INF])
+def test_mass_of_a_row_that_is_no_number(Hq, Hkv, T, D, N, page, window, sinks, case):
+    """A log-sum-exp that is NaN (given as such, or that of a query with a NaN or an infinity) makes the masses of the tokens
+    that the row sees NaN; all other masses have the bits that they have without it."""
+    B = 2
+    x = Problem(B, Hq, Hkv, T, D, N, "f16", page, [N, N - 5], seed=D + N)
+    args = dict(kv_len=x.kv_len, page_table=x.table, window=window, sinks=sinks)
+    lse = K().prompt_sdpa(x.q, x.k, x.v, x.scale, return_lse=True, **args)[1]
+    cap = N if not page else x.table.shape[1] * page
+    clean, mass = (torch.full((B, Hkv, cap), 0.5, device="cuda") for _ in range(2))
+    K().attention_mass(x.q, x.k, lse, x.scale, clean, **args)
+    q, bad_lse = x.q.clone(), lse.clone()
+    hit = torch.zeros(B, Hkv, cap, dtype=torch.bool, device="cuda")
+    for b, h, t in [(0, 1, T // 2), (1, Hq - 1, T - 2)]:
+        if case == "lse":
+            bad_lse[b, h, t] = NAN
+        else:
+            q[b, h, t, 5] = case
+        hit[b, h // (Hq // Hkv), :x.kv[b]] |= x.seen(b, window, sinks)[t]
+    if case != "lse":
+        bad_lse = K().prompt_sdpa(q, x.k, x.v, x.scale, return_lse=True, **args)[1]
+    K().attention_mass(q, x.k, bad_lse, x.scale, mass, **args)
+    K().device_status()
+    assert torch.isnan(mass[hit]).all()
+    assert torch.equal(mass[~hit], clean[~hit])
