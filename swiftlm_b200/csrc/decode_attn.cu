@@ -16,7 +16,8 @@
 //   nothing.  The W warps agree on the tile's maxima through shared memory, write P as 16-bit rows, and each warp then
 //   owns D / W rows of O^T = V^T P^T for all the tile's keys: one accumulator per CTA, no merge of warps, two
 //   barriers a tile.  O is rescaled only when a maximum grows by more than 2^8 (its scale is exact in fp32).
-//   P is rounded to the inputs' type (the sum of the weights is not): the product needs a 16-bit operand.
+//   P is rounded to the inputs' type (the sum of the weights is not): the product needs a 16-bit operand (f16: lifted
+//   first, mma_sync.cuh).
 // * A unit that one CTA covers is normalised and written at once; the others leave (O, maximum, sum) in the workspace
 //   and decode_finish_kernel, chained by a programmatic launch, joins them in a fixed order.
 // * With `mass`, the scaled scores of the visible tokens are kept (4 bytes per head and key, 3 % of the bytes read at
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(Shape<D>::W * 32, Shape<D>::per_sm) decode_ker
         }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const float z0 = m[t][0] == -INFINITY ? 0.f : m[t][0], z1 = m[t][1] == -INFINITY ? 0.f : m[t][1];
+        const float z0 = m[t][0] == -INFINITY ? 0.f : m[t][0] - mma::kLift<T>, z1 = m[t][1] == -INFINITY ? 0.f : m[t][1] - mma::kLift<T>;
         const float w0 = mma::exp2_approx(x[t][0] - z0), w1 = mma::exp2_approx(x[t][1] - z1);
         const float w2 = mma::exp2_approx(x[t][2] - z0), w3 = mma::exp2_approx(x[t][3] - z1);
         l[t][0] = l[t][0] * f[t][0] + (w0 + w2);
@@ -403,7 +404,7 @@ __global__ void __launch_bounds__(Shape<D>::W * 32, Shape<D>::per_sm) decode_ker
               dst[k * 16 + 8] = from_f32<T>(o[k][t][i + 2] * inv);
             }
             if (warp == 0 && lane < 4) {
-              const float z = sum == 0.f ? -INFINITY : m[t][i] + log2f(sum);
+              const float z = sum == 0.f ? -INFINITY : m[t][i] - mma::kLift<T> + log2f(sum);
               if (a.lse) a.lse[row] = z * kLn2;
               if (p.lse2) p.lse2[row] = z;
             }
@@ -416,7 +417,7 @@ __global__ void __launch_bounds__(Shape<D>::W * 32, Shape<D>::per_sm) decode_ker
             dst[k * 16 + 8] = o[k][t][i + 2];
           }
           if (warp == 0 && lane < 4) {
-            p.part_m[slot * H + j] = m[t][i];
+            p.part_m[slot * H + j] = m[t][i] - mma::kLift<T>;
             p.part_l[slot * H + j] = sum;
           }
         }

@@ -41,6 +41,12 @@ template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// Softmax weights 2^(s - m) are at most 2^8 (running maxima lag by that much) and become 16-bit operands.  In f16 they are
+// lifted by 2^7, which the sum of the weights cancels: what is lost begins at 2^-32 of the largest and not at 2^-25, where a
+// few thousand light tokens beside one heavy one still add up.  bf16 has the range of fp32.
+template <typename T> constexpr float kLift = 0.f;
+template <> constexpr float kLift<__half> = 7.f;
+
 __device__ __forceinline__ float exp2_approx(float x) {   // exp2(-inf) = +0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

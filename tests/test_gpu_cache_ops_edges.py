@@ -98,3 +98,32 @@ def test_mass_of_a_row_that_is_no_number(Hq, Hkv, T, D, N, page, window, sinks, 
     K().device_status()
     assert torch.isnan(mass[hit]).all()
     assert torch.equal(mass[~hit], clean[~hit])
+
+
+def light_tokens(B, T, D, N, seed):
+    """f16: token 0 takes nearly all of the weight and has no value; the others weigh 2^-26.5 of it each, all their values are in
+    [1, 2].  (q, k, v, out in 64 bits, bound).  Bound: half a step u of the output, its subnormal half step 2^-25, half a step u of
+    each weight and, for weights below the smallest normal one, half of 2^-24 at a lift of 2^7: 2^-32 each."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.zeros(B, 2, T, D, device="cuda", dtype=torch.float16)
+    k, v = (torch.zeros(B, 1, N, D, device="cuda", dtype=torch.float16) for _ in range(2))
+    q[..., 0] = 1.0
+    k[:, :, 0, 0] = 18.375
+    v[:, :, 1:] = (torch.rand(B, 1, N - 1, D, device="cuda", generator=g) + 1).half()
+    pos = torch.arange(N - T, N, device="cuda")
+    s = q.double() @ k.double().transpose(-1, -2)
+    w = s.masked_fill(torch.arange(N, device="cuda") > pos[:, None], -INF).softmax(-1)
+    out = w @ v.double()
+    u = 2.0 ** -11
+    return q, k, v, out, u * out + 2.0 ** -25 + u * out + 2.0 ** -32 * (pos[:, None] + 1) * 2 + 2.0 ** -20 * out
+
+
+# sequences that a CTA covers alone, and one that is cut: only the piece with the heavy token has light weights then
+@pytest.mark.parametrize("B,D,N", [(300, 64, 2000), (200, 128, 700), (200, 256, 1500), (1, 64, 60000)])
+def test_decode_keeps_light_f16_weights(B, D, N):
+    q, k, v, out, bound = light_tokens(B, 1, D, N, D)
+    got, lse = K().decode_sdpa(q[:, :, 0], k, v, 1.0, return_lse=True)
+    K().device_status()
+    assert ((got.double() - out[:, :, 0]).abs() <= bound[:, :, 0]).all()
+    want = math.log(math.exp(18.375) + N - 1)
+    assert ((lse.double() - want).abs() <= 2.0 ** -20 * want).all()
