@@ -14,7 +14,7 @@
 //   keys of a tile and half of the value columns.  One CTA alone would read 128 KiB of keys and
 //   values from L2 for each 128 x 128 tile: that ran at 4600 clocks a tile, waiting for L2 and for shared memory.
 // * Warps: 0 loads queries and keys, 1 values, 2 issues S = Q K^T, 3 issues O += P V (P replaces S in tensor memory,
-//   in the inputs' type: the product needs a 16-bit operand), the others softmax, two threads a row: with one
+//   in the inputs' type: the product needs a 16-bit operand; f16: lifted first, mma_sync.cuh), the others softmax, two threads a row: with one
 //   the row's 128 exponentials were a chain of 4000 clocks.
 // * Only the key tiles that some row of the unit sees are visited; only those that some row does not see whole are masked.
 //   Value rows behind the sequence's length are zeroed in shared memory before the product, whatever the cache holds there.
@@ -470,7 +470,7 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
           l *= f;
         }
         const bool rescale = j > s.lo && __any_sync(0xffffffffu, grow);
-        const float neg = m == -INFINITY ? 0.f : -m * p.scale_log2;
+        const float neg = m == -INFINITY ? 0.f : mma::kLift<T> - m * p.scale_log2;
         // the last product is done with the accumulator
         if (rescale) {
           constexpr int kCols = D / 2;
@@ -560,8 +560,8 @@ prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
       }
       ptx::tc_fence_before();              // the next segment's first half of P says that the accumulator has been read
       if (grp == 0) {
-        if (s.slot >= 0) p.part_ml[(long long)s.slot * 256 + tile * 128 + r] = make_float2(m * p.scale_log2, l);
-        else if (used && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m * p.scale_log2 + log2f(l)) * kLn2;
+        if (s.slot >= 0) p.part_ml[(long long)s.slot * 256 + tile * 128 + r] = make_float2(m * p.scale_log2 - mma::kLift<T>, l);
+        else if (used && a.lse) a.lse[row] = l == 0.f ? -INFINITY : (m * p.scale_log2 - mma::kLift<T> + log2f(l)) * kLn2;
       }
     }
   }

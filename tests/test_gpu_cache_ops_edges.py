@@ -127,3 +127,14 @@ def test_decode_keeps_light_f16_weights(B, D, N):
     assert ((got.double() - out[:, :, 0]).abs() <= bound[:, :, 0]).all()
     want = math.log(math.exp(18.375) + N - 1)
     assert ((lse.double() - want).abs() <= 2.0 ** -20 * want).all()
+
+
+@pytest.mark.parametrize("T,D,N", [(130, 64, 1000), (300, 128, 700), (140, 256, 1500), (2, 128, 1500)])
+def test_prompt_keeps_light_f16_weights(T, D, N):
+    """As many sequences as there are whole units to show it in."""
+    q, k, v, out, bound = light_tokens(40, T, D, N, D)
+    got, lse = K().prompt_sdpa(q, k, v, 1.0, return_lse=True)
+    K().device_status()
+    assert ((got.double() - out).abs() <= bound).all()
+    want = torch.log(math.exp(18.375) + torch.arange(N - T, N, device="cuda").double())
+    assert ((lse.double() - want).abs() <= 2.0 ** -20 * want).all()
