@@ -250,7 +250,7 @@ int32_t dflash_kv_commit(int32_t* kv_len, const int32_t* commit, int32_t B, int3
  *              the query heads of its KV head.  Always added to, in an order that does not change from run to run.
  *   scale      positive, 1e-30 .. 1e30.
  *   Supported: dtype bf16 / f16, D in {64, 128, 256}, Hq % Hkv == 0.  Neither outputs nor workspace may overlap
- *   another argument unless it is said.
+ *   another argument unless it is said (refused: DFLASH_ERR_INVALID_ARG); out may be q itself.
  */
 
 /* Attention of one new token per sequence (the last cached one):  q, out [B,Hq,D];  lse [B,Hq] or NULL;

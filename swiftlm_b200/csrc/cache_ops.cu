@@ -47,6 +47,18 @@ int32_t check_workspace(const char* op, const CacheArgs& a, size_t need) {
   return DFLASH_OK;
 }
 
+// Outputs and workspace against each other and the inputs.  out may be q itself: a unit's queries are read before its rows are
+// written, by the one CTA that has all of it or by the launch in front of the join.
+int32_t check_apart(const char* op, const CacheArgs& a, bool lse_written, size_t workspace) {
+  const unsigned long long rows = (unsigned long long)a.B * a.Hq * a.T, heads = (unsigned long long)a.B * a.Hkv, row_bytes = 2ull * a.D;
+  const unsigned long long kv = a.page_table ? (unsigned long long)a.num_pages * a.Hkv * a.page_tokens * row_bytes : heads * a.N * row_bytes;
+  const Span lse{a.lse, rows * 4}, none{nullptr, 0};
+  const Span s[] = {{a.out, rows * row_bytes}, {a.mass, ((heads - 1) * a.mass_stride + a.N) * 4}, {a.workspace, workspace}, lse_written ? lse : none,
+                    lse_written ? none : lse, {a.out == a.q ? nullptr : a.q, rows * row_bytes}, {a.k, kv}, {a.v, kv},
+                    {a.page_table, 4ull * a.B * a.max_pages}, {a.q_len, 4ull * a.B}, {a.kv_len, 4ull * a.B}};
+  return apart(s, 4) ? DFLASH_OK : invalid(op, "an output or the workspace overlaps another argument");
+}
+
 int32_t with_status(CacheArgs& a) {
   a.status = device_status_word();
   if (!a.status) { set_error("no CUDA device"); return DFLASH_ERR_CUDA; }
@@ -70,7 +82,9 @@ int32_t dflash_decode_sdpa(const void* q, const void* k, const void* v, const in
   CacheArgs a{q, k, v, page_table, nullptr, kv_len, out, lse, mass, workspace, workspace_bytes, B, Hq, Hkv, 1, D, N,
               page_tokens, max_pages, num_pages, mass_stride, window, sinks, scale, dtype, nullptr};
   if (int32_t st = check(op, a)) return st;
-  if (int32_t st = check_workspace(op, a, decode_workspace_bytes(B, Hq, Hkv, D, N, a.window, a.sinks, mass != nullptr))) return st;
+  const size_t need = decode_workspace_bytes(B, Hq, Hkv, D, N, a.window, a.sinks, mass != nullptr);
+  if (int32_t st = check_workspace(op, a, need)) return st;
+  if (int32_t st = check_apart(op, a, true, need)) return st;
   if (int32_t st = with_status(a)) return st;
   return launch_decode(a, reinterpret_cast<cudaStream_t>(stream));
 }
@@ -91,7 +105,9 @@ int32_t dflash_prompt_sdpa(const void* q, const void* k, const void* v, const in
   CacheArgs a{q, k, v, page_table, q_len, kv_len, out, lse, nullptr, workspace, workspace_bytes, B, Hq, Hkv, T, D, N,
               page_tokens, max_pages, num_pages, 0, window, sinks, scale, dtype, nullptr};
   if (int32_t st = check(op, a)) return st;
-  if (int32_t st = check_workspace(op, a, prompt_workspace_bytes(B, Hq, Hkv, T, D, N))) return st;
+  const size_t need = prompt_workspace_bytes(B, Hq, Hkv, T, D, N);
+  if (int32_t st = check_workspace(op, a, need)) return st;
+  if (int32_t st = check_apart(op, a, true, need)) return st;
   if (int32_t st = with_status(a)) return st;
   return launch_prompt(a, reinterpret_cast<cudaStream_t>(stream));
 }
@@ -111,7 +127,9 @@ int32_t dflash_attention_mass(const void* q, const void* k, const int32_t* page_
   CacheArgs a{q, k, nullptr, page_table, q_len, kv_len, nullptr, const_cast<float*>(lse), mass, workspace, workspace_bytes,
               B, Hq, Hkv, T, D, N, page_tokens, max_pages, num_pages, mass_stride, window, sinks, scale, dtype, nullptr};
   if (int32_t st = check(op, a)) return st;
-  if (int32_t st = check_workspace(op, a, mass_workspace_bytes(B, Hq, Hkv, T, D, N))) return st;
+  const size_t need = mass_workspace_bytes(B, Hq, Hkv, T, D, N);
+  if (int32_t st = check_workspace(op, a, need)) return st;
+  if (int32_t st = check_apart(op, a, false, need)) return st;
   if (int32_t st = with_status(a)) return st;
   return launch_mass(a, reinterpret_cast<cudaStream_t>(stream));
 }

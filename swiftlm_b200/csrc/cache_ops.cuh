@@ -53,6 +53,24 @@ __device__ __forceinline__ bool sees(const CacheArgs& a, int p, int n) {
   return n <= p && (a.window == 0 || n > p - a.window || n < a.sinks);
 }
 
+// A range of memory that a call reads or writes, for the refusal of calls that would read what they have written.
+struct Span {
+  const void* at;
+  unsigned long long bytes;
+  bool meets(const Span& o) const {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(at), b = reinterpret_cast<uintptr_t>(o.at);
+    return at && o.at && a < b + o.bytes && b < a + bytes;
+  }
+};
+// The first `written` of the spans meet none of the others?
+template <int N>
+inline bool apart(const Span (&s)[N], int written) {
+  for (int i = 0; i < written; ++i)
+    for (int j = i + 1; j < N; ++j)
+      if (s[i].meets(s[j])) return false;
+  return true;
+}
+
 // Dynamic shared memory of a kernel, set once per device (a driver call of a microsecond); `ready` belongs to the kernel.
 template <typename F>
 inline cudaError_t allow_shared(std::atomic<uint64_t>& ready, F kernel, int bytes) {

@@ -381,7 +381,8 @@ def decode_sdpa(queries, keys, values, scale: float, kv_len=None, page_table=Non
     [num_pages,Hkv,page_tokens,D] (page_tokens a multiple of 16); kv_len int32 [B]: cached tokens (0 for an unused place:
     its output is 0).  window > 0: the last `window` tokens are visible, and the first `sinks`.  mass fp32
     [B,Hkv,>= capacity]: the weight of every visible token, summed over the query heads of its KV head, is added to
-    it.  n_max: an upper bound of kv_len for a page pool, when less than the table's reach is in use.
+    it.  n_max: an upper bound of kv_len for a page pool, when less than the table's reach is in use.  out: a tensor like
+    queries, or queries itself.
     Returns [B,Hq,D], or (that, lse fp32 [B,Hq]) with return_lse.
     """
     _cache_tensors(queries, 3, keys, values, page_table, mass, out)

@@ -138,3 +138,23 @@ def test_prompt_keeps_light_f16_weights(T, D, N):
     assert ((got.double() - out).abs() <= bound).all()
     want = torch.log(math.exp(18.375) + torch.arange(N - T, N, device="cuda").double())
     assert ((lse.double() - want).abs() <= 2.0 ** -20 * want).all()
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,N,page", [(4, 2, 64, 300, 16), (8, 1, 128, 300, 0), (16, 2, 256, 20000, 0)])
+def test_output_in_place_of_the_queries(Hq, Hkv, D, N, page):
+    from swiftlm_b200 import _lib
+    x = Problem(2, Hq, Hkv, 150, D, N, "bf16", page, [N, N - 7], [150, 70], seed=D)
+    args = dict(q_len=x.q_len, kv_len=x.kv_len, page_table=x.table)
+    want = K().prompt_sdpa(x.q, x.k, x.v, x.scale, out=x.q.clone(), **args)
+    q = x.q.clone()
+    assert K().prompt_sdpa(q, x.k, x.v, x.scale, out=q, **args) is q and torch.equal(q, want)
+    one = x.q[:, :, 0].contiguous()
+    args.pop("q_len")
+    want = K().decode_sdpa(one, x.k, x.v, x.scale, **args)
+    assert K().decode_sdpa(one, x.k, x.v, x.scale, out=one, **args) is one and torch.equal(one, want)
+    both = torch.zeros(2 * one.numel(), dtype=x.dt, device="cuda")
+    launches = K().launch_count()
+    with pytest.raises(_lib.DFlashError):                  # half of it
+        K().decode_sdpa(both[:one.numel()].view_as(one), x.k, x.v, x.scale, out=both[D:D + one.numel()].view_as(one), **args)
+    assert K().launch_count() == launches
+    K().device_status()
