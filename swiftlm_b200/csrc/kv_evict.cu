@@ -357,6 +357,20 @@ extern "C" int32_t dflash_kv_evict(void* k_cache, void* v_cache, const int32_t* 
     set_error("kv_evict: workspace of %zu bytes needed, %zu given", need, workspace ? workspace_bytes : (size_t)0);
     return DFLASH_ERR_WORKSPACE;
   }
+  // kv_len_out and mass_out may be kv_len and mass; two arrays of masses may lie in each other's gaps
+  const unsigned long long heads = (unsigned long long)B * Hkv, mass_bytes = ((heads - 1) * mass_stride + N) * 4;
+  const unsigned long long kv = (page_table ? (unsigned long long)num_pages * Hkv * page_tokens : heads * N) * row_bytes;
+  const Span old{mass == mass_out ? nullptr : mass, mass_bytes};
+  const Span s[] = {{k_cache, kv}, {v_cache, kv}, {kv_len_out, 4ull * B}, {kept, heads * budget * 4}, {workspace, need}, {mass_out, mass_bytes},
+                    {kv_len == kv_len_out ? nullptr : kv_len, 4ull * B}, {page_table, 4ull * B * max_pages}};
+  bool ok = apart(s, 6);
+  for (int i = 0; i < 5; ++i) ok = ok && !s[i].meets(old);
+  if (s[5].meets(old)) {
+    const unsigned long long a = reinterpret_cast<uintptr_t>(mass), b = reinterpret_cast<uintptr_t>(mass_out), row = 4ull * mass_stride;
+    const unsigned long long off = (a < b ? b - a : a - b) % row;
+    ok = ok && off >= 4ull * N && row - off >= 4ull * N;
+  }
+  if (!ok) return invalid("an output or the workspace overlaps another argument");
   int* status = device_status_word();
   if (!status) { set_error("no CUDA device"); return DFLASH_ERR_CUDA; }
   EvictParams p{reinterpret_cast<uint8_t*>(k_cache), reinterpret_cast<uint8_t*>(v_cache), page_table, kv_len, mass, kv_len_out, mass_out,

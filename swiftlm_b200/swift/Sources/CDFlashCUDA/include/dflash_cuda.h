@@ -292,6 +292,7 @@ size_t dflash_attention_mass_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv,
  *              old length; nothing behind it is written.
  *   kept       int32 [B,Hkv,budget] or NULL: the old place of each row that stays, ascending; -1 behind the last.
  *   workspace  dflash_kv_evict_workspace_bytes() bytes, with or without `kept`.
+ * Outputs, caches and workspace that overlap another argument in any other way are refused.
  * k_cache / v_cache rows of any dtype of dflash_kv_append with D * size a multiple of 16 bytes; page_tokens any
  * positive number.  The pages of a sequence that is cut must belong to it alone (a page shared with another
  * sequence would change under it).  Rows on a page outside the pool are skipped and reported. */

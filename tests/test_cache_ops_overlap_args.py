@@ -28,7 +28,7 @@ def refused(op, **at):
     return call(op, **args) == _lib.ERR_INVALID_ARG and b"overlap" in _lib.lib().dflash_last_error_string()
 
 
-@pytest.mark.parametrize("op", ["decode", "prompt", "mass"])
+@pytest.mark.parametrize("op", ["decode", "prompt", "mass", "evict"])
 def test_overlapping_outputs_are_refused(op):
     for a, b in itertools.combinations(USED[op], 2):
         if not {a, b} & WRITTEN[op]:
@@ -37,3 +37,10 @@ def test_overlapping_outputs_are_refused(op):
             at = places()
             at[b] = at[a] + off
             assert refused(op, **at), (a, b, off)
+
+
+def test_evict_refuses_masses_that_share_rows():
+    at = places()
+    for off in (4, 99, 128 - 99, 127, 128 * 3 + 1):          # rows of 100 floats every 128
+        for sign in (1, -1):
+            assert refused("evict", **dict(at, mass_out=at["mass"] + 4 * off * sign)), off

@@ -158,3 +158,28 @@ def test_output_in_place_of_the_queries(Hq, Hkv, D, N, page):
         K().decode_sdpa(both[:one.numel()].view_as(one), x.k, x.v, x.scale, out=both[D:D + one.numel()].view_as(one), **args)
     assert K().launch_count() == launches
     K().device_status()
+
+
+def test_evict_between_masses_in_each_others_gaps():
+    """mass and mass_out as two columns of one array: rows of 50 every 128, 64 apart."""
+    from swiftlm_b200 import _lib
+    B, Hkv, D, N, budget = 3, 2, 64, 50, 20
+    x = Problem(B, Hkv, Hkv, 1, D, N, "bf16", 0, [50, 31, 7], seed=1, junk=2.0)
+    array = torch.rand(B, Hkv, 128, device="cuda")
+    before, mass = array.clone(), array[:, :, :N].contiguous()
+    k, v, lens = x.k.clone(), x.v.clone(), x.kv_len.clone()
+    want = torch.zeros_like(mass)
+    K().kv_evict(k, v, mass, lens, budget, 5, 2, mass_out=want)
+    out_lens = torch.zeros_like(x.kv_len)
+    L = _lib.lib()
+    need = L.dflash_kv_evict_workspace_bytes(B, Hkv, N, budget)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    _lib.check(L.dflash_kv_evict(x.k.data_ptr(), x.v.data_ptr(), None, x.kv_len.data_ptr(), array.data_ptr(), out_lens.data_ptr(),
+                                 array.data_ptr() + 4 * 64, None, ws.data_ptr(), need, B, Hkv, D, N, 0, 0, 0, 128, budget, 5, 2,
+                                 _lib.BF16, torch.cuda.current_stream().cuda_stream))
+    K().device_status()
+    assert torch.equal(x.k, k) and torch.equal(x.v, v) and torch.equal(out_lens, lens)
+    for b, n in enumerate([50, 31, 7]):
+        assert torch.equal(array[b, :, 64:64 + n], want[b, :, :n])
+        before[b, :, 64:64 + n] = array[b, :, 64:64 + n]
+    assert torch.equal(array, before)
