@@ -183,3 +183,102 @@ def test_evict_between_masses_in_each_others_gaps():
         assert torch.equal(array[b, :, 64:64 + n], want[b, :, :n])
         before[b, :, 64:64 + n] = array[b, :, 64:64 + n]
     assert torch.equal(array, before)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,D,N,page,window", [
+    (32, 16, 2, 64, 6000, 0, 0),          # a block of the joining kernel goes through several runs of 256 keys
+    (40, 20, 4, 128, 5000, 16, 3000),
+    (33, 40, 2, 64, 3000, 0, 0),          # the same with two groups of heads
+])
+def test_decode_weights_of_large_batches(B, Hq, Hkv, D, N, page, window):
+    lens = [(N * (3 + 5 * b % 17)) // 19 for b in range(B - 2)] + [0, N]
+    x = Problem(B, Hq, Hkv, 1, D, N, "bf16", page, lens, seed=B)
+    out, lse, mass = x.want(window, 7)
+    m = torch.zeros(B, Hkv, N if not page else x.table.shape[1] * page, device="cuda")
+    got, z = K().decode_sdpa(x.q[:, :, 0], x.k, x.v, x.scale, kv_len=x.kv_len, page_table=x.table, window=window, sinks=7, mass=m,
+                             return_lse=True)
+    K().device_status()
+    live = x.kv_len > 0
+    x.close(got[live], out[live, :, 0])
+    x.close_lse(z, lse[:, :, 0])
+    x.close_mass(m[:, :, :N], mass)
+
+
+# (sequence, unit of a row) pairs around 2048, the most whose costs the plan keeps in shared memory
+@pytest.mark.parametrize("B,T", [(682, 130), (1024, 70), (683, 130), (2300, 20)])
+def test_prompts_around_the_plans_table(B, T):
+    g = torch.Generator().manual_seed(B)
+    rows = torch.randint(0, T + 1, (B,), generator=g).tolist()
+    lens = [r + int(torch.randint(0, 11, (1,), generator=g)) for r in rows]
+    rows[-1] = lens[-1] = 0
+    x = Problem(B, 4, 1, T, 64, T + 10, "f16", 0, lens, rows, seed=B)  # units of 64 tokens
+    x.q[:, :] = x.q[:, :1]                                              # one head four times: a quarter of the oracle's work
+    y = Problem(B, 1, 1, T, 64, T + 10, "f16", 0, lens, rows, seed=B)
+    y.q, y.kd, y.vd = x.q[:, :1], x.kd, x.vd
+    want, want_lse, mass = y.want(17, 3)
+    got, z = K().prompt_sdpa(x.q, x.k, x.v, x.scale, q_len=x.q_len, kv_len=x.kv_len, window=17, sinks=3, return_lse=True,
+                             out=torch.zeros_like(x.q))
+    for h in range(4):
+        x.close(got[:, h:h + 1], want)
+        x.close_lse(z[:, h:h + 1], want_lse)
+    m = torch.zeros(B, 1, T + 10, device="cuda")
+    K().attention_mass(x.q, x.k, z, x.scale, m, q_len=x.q_len, kv_len=x.kv_len, window=17, sinks=3)
+    K().device_status()
+    assert ((m.double() - 4 * mass).abs() <= 4 * (4e-4 * mass + 1e-7) + 4e-4 * 4 * mass).all()      # the lse's error and the scores'
+
+
+@pytest.mark.parametrize("B,N", [(64, 8190), (70, 8000), (683, 700), (2049, 200)])
+def test_weights_around_the_plans_table(B, N):
+    g = torch.Generator().manual_seed(N)
+    lens = torch.randint(0, N + 1, (B,), generator=g).tolist()
+    lens[0], lens[1] = N, 0
+    rows = [min(3, n) for n in lens]
+    x = Problem(B, 1, 1, 3, 64, N, "bf16", 0, lens, rows, seed=B)
+    lse = x.want()[1].float()
+    want = x.want(lse_in=lse)[2]
+    m = torch.zeros(B, 1, N, device="cuda")
+    K().attention_mass(x.q, x.k, lse, x.scale, m, q_len=x.q_len, kv_len=x.kv_len)
+    K().device_status()
+    x.close_mass(m, want)
+
+
+@pytest.mark.parametrize("Hq,Hkv,T,D,N,page,window,sinks", [
+    (4, 1, 4100, 128, 4100, 0, 0, 0),                      # causal prompts of thousands of tokens
+    (4, 2, 4097, 64, 4200, 64, 0, 0),
+    (4, 1, 2500, 64, 5001, 0, 700, 64),
+    (2, 1, 2049, 256, 4000, 256, 0, 0),
+    (8, 2, 40, 128, 30000, 128, 0, 0),                     # a short turn over a long cache
+    (8, 2, 33, 256, 20011, 0, 0, 0),
+    (16, 2, 65, 64, 30001, 256, 0, 0),
+])
+def test_long_prompts_and_short_turns(Hq, Hkv, T, D, N, page, window, sinks):
+    x = Problem(1, Hq, Hkv, T, D, N, "bf16", page, seed=T + D)
+    args = dict(page_table=x.table, window=window, sinks=sinks, n_max=N)
+    want, want_lse, _ = x.want(window, sinks)
+    got, z = K().prompt_sdpa(x.q, x.k, x.v, x.scale, kv_len=x.kv_len, return_lse=True, **args)
+    x.close(got, want)
+    x.close_lse(z, want_lse)
+    m = torch.zeros(1, Hkv, N, device="cuda")
+    K().attention_mass(x.q, x.k, z, x.scale, m, kv_len=x.kv_len, **args)
+    K().device_status()
+    x.close_mass(m, x.want(window, sinks, lse_in=z)[2])
+
+
+@pytest.mark.parametrize("B,Hkv,D,N,page,budget", [(6, 2, 64, 9000, 32, 3000), (3, 1, 256, 20000, 0, 17000)])
+def test_evict_of_many_fp32_rows(B, Hkv, D, N, page, budget):
+    from tests.test_gpu_cache_attention import TYPES, evict_reference
+    TYPES.setdefault("f32", torch.float32)
+    x = Problem(B, Hkv, Hkv, 1, D, N, "f32", page, [N - 500 * b for b in range(B)], seed=N, junk=2.0)
+    mass = torch.randint(0, 200, (B, Hkv, N if not page else x.table.shape[1] * page), device="cuda").float()     # many ties
+    places = evict_reference(x, mass.cpu(), budget, 600, 4)
+    kept = torch.empty(B, Hkv, budget, dtype=torch.int32, device="cuda")
+    K().kv_evict(x.k, x.v, mass, x.kv_len, budget, 600, 4, page_table=x.table, kept=kept)
+    K().device_status()
+    at = torch.arange(budget, device="cuda")
+    for b in range(B):
+        for h in range(Hkv):
+            p = places[b * Hkv + h]
+            assert kept[b, h].tolist() == p
+            for pool, dense in ((x.k, x.kd), (x.v, x.vd)):
+                rows = pool[b, h, :budget] if not page else pool[x.table[b, at // page].long(), h, at % page]
+                assert torch.equal(rows, dense[b, h, p])
