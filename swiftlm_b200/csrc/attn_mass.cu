@@ -14,9 +14,10 @@
 // are cut into equal ranges per CTA (ranges.cuh); pieces of a cut unit leave 256 sums in the workspace, added in order by
 // mass_join_kernel: the order of every sum is fixed.
 //
-// Measured (B200, the whole call): 2048 rows of 32 / 8 heads over 16384 tokens, D = 128, 0.38 ms = 0.68 PFLOP/s; 1.0e9
-// exponentials take 0.24 ms at 16 a clock and SM.  16 rows of 32 sequences of 1.4 to 4.1 thousand tokens, D = 256: 36 us, the 94 MB
-// take 14 at the HBM's rate; the plan and the start of the CTAs are behind most of the rest.
+// Measured (B200, the whole call): 2048 rows of 32 / 8 heads over 16384 tokens, D = 128, 0.385 ms = 0.67 PFLOP/s; 1.0e9
+// exponentials take 0.24 ms at 16 a clock and SM.  16 rows of 32 sequences of 1.4 to 4.1 thousand tokens, D = 256: 35 us, the 94 MB
+// take 14 at the HBM's rate; the plan and the start of the CTAs are behind most of the rest.  2048 rows of 16 / 2 heads over 16384
+// tokens, D = 256, 0.31 ms = 0.82 PFLOP/s: its ring holds one query tile, whose successor loads when the last product has read it.
 #include "ranges.cuh"
 #include "tc_common.cuh"
 

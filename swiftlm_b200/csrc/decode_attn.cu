@@ -1,7 +1,8 @@
 // Attention of one new token per sequence over the KV cache: out = softmax(scale q K^T over the visible tokens) V.
 //
-// Every visible key and value is read once and used by the G query heads of its KV head: 4 G operations a byte, far below
-// what the tensor cores need to be busy, so the kernel is built to keep HBM reads in flight and nothing else.  (On the CUDA
+// Every visible key and value is read once and used by the G query heads of its KV head (more than 16 of them: once for every
+// group of 16, each group's units a pass of their own): G operations a byte, far below what the tensor cores need to be busy, so
+// the kernel is built to keep HBM reads in flight and nothing else.  (On the CUDA
 // cores G = 8 would take 4096 fused multiply-adds per kilobyte, which is 0.8 of the fp32 rate at full HBM speed; as
 // warp-level matrix products it is some 200 issue slots per 16 keys.)
 //
@@ -20,14 +21,15 @@
 //   first, mma_sync.cuh).
 // * A unit that one CTA covers is normalised and written at once; the others leave (O, maximum, sum) in the workspace
 //   and decode_finish_kernel, chained by a programmatic launch, joins them in a fixed order.
-// * With `mass`, the scaled scores of the visible tokens are kept (4 bytes per head and key, 3 % of the bytes read at
-//   D = 256, G = 8) and decode_finish_kernel turns them into weights when every head's sum is known: reading K a second
-//   time would cost sixteen times as much.
+// * With `mass`, the scaled scores of the visible tokens are kept and decode_finish_kernel turns them into weights when every
+//   head's sum is known.  A key has 4 bytes for each of 8 or 16 heads, whether there are as many or not: written and read
+//   again, 6 % of the bytes of K and V at D = 256 and up to 8 heads, where reading K again would be half of them; 25 % at
+//   D = 64, however few the heads.
 //
 // Measured (B200, the whole call; of the 6.57 TB/s that a copy reaches): 8 sequences of 34 to 102 thousand tokens at D = 256
-// 189 us (0.94); 32 of 3 to 8 thousand with weights 78 us (0.71: the main kernel is at 0.86, the rest is the second launch and
-// the scores); 64 sequences x 8 KV heads at D = 128 with a window of 1024 and 64 sinks 58 us (0.75); one sequence of
-// 517 tokens 18 us, bound by the host (12 us of kernels).
+// 175 to 189 us, from card to card (1.02 to 0.94); 32 of 3 to 8 thousand with weights 78 us (0.71: the main kernel takes 63, the
+// second 14); 64 sequences x 8 KV heads at D = 128 with a window of 1024 and 64 sinks 58 us (0.75); one sequence of
+// 517 tokens 18 us, bound by the host (12 us of kernels, 6 and 5.5).
 #include <type_traits>
 
 #include "cache_ops.cuh"
@@ -643,7 +645,9 @@ int32_t launch_typed(const CacheArgs& a, const Plan& t, cudaStream_t stream) {
     const int heads = t.G < 8 * NT ? t.G : 8 * NT;
     p.heads = units >= grid / 4 ? heads : 1;
     const long long x = units * ((heads + p.heads - 1) / p.heads), blocks = 1 + (a.mass ? ((long long)t.max_chunks * 16 + kFinishThreads - 1) / kFinishThreads : 0);
-    // enough blocks for the mass to fill the GPU once: each finds the log-sum-exps for itself
+    // Rows of blocks for the mass: six blocks an SM in all, as each finds the log-sum-exps for itself.  Of a row, one block a
+    // (sequence, KV head) works, the first of its head blocks; the others return.  With a block a head (few units, long
+    // caches) those that work are fewer by the number of heads: 112 for one sequence with 2 KV heads of 8 query heads each.
     const long long once = 1 + (6 * (long long)sm_count() + x - 1) / x;
     const unsigned y = (unsigned)(blocks < once ? blocks : (once < 65535 ? once : 65535));
     DFLASH_CUDA_CHECK(launch_chained(decode_finish_kernel<T, D, NT>, dim3((unsigned)x, y), kFinishThreads, p, stream));

@@ -15,8 +15,8 @@
 // in front of which the stores of this chunk end: the next chunk's loads are in flight while this one is stored, and one
 // barrier a chunk is enough.  Bound by HBM: every row that moves is read once and written once.
 //
-// Measured (B200, the whole call): 32 sequences x 2 heads from 1104 to 1088 tokens (135 MB) 41 us, selection 11 and move 26 (20.6
-// at the HBM's rate); 8 x 2 heads from up to 32768 to 4096 53 us, selection 22 and move 27.  (With masses read once a digit, a
+// Measured (B200, the whole call; fp32 rows of as many bytes take the same): 32 sequences x 2 heads from 1104 to 1088 tokens
+// (135 MB) 41 us, selection 11 and move 26 (20.6 at the HBM's rate); 8 x 2 heads from up to 32768 to 4096 53 us, selection 22 and move 27.  (With masses read once a digit, a
 // second meeting a digit and places written by the threads that found them: 43 and 60 us.)
 #include "cache_ops.cuh"
 #include "ptx.cuh"
@@ -271,8 +271,9 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParam
   meet();                                                 // no CTA leaves while another reads its shared memory
 }
 
-// Rows a thread has in flight in one chunk, with 64 bytes of a row a CTA.  Measured at 32 x 1104 tokens and 8 x 32768 (whole
-// call): 2 rows 35 and 73 us, 4 rows 34 and 61, 8 rows 39 and 75; 32 bytes a CTA 41 and 67, 128 bytes 34 and 70.
+// Rows a thread has in flight in one chunk, with 64 bytes of a row a CTA (`vecs` below).  Measured, the whole call, at 32 x 2
+// heads from 1104 to 1088 tokens, 8 x 2 from up to 32768 to 4096 (512-byte rows both) and 8 x 8 from up to 4000 to 2000 (128-byte
+// rows): 4 rows 41, 53 and 29 us, 2 rows 39, 65 and 34, 8 rows 46, 68 and 35; 32 bytes a CTA 45, 61 and 33, 128 bytes 41, 63 and 35.
 constexpr int kMoveThreads = 256, kMoveRows = 4;
 // One CTA: `vecs` 16-byte columns from vecs * blockIdx.x on, of K (z = 0) or V (z = 1) of one (b, h).
 __global__ void __launch_bounds__(kMoveThreads) move_kernel(const EvictParams p, int vecs) {

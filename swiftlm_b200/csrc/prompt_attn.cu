@@ -22,10 +22,11 @@
 //   lengths, causal triangles and few query rows over a long cache all fill the GPU.  A unit cut in pieces leaves (O, m, l) per piece in the workspace and
 //   join_kernel adds them up in order.
 //
-// Measured (B200, the whole call): 16 query / 2 KV heads, D = 256, a prompt of 8192 0.47 ms = 1.18 PFLOP/s (0.72 of what cuBLAS
-// reaches in a burst, 0.84 of what it sustains under the power cap), a chunk of 2048 over 10240 tokens 0.26 ms (0.72); a key
+// Measured (B200, the whole call): 16 query / 2 KV heads, D = 256, a prompt of 8192 0.46 ms = 1.19 PFLOP/s (0.73 of what cuBLAS
+// reaches in a burst, 0.85 of what it sustains under the power cap), a chunk of 2048 over 10240 tokens 0.26 ms (0.73), 48 rows
+// over 32768 0.057 ms; a key
 // tile takes 2670 clocks, 2048 of them on the tensor pipe.  32 / 8 heads, D = 128, two prompts of 8192 with a window of 1024:
-// 0.42 ms (0.40): 4300 clocks for the two tiles' 2048 of products and 2048 of exponentials, the softmax threads' waits
+// 0.41 ms (0.41; a causal prompt of 8192 0.65 ms = 0.52, at D = 64 0.51 ms = 0.33): 4300 clocks for the two tiles' 2048 of products and 2048 of exponentials, the softmax threads' waits
 // (tensor-memory loads and stores, the other half's maximum, the hand-over of P) are most of the rest.  Five prompts of up to 193:
 // 23 us, three launches' latency.
 #include "ranges.cuh"
